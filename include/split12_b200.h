@@ -254,7 +254,8 @@ int s12_version(void);
  * streaming GEMV's copy, consumer, reduction and epilogue waits, 0x10-0x4000
  * the tensor-core GEMM's roles, 0x8000 a peer wait of the all-reduce,
  * 0x10000-0x80000 the streaming small-batch kernel's weight copies,
- * activation copies, consumers and epilogue / hand-over), including
+ * activation copies, consumers and epilogue / hand-over; 0x100000 is no wait
+ * but a page of a paged cache that a block table does not have), including
  * the word of s12_gemm_noalloc_async.  When it was non-zero the GEMM's
  * hand-over counters are zeroed again, so later launches start clean.
  * Synchronises the device. */
@@ -454,6 +455,73 @@ int s12_rope_store_kv_batch(float* q, float* k, const float* v, int8_t* kv_k, in
                             float* kv_scale_k, float* kv_scale_v, const int* positions, int head_dim,
                             int n_head, int n_head_kv, long long kv_stride, float theta, int batch_size,
                             void* stream);
+
+/* --------------------------------------------------------------------------
+ * A paged INT8 KV cache: sequences of different lengths share one pool of pages
+ * --------------------------------------------------------------------------
+ * No counterpart in the reference, which has one contiguous cache and runs a
+ * prompt as decode steps.  Position t of sequence s lies in page
+ * block_table[s * table_stride + t / page_size], row t % page_size; one table
+ * serves all layers.  A (position, kv head) is head_dim int8 codes and one fp32
+ * scale = absmax / 127, as in the contiguous cache.  Pages are head-major. */
+typedef struct S12PagedKv {
+    int8_t* k;                  /* [num_pages][n_head_kv][page_size][head_dim], 16-byte aligned, as the other three */
+    int8_t* v;
+    float*  scale_k;            /* [num_pages][n_head_kv][page_size] */
+    float*  scale_v;
+    int num_pages;
+    int page_size;              /* a power of two from 16 to 1024 */
+    int n_head_kv;
+    int head_dim;               /* a multiple of 4 up to 256 */
+} S12PagedKv;
+/* The packed new tokens of num_seqs sequences: rows [q_start[s], q_start[s+1])
+ * of q / k / v / out are sequence s's LAST positions, kv_len[s] counts them in.
+ * q_start null: one token per sequence (num_tokens == num_seqs).  Rows behind
+ * q_start[num_seqs] are not read and left as they were.  The three arrays are
+ * device int32, so a captured graph serves later steps; the rest is the host's.
+ * num_tokens, max_new and max_len are bounds that hold for every replay: rows,
+ * new tokens of one sequence, positions of one sequence. */
+typedef struct S12PagedBatch {
+    const int32_t* block_table; /* [num_seqs][table_stride], table_pages entries of a row in use */
+    const int32_t* kv_len;      /* [num_seqs] */
+    const int32_t* q_start;     /* [num_seqs + 1], ascending, or null */
+    int num_seqs;
+    int table_stride;
+    int table_pages;
+    int num_tokens;
+    int max_new;
+    int max_len;
+} S12PagedBatch;
+/* RoPE of q into q_out (which may be q), RoPE of k, INT8 store of k and v at the
+ * tokens' positions, one launch.  k and v are left as they were (kv_stride:
+ * floats between their rows).  Angles, k's rotation and the codes are computed
+ * in 64 bits.  A position whose page the table does not have (an entry outside
+ * [0, num_pages), a position past the table) is not stored and sets bit 0x100000
+ * of the device status word; tokens before position 0 (a batch row that holds no
+ * sequence: kv_len 0) are not stored.  A NaN or an infinity in a row of k or v
+ * makes the row's scale one. */
+int s12_rope_store_kv_paged_async(const float* q, int q_stride, const float* k, const float* v, int kv_stride,
+                                  float* q_out, int q_out_stride, const S12PagedKv* kv, const S12PagedBatch* batch,
+                                  int n_head, float theta, void* stream);
+/* Causal attention of the new tokens over the pages, grouped heads (n_head a
+ * multiple of n_head_kv): out[row][head] = sum_j softmax_j(scale * q . k_j) v_j
+ * over the positions j up to the row's own; bf16 [num_tokens][out_stride].
+ * Rows without a position (kv_len below the token's) give 0.  Positions whose
+ * page the table does not have count as masked and set bit 0x100000.
+ * workspace: s12_attention_paged_workspace_bytes of device memory, 16-byte
+ * aligned, zero before its first use; a call leaves it fit for the next.  Calls
+ * that may overlap on the GPU need workspaces of their own. */
+int64_t s12_attention_paged_workspace_bytes(int n_head, int n_head_kv, int head_dim, int num_seqs, int max_new);
+int s12_attention_paged_async(const float* q, int q_stride, const S12PagedKv* kv, const S12PagedBatch* batch,
+                              void* out_bf16, int out_stride, int n_head, float scale, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+/* Copies pages src[i] to dst[i] (device int32 [count]) in every layer; the
+ * layers of each array follow one another (num_pages pages apart).  The dst
+ * pages must differ from one another and from all src pages.  An index outside
+ * the pool skips its copy and sets bit 0x100000.  Forks a sequence (its last,
+ * partly filled page), compacts a pool (pages above a line into free ones). */
+int s12_copy_pages_async(const S12PagedKv* kv, int layers, const int32_t* src, const int32_t* dst, int count,
+                         void* stream);
 
 /* --------------------------------------------------------------------------
  * Tensor parallelism: all-reduce after the row-parallel projections

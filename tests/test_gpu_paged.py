@@ -1,0 +1,267 @@
+"""The paged INT8 cache's operators against 64 bits (paged_oracle.py derives the bounds)."""
+import math
+
+import pytest
+import torch
+
+import paged_oracle as PO
+
+pytestmark = pytest.mark.gpu
+
+KINDS = {
+    "one_token": [(0, 1)],
+    "decode": [(n - 1, 1) for n in (1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 200, 1000)],
+    "long_decode": [(9000, 1), (4095, 1), (0, 1)],
+    "prompt": [(0, 150)],
+    "tile_ends": [(0, n) for n in (31, 32, 33, 63, 64, 65)] + [(0, n) for n in (127, 128, 129)],
+    "ragged": [(0, 7), (0, 0), (130, 5), (0, 1), (3, 261), (0, 0)],
+    "chunks": [(1000, 3), (64, 64), (77, 200)],
+}
+SHAPES = [(32, 8, 128), (8, 8, 128), (8, 1, 128), (6, 2, 128), (10, 2, 64), (16, 1, 96), (4, 2, 64), (40, 2, 128), (2, 2, 20), (4, 2, 80), (2, 1, 256)]
+
+
+def run_attention(c, scale, q=None, out=None, workspace=None, table=None):
+    from turbo_lossless_b200 import Split12Engine
+    e = Split12Engine()
+    if out is None:
+        out = torch.full((c.q.shape[0], c.n_head * c.hd), 0x5A5A, dtype=torch.int16, device="cuda")
+    q_start = None if all(n == 1 for _, n in c.lens) and c.q.shape[0] == c.tokens else c.q_start
+    e.attention_paged(c.q if q is None else q, *c.cache(), out, c.table if table is None else table, c.kv_len, q_start, c.n_head, scale,
+                      c.max_new, c.max_len, workspace)
+    torch.cuda.synchronize()
+    return out, e.device_status()
+
+
+def check(out, want, bound):
+    got = out.view(torch.bfloat16).double()
+    assert torch.isfinite(got).all()
+    over = ((got - want).abs() - bound).max().item()
+    assert over <= 0, f"{over} above the bound"
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd", SHAPES)
+@pytest.mark.parametrize("kind", sorted(KINDS))
+def test_attention_against_64_bits(kind, n_head, n_kv, hd):
+    page = 16 << (len(kind) + n_head) % 4
+    c = PO.Case(KINDS[kind], n_head, n_kv, hd, page, seed=7)
+    out, status = run_attention(c, hd ** -0.5)
+    assert status == 0
+    check(out, *PO.attention(c, hd ** -0.5))
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256, 1024])
+def test_attention_over_every_page_size(page):
+    for lens in ([(0, 300), (500, 40)], [(700, 1), (31, 1), (1023, 1)]):
+        c = PO.Case(lens, 16, 4, 128, page, seed=page)
+        out, status = run_attention(c, 0.1)
+        assert status == 0
+        check(out, *PO.attention(c, 0.1))
+
+
+@pytest.mark.parametrize("lens", [[(5, 1), (90, 1)], [(5, 30), (90, 170)]])
+def test_rows_with_strides_and_rows_behind_the_last_sequence(lens):
+    c = PO.Case(lens, 8, 2, 128, 32, seed=1, spare_rows=9)
+    wide = torch.full((c.q.shape[0], c.q.shape[1] + 24), math.nan, device="cuda")
+    wide[:, :c.q.shape[1]] = c.q
+    wide[c.tokens:] = math.nan
+    out = torch.full((c.q.shape[0], c.q.shape[1] + 40), 77, dtype=torch.int16, device="cuda")
+    run_attention(c, 0.09, q=wide[:, :c.q.shape[1]], out=out[:, :c.q.shape[1]])
+    check(out[:c.tokens, :c.q.shape[1]].contiguous(), *PO.attention(c, 0.09))
+    assert (out[c.tokens:] == 77).all() and (out[:, c.q.shape[1]:] == 77).all()
+
+
+@pytest.mark.parametrize("hd", [128, 80])
+@pytest.mark.parametrize("lens", [[(200, 1), (70, 1)], [(100, 100), (70, 3)]])
+def test_sequences_that_hold_nothing_give_zeros(lens, hd):
+    c = PO.Case(lens + [(0, lens[0][1])], 8, 2, hd, 16, seed=2)
+    c.kv_len[2] = 0                                                   # its tokens come before position 0
+    out, status = run_attention(c, 0.1)
+    assert status == 0
+    n = c.tokens - lens[0][1]
+    assert (out[n:] == 0).all()
+    c.lens = c.lens[:2]
+    c.tokens = n
+    check(out[:n], *PO.attention(c, 0.1))
+
+
+@pytest.mark.parametrize("hd", [128, 80])
+@pytest.mark.parametrize("lens", [[(400, 1), (70, 1)], [(200, 100), (70, 3)]])
+def test_pages_that_the_table_lacks_are_masked_and_reported(lens, hd):
+    c = PO.Case(lens, 8, 2, hd, 64, seed=3)
+    want = PO.attention(c, 0.1, absent=[(0, 1), (0, 3), (1, 0)])
+    c.table[0, 1], c.table[0, 3], c.table[1, 0] = -1, c.codes[0].shape[0], 1 << 30
+    out, status = run_attention(c, 0.1)
+    assert status == 0x100000
+    check(out, *want)
+
+
+@pytest.mark.parametrize("lens", [[(300, 1)], [(100, 200)]])
+def test_sizes_of_values_and_scores(lens):
+    """Scales over 30 binary orders, one score far above the others, q of a row with one large element."""
+    c = PO.Case(lens, 8, 2, 128, 64, seed=4)
+    t = torch.arange(sum(lens[0]), device="cuda")
+    c.scales[1][c.table[0].long()[t // 64], :, t % 64] *= torch.exp2((t % 31 - 15).float())[:, None]
+    c.q[:, 5] *= 40
+    c.codes[0][c.table[0, 0].long(), :, 3] = 127
+    out, _ = run_attention(c, 0.1)
+    check(out, *PO.attention(c, 0.1))
+
+
+@pytest.mark.parametrize("lens", [[(300, 1), (20, 1)], [(100, 200), (20, 30)]])
+@pytest.mark.parametrize("what", ["q", "scale_k", "scale_v"])
+def test_a_nan_stays_with_the_rows_that_use_it(lens, what):
+    c = PO.Case(lens, 8, 2, 128, 32, seed=5)
+    want, bound = PO.attention(c, 0.1)
+    if what == "q":
+        c.q[0, 2 * 128 + 3] = math.nan
+        hit = [(0, 2)]
+    else:
+        c.scales[what == "scale_v"][c.table[0, 0].long(), 1, 9] = math.nan
+        hit = [(r, h) for r in range(lens[0][1]) for h in range(4, 8)]
+    out, _ = run_attention(c, 0.1)
+    got = out.view(torch.bfloat16).double().view(c.tokens, 8, 128)
+    touched = torch.zeros(c.tokens, 8, dtype=torch.bool, device="cuda")
+    for r, h in hit:
+        touched[r, h] = True
+    assert torch.isnan(got[touched]).any(-1).all()
+    check(out.view(c.tokens, 8, 128)[~touched], want.view(c.tokens, 8, 128)[~touched], bound.view(c.tokens, 8, 128)[~touched])
+
+
+@pytest.mark.parametrize("lens", [[(300, 1), (20, 1), (4000, 1)], [(100, 200), (20, 30)]])
+def test_a_captured_call_follows_the_lengths_and_repeats_its_bits(lens):
+    from turbo_lossless_b200 import Split12Engine
+    c = PO.Case(lens, 16, 4, 128, 64, seed=6)
+    e = Split12Engine()
+    out = torch.zeros(c.tokens, 16 * 128, dtype=torch.int16, device="cuda")
+    ws = e.attention_paged_workspace(16, 4, 128, len(lens), c.max_new)
+    q_start = None if c.max_new == 1 else c.q_start
+    args = (c.q, *c.cache(), out, c.table, c.kv_len, q_start, 16, 0.1, c.max_new, c.max_len, ws)
+    e.attention_paged(*args)
+    torch.cuda.synchronize()
+    first = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        e.attention_paged(*args)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
+    c.lens = [(b // 2, n) for b, n in lens]
+    c.kv_len.copy_(torch.tensor([b + n for b, n in c.lens], dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    check(out, *PO.attention(c, 0.1))
+
+
+STORES = [("decode", 32, 8, 128), ("ragged", 6, 2, 128), ("prompt", 4, 4, 64), ("tile_ends", 16, 1, 96), ("chunks", 2, 2, 20), ("chunks", 3, 1, 256),
+          ("long_decode", 8, 1, 80), ("one_token", 32, 8, 128)]
+
+
+@pytest.mark.parametrize("kind,n_head,n_kv,hd", STORES)
+def test_store_against_64_bits(kind, n_head, n_kv, hd):
+    """Codes and scales are the exact ones; q is off by the rounding of cos, sin, two products and a sum: 5 * 2^-24 of the
+    pair's size."""
+    from turbo_lossless_b200 import Split12Engine
+    c = PO.Case(KINDS[kind], n_head, n_kv, hd, 16 << n_head % 4, seed=11, spare_rows=3)
+    c.k[:c.tokens // 2, :hd] *= 1000
+    c.v[0] = 0
+    q, k, v = c.q.clone(), c.k.clone(), c.v.clone()
+    want_q, codes, scales = PO.store(c, 500000.0)
+    e = Split12Engine()
+    e.rope_store_kv_paged(c.q, c.k, c.v, *c.cache(), c.table, c.kv_len, c.q_start, n_head, 500000.0)
+    torch.cuda.synchronize()
+    assert e.device_status() == 0
+    assert torch.equal(c.k, k) and torch.equal(c.v, v) and torch.equal(c.q[c.tokens:], q[c.tokens:])
+    pair = q[:c.tokens].double().view(c.tokens, n_head, 2, hd // 2)
+    size = (pair[:, :, 0].square() + pair[:, :, 1].square()).sqrt().repeat(1, 1, 2).view(c.tokens, -1)
+    assert ((c.q[:c.tokens].double() - want_q).abs() <= 5 * 2.0 ** -24 * math.sqrt(2) * size).all()
+    for j in (0, 1):
+        assert torch.equal(c.codes[j], codes[j])
+        assert torch.equal(c.scales[j].nan_to_num(-1), scales[j].nan_to_num(-1))
+
+
+def test_store_keeps_other_buffers_and_reports_missing_pages():
+    from turbo_lossless_b200 import Split12Engine
+    c = PO.Case([(10, 60), (0, 5), (3, 2)], 8, 2, 64, 16, seed=12)
+    c.table[0, 2] = -1
+    c.table[1, 0] = c.codes[0].shape[0]
+    c.kv_len[2] = 0                                                   # rows that hold no sequence: no error, no store
+    want_q, codes, scales = PO.store(c.__class__([(10, 60), (0, 5), (3, 2)], 8, 2, 64, 16, seed=12), 10000.0)
+    fused = torch.zeros(c.tokens, 8 * 64 + 4 * 64, device="cuda")     # q, k, v side by side, as one projection gives them
+    fused[:, :512], fused[:, 512:640], fused[:, 640:] = c.q, c.k, c.v
+    before = [x.clone() for x in c.cache()]
+    keep, q_out = fused.clone(), torch.zeros(c.tokens, 512, device="cuda")
+    e = Split12Engine()
+    e.rope_store_kv_paged(fused[:, :512], fused[:, 512:640], fused[:, 640:], *c.cache(), c.table, c.kv_len, c.q_start, 8, 10000.0, q_out=q_out)
+    torch.cuda.synchronize()
+    assert e.device_status() == 0x100000 and torch.equal(fused, keep)
+    for x, b, w in zip(c.cache(), before, (*codes, *scales)):
+        for t in range(10, 70):
+            page = int(c.table[0, t // 16])
+            if page >= 0:
+                assert torch.equal(x[page, :, t % 16], w[page, :, t % 16])
+                b[page, :, t % 16] = x[page, :, t % 16]
+        assert torch.equal(x.nan_to_num(-1), b.nan_to_num(-1)) if x.is_floating_point() else torch.equal(x, b)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_value_that_is_not_finite_marks_its_row(bad):
+    from turbo_lossless_b200 import Split12Engine
+    c = PO.Case([(0, 4)], 4, 2, 128, 16, seed=13)
+    _, _, scales = PO.store(c, 10000.0)
+    c.k[1, 7], c.v[2, 128 + 5] = bad, bad
+    Split12Engine().rope_store_kv_paged(c.q, c.k, c.v, *c.cache(), c.table, c.kv_len, c.q_start, 4, 10000.0)
+    page = c.table[0, 0].long()
+    for j, row, head in ((0, 1, 0), (1, 2, 1)):
+        got, want = c.scales[j][page, :, :4].clone(), scales[j][page, :, :4].clone()
+        assert not torch.isfinite(got[head, row])
+        got[head, row] = want[head, row] = 0
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("layers,pages,n_kv,page,hd,count", [(1, 5, 1, 16, 4, 1), (3, 40, 2, 32, 96, 17), (2, 9, 8, 64, 128, 4), (5, 7, 3, 16, 20, 2), (1, 300, 1, 16, 64, 150)])
+def test_copy_pages(layers, pages, n_kv, page, hd, count):
+    from turbo_lossless_b200 import Split12Engine
+    g = torch.Generator(device="cuda").manual_seed(count)
+    shape = (layers, pages, n_kv, page)
+    kv = [torch.randint(-128, 128, (*shape, hd), dtype=torch.int8, device="cuda", generator=g) for _ in "kv"]
+    sc = [torch.randn(shape, device="cuda", generator=g) for _ in "kv"]
+    order = torch.randperm(pages, device="cuda", generator=g).to(torch.int32)
+    src, dst = order[:count].clone(), order[count:2 * count].clone()
+    want = [x.clone() for x in (*kv, *sc)]
+    status = 0
+    if count > 3:
+        src[1] = src[0]                                               # one source twice
+    for i in range(count):
+        if count > 3 and i == 2:                                      # one copy that is skipped
+            src[i], status = pages, 0x100000
+            continue
+        for x in want:
+            x[:, dst[i]] = x[:, src[i]]
+    e = Split12Engine()
+    e.copy_pages(*kv, *sc, src, dst)
+    torch.cuda.synchronize()
+    assert e.device_status() == status
+    for x, w in zip((*kv, *sc), want):
+        assert torch.equal(x, w)
+    e.copy_pages(*kv, *sc, src[:0], dst[:0])                          # nothing to do
+
+
+def test_wrappers_refuse_what_the_kernels_cannot_take():
+    from turbo_lossless_b200 import S12Error, Split12Engine
+    c = PO.Case([(0, 4), (3, 2)], 4, 2, 128, 16, seed=14)
+    e = Split12Engine()
+    out = torch.zeros(c.tokens, 512, dtype=torch.int16, device="cuda")
+    ok = dict(q=c.q, kv_k=c.codes[0], kv_v=c.codes[1], scale_k=c.scales[0], scale_v=c.scales[1], out_bf16=out, block_table=c.table,
+              kv_len=c.kv_len, q_start=c.q_start, n_head=4, scale=0.1, max_new=4, max_len=5)
+    e.attention_paged(**ok)
+    for edit in (dict(q=c.q.double()), dict(q=c.q[:, :500]), dict(q=c.q.t()), dict(q=c.q.cpu()), dict(kv_k=c.codes[0].cpu()), dict(kv_v=c.codes[1][1:]),
+                 dict(scale_k=c.scales[0].double()), dict(kv_k=c.codes[0].transpose(1, 2), kv_v=c.codes[1].transpose(1, 2)), dict(out_bf16=out[:3]),
+                 dict(out_bf16=out.view(torch.bfloat16)), dict(block_table=c.table.long()), dict(block_table=c.table[:1]), dict(kv_len=c.kv_len.cpu()),
+                 dict(q_start=c.q_start[:2]), dict(q_start=c.q_start.long()), dict(block_table=c.table.t().contiguous().t())):
+        with pytest.raises(ValueError):
+            e.attention_paged(**{**ok, **edit})
+    for edit in (dict(q_start=None), dict(n_head=3), dict(max_new=0), dict(max_len=0), dict(n_head=0)):
+        with pytest.raises(S12Error):
+            e.attention_paged(**{**ok, **edit})

@@ -25,6 +25,18 @@ class S12PatchBatchDesc(C.Structure):
                 ("patch_wrong", _vp), ("activations", _vp), ("output", _vp), ("M", _i)]
 
 
+class S12PagedKv(C.Structure):
+    """Mirror of the C struct S12PagedKv (device pointers of one layer's paged cache)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("scale_k", _vp), ("scale_v", _vp), ("num_pages", _i), ("page_size", _i),
+                ("n_head_kv", _i), ("head_dim", _i)]
+
+
+class S12PagedBatch(C.Structure):
+    """Mirror of the C struct S12PagedBatch (packed new tokens over a paged cache)."""
+    _fields_ = [("block_table", _vp), ("kv_len", _vp), ("q_start", _vp), ("num_seqs", _i), ("table_stride", _i),
+                ("table_pages", _i), ("num_tokens", _i), ("max_new", _i), ("max_len", _i)]
+
+
 # name -> (restype, argtypes); every symbol include/split12_b200.h declares
 SIGNATURES = {
     "nv_launch_split12_v2_async": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _vp]),
@@ -84,6 +96,10 @@ SIGNATURES = {
     "launch_flash_attention_batch": (_i, [_vp] * 7 + [_i, _i, _i, _i, C.c_float, _i, _i, _vp]),
     "s12_store_kv_batch": (_i, [_vp] * 7 + [_i, _i, C.c_longlong, _i, _vp]),
     "s12_rope_store_kv_batch": (_i, [_vp] * 8 + [_i, _i, _i, C.c_longlong, C.c_float, _i, _vp]),
+    "s12_rope_store_kv_paged_async": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, C.POINTER(S12PagedKv), C.POINTER(S12PagedBatch), _i, C.c_float, _vp]),
+    "s12_attention_paged_workspace_bytes": (C.c_int64, [_i] * 5),
+    "s12_attention_paged_async": (_i, [_vp, _i, C.POINTER(S12PagedKv), C.POINTER(S12PagedBatch), _vp, _i, _i, C.c_float, _vp, C.c_int64, _vp]),
+    "s12_copy_pages_async": (_i, [C.POINTER(S12PagedKv), _i, _vp, _vp, _i, _vp]),
     "s12_comm_handle_bytes": (_i, []),
     "s12_comm_create": (_i, [_i, _i, C.c_longlong, C.POINTER(_vp), _vp]),
     "s12_comm_connect": (_i, [_vp, _vp]),
