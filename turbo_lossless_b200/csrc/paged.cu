@@ -313,7 +313,8 @@ int64_t s12_attention_paged_workspace_bytes(int n_head, int n_head_kv, int head_
 {
     if (n_head < 1 || n_head_kv < 1 || head_dim < 1 || num_seqs < 1 || max_new < 1)
         return fail(S12_ERR_BAD_ARG, "s12_attention_paged_workspace_bytes: sizes must be positive");
-    return 0;
+    if (n_head % n_head_kv) return fail(S12_ERR_UNSUPPORTED, "s12_attention_paged_workspace_bytes: n_head is not a multiple of n_head_kv");
+    return paged_decode_workspace_bytes(n_head, n_head_kv, num_seqs, max_new);
 }
 
 int s12_attention_paged_async(const float* q, int q_stride, const S12PagedKv* kv, const S12PagedBatch* batch, void* out_bf16,
@@ -330,6 +331,7 @@ int s12_attention_paged_async(const float* q, int q_stride, const S12PagedKv* kv
     if ((rc = paged_status(P.c, who)) != S12_OK) return rc;
     P.q = q; P.out = (int16_t*)out_bf16; P.q_stride = q_stride; P.out_stride = out_stride; P.n_head = n_head; P.scale = scale;
     P.max_new = batch->max_new; P.max_len = batch->max_len; P.workspace = workspace; P.workspace_bytes = workspace_bytes;
+    if ((rc = paged_decode_launch(P, stream, who)) <= 0) return rc;
     return launch(paged_attention_general_kernel, dim3(batch->num_tokens, n_head), dim3(kGenWarps * 32), 0, stream, who, P);
 }
 

@@ -73,5 +73,7 @@ struct PagedAttn {
     int max_new, max_len;       // the caller's bounds: new tokens and positions of a sequence
     void* workspace; int64_t workspace_bytes;
 };
+int64_t paged_decode_workspace_bytes(int n_head, int n_head_kv, int num_seqs, int max_new);
+int paged_decode_launch(const PagedAttn& A, void* stream, const char* who);
 
 }  // namespace s12
