@@ -13,10 +13,10 @@
 //             are the A operand of the second product as they lie, against V's rows in order
 //   dims      column n of PV tile j is dim n * head_dim / 8 + j: a lane reads consecutive bytes of each of eight rows
 //             and turns them by byte permutes
-// Work is cut by the device, which alone knows the lengths: the units of 128 positions of all (sequence, kv head, rows)
-// items follow one another and every CTA takes an equal range; ends within an eighth of a range of an item's end move
-// there.  An item of several CTAs leaves its partial results in the workspace, and the CTA that comes last adds them in
-// order, so that the result does not depend on who came when.
+// Work is cut by the device, which alone knows the lengths: the units of all (sequence, kv head, rows) items follow one
+// another and every team of warps takes an equal range; ends within an eighth of a range of an item's end move there.  An
+// item of several teams leaves its partial results in the workspace; of 16 neighbouring parts the team that comes last adds
+// them in order, and of these sums the last again, so that the result does not depend on who came when.
 #include "paged.cuh"
 #include <algorithm>
 #include <atomic>
@@ -26,24 +26,25 @@ namespace s12 {
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecChunk = 32;                       // positions of a warp's step
-constexpr int kDecUnit = kDecWarps * kDecChunk;     // positions of a unit
 constexpr int kDecCtasPerSm = 3;
 constexpr int kDecMaxRows = 16, kDecMaxDim = 128;
+constexpr int kDecMostRows = 64;                    // of a sequence and kv head: in groups of 16
+constexpr int kDecGroup = 16;                       // parts that are added up together
 constexpr float kDigits = 32512.f;                  // 127 * 256: the high digit stays below 128
-constexpr int64_t kDecSlotFloats = kDecMaxRows * (kDecMaxDim + 2);
+// a partial result: [rows][head_dim], then [rows][max, sum], then the same of a group that begins with this part
+__host__ __device__ constexpr int64_t dec_slot_floats(int rows) { return (int64_t)rows * (kDecMaxDim + 4); }
 
 struct DecodeParams {
     PagedAttn a;
-    float* slots;               // [2 * CTAs][rows][head_dim + 2] partial results
-    unsigned int* counters;     // [items] partial results written, zero between calls
-    int groups;                 // groups of rows of a kv head
-    int min_units;              // units of a CTA, at least
+    float* slots;               // [2 * teams] partial results
+    unsigned int* groups_done;  // [2 * teams] parts of a group that are there, zero between calls
+    unsigned int* items_done;   // [items] groups of an item that are there, zero between calls
+    int row_groups;             // groups of rows of a kv head
+    int min_units;              // units of a team, at least
 };
 
 __host__ __device__ constexpr int dec_row_floats(int hd) { return hd + hd / 8; }   // padded: the lanes of a store meet different banks
 __device__ __forceinline__ int dec_pad(int d) { return d + (d >> 5) * 4; }
-template <int kHD, int kTiles>
-__host__ __device__ constexpr int dec_smem_bytes() { return kDecWarps * kTiles * 8 * dec_row_floats(kHD) * 4; }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
@@ -94,126 +95,190 @@ __device__ __forceinline__ void load_v(VRow<kHD>& r, const int8_t* row, int g)
     }
 }
 
-// units of an item of sequence s
-__device__ __forceinline__ int dec_units(const PagedArgs& C, int s)
+
+// what a team does next: units [x, end) of item [a, a + units)
+struct DecodeCut {
+    long long total, tol;
+    int teams;
+    __device__ long long cut(int c) const { return total * c / teams; }                 // a range's end before it moves to an item's
+    __device__ long long snap(long long x, long long a, long long b) const { return x - a < tol ? a : b - x < tol ? b : x; }   // x in item [a, b)
+};
+
+// one row's sum and output
+__device__ __forceinline__ void dec_store4(int16_t* o, const float4& n, float den)
 {
-    const int n = paged_len(C, s);
-    return n <= 0 ? 1 : (n + kDecUnit - 1) / kDecUnit;
+    const float rd = den == 0.f ? 0.f : 1.f / den;                 // no position at all: zero
+    const uint32_t lo = (uint16_t)paged_bf16_rne(n.x * rd) | (uint32_t)(uint16_t)paged_bf16_rne(n.y * rd) << 16;
+    const uint32_t hi = (uint16_t)paged_bf16_rne(n.z * rd) | (uint32_t)(uint16_t)paged_bf16_rne(n.w * rd) << 16;
+    if ((reinterpret_cast<uintptr_t>(o) & 7) == 0) *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+    else { o[0] = (int16_t)lo; o[1] = (int16_t)(lo >> 16); o[2] = (int16_t)hi; o[3] = (int16_t)(hi >> 16); }
 }
 
-template <int kHD, int kTiles>
+// A team is one warp (many items: nothing waits for another warp) or the CTA (few, long items).
+template <int kHD, int kTiles, int kTeam>
 __global__ void __launch_bounds__(kDecThreads, kTiles == 1 ? kDecCtasPerSm : 2)
 paged_decode_kernel(const __grid_constant__ DecodeParams P)
 {
-    constexpr int kRows = 8 * kTiles, kSteps = kHD / 32, kCols = kHD / 8;
-    extern __shared__ __align__(16) float dec_smem[];
-    __shared__ __align__(16) int8_t digits[2][kRows][kHD + 16];    // padded: the lanes of a load meet different banks
-    __shared__ float factor_s[kRows], m_s[kDecWarps][kRows], l_s[kDecWarps][kRows];
+    constexpr int kRows = 8 * kTiles, kSteps = kHD / 32, kCols = kHD / 8, kUnit = kTeam * kDecChunk, kRow = dec_row_floats(kHD);
+    constexpr int64_t kSlot = dec_slot_floats(kRows);
+    constexpr int kTeamThreads = kTeam * 32;
+    struct Digits { int8_t d[2][kRows][kHD + 16]; };               // padded: the lanes of a load meet different banks
+    union WarpRoom { Digits q; float acc[kTeam > 1 ? kRows * kRow : 4]; };   // q as digits, then the warp's sums
+    __shared__ __align__(16) WarpRoom room_s[kDecWarps];
+    __shared__ float m_s[kTeam][kRows], l_s[kTeam][kRows];
     __shared__ int last_s;
     grid_launch_dependents();
     grid_dependency_wait();
     const PagedArgs& C = P.a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-    const int gqa = P.a.n_head / C.n_head_kv, per_seq = C.n_head_kv * P.groups;
+    const int team = blockIdx.x * (kDecWarps / kTeam) + warp / kTeam, tw = warp % kTeam, tt = threadIdx.x % kTeamThreads;
+    const int gqa = P.a.n_head / C.n_head_kv, per_seq = C.n_head_kv * P.row_groups;
+    auto team_sync = [] { if (kTeam > 1) __syncthreads(); else __syncwarp(); };
+    auto units_of = [&](int s) { const int n = paged_len(C, s); return n <= 0 ? 1 : (n + kUnit - 1) / kUnit; };
 
-    // ---- the units of all items, and this CTA's start: the sequence that holds it (every warp for itself)
-    long long total = 0;
+    // ---- the units of all items, and the sequence that holds this team's start (every warp for itself)
+    DecodeCut W = {};
+    const long long u_first = lane < C.num_seqs ? (long long)units_of(lane) * per_seq : 0;
     for (int s0 = 0; s0 < C.num_seqs; s0 += 32) {
-        long long u = s0 + lane < C.num_seqs ? dec_units(C, s0 + lane) : 0;
+        long long u = s0 == 0 ? u_first : s0 + lane < C.num_seqs ? (long long)units_of(s0 + lane) * per_seq : 0;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) u += __shfl_xor_sync(0xFFFFFFFFu, u, off);
-        total += u * per_seq;
+        W.total += u;
     }
-    const long long most = (total + P.min_units - 1) / P.min_units;
-    const int ctas = most < (long long)gridDim.x ? (int)most : (int)gridDim.x, cta = blockIdx.x;
-    if (cta >= ctas) return;
-    const long long tol = max(1ll, total / ctas / 8);
-    auto cut = [&](int c) { return total * c / ctas; };            // a range's end before it moves to an item's
-    auto snap = [&](long long x, long long a, long long b) { return x - a < tol ? a : b - x < tol ? b : x; };   // x in item [a, b)
-    long long x = cut(cta), base = 0;                              // base: first unit of sequence seq
+    const long long most = (W.total + P.min_units - 1) / P.min_units, all = (long long)gridDim.x * (kDecWarps / kTeam);
+    W.teams = (int)(most < all ? most : all);
+    if (team >= W.teams) return;
+    W.tol = max(1ll, W.total / W.teams / 8);
+    long long x = W.cut(team), a = 0;
     int seq = 0;
     for (int s0 = 0; s0 < C.num_seqs; s0 += 32) {
-        long long u = s0 + lane < C.num_seqs ? (long long)dec_units(C, s0 + lane) * per_seq : 0;
+        const long long u = s0 == 0 ? u_first : s0 + lane < C.num_seqs ? (long long)units_of(s0 + lane) * per_seq : 0;
         long long upto = u;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const long long o = __shfl_up_sync(0xFFFFFFFFu, upto, off);
             if (lane >= off) upto += o;
         }
-        const unsigned over = __ballot_sync(0xFFFFFFFFu, base + upto > x);
+        const unsigned over = __ballot_sync(0xFFFFFFFFu, a + upto > x);
         if (over) {
             const int l = __ffs(over) - 1;
             seq = s0 + l;
-            base += __shfl_sync(0xFFFFFFFFu, upto - u, l);
+            a += __shfl_sync(0xFFFFFFFFu, upto - u, l);
             break;
         }
-        base += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        a += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
-    int units = dec_units(C, seq), item = (int)((x - base) / units);   // item of the sequence
-    long long a = base + (long long)item * units;                  // its first unit
-    x = snap(x, a, a + units);
-    const long long next = cut(cta + 1);                           // this CTA's end lies in or at the end of an item met below
-
+    int units = units_of(seq), item = (int)((x - a) / units);      // item of the sequence
+    a += (long long)item * units;                                  // its first unit
+    x = W.snap(x, a, a + units);
+    const long long next = W.cut(team + 1);                        // this team's end lies in, or at the end of, an item met below
     const float to_log2 = P.a.scale * 1.4426950408889634f;
-    while (a < total) {
-        if (x >= a + units) {                                      // the start moved to the item's end
-            a += units;
+    const int ps = 1 << C.page_shift;
+
+    while (true) {
+        if (x >= a + units) {                                      // the start moved to the item's end, or the item is done
+            a += units; x = a;
             if (++item == per_seq) {
                 if (++seq == C.num_seqs) break;
-                item = 0; units = dec_units(C, seq);
+                item = 0; units = units_of(seq);
             }
-            if (x > a) x = a;
         }
-        // the part [x, end) of item [a, a + units)
         long long end = a + units;
-        if (next < end) end = snap(next, a, end);
+        if (next < end) end = W.snap(next, a, end);
         if (x >= end) break;
-        const int kvh = item / P.groups, row_base = (item - kvh * P.groups) * kRows;
+        const int kvh = item / P.row_groups, row_base = (item - kvh * P.row_groups) * kRows;
         int lo, hi;
         paged_rows(C, seq, lo, hi);
         const int rows = min(kRows, (hi - lo) * gqa - row_base);   // rows of this item; 0 or less: none
         if (rows > 0) {
-            const int len = C.kv_len[seq], room = paged_len(C, seq);
-            __syncthreads();                                       // the last item's shared memory has been read
-            for (int r = warp; r < kRows; r += kDecWarps) {
-                float v[kHD / 32], top = 0.f;
-                const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
-                const float* q = P.a.q + (size_t)(lo + tok) * P.a.q_stride + (size_t)(kvh * gqa + head) * kHD;
+            const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // row r sees min(before + token, room) positions
+            const int least = min(before + row_base / gqa, room), most_seen = min(before + (row_base + rows - 1) / gqa, room);
+            const int t_lo = (int)(x - a) * kUnit, t_hi = (int)min((end - a) * kUnit, (long long)most_seen);
+            const int* table = C.table + (size_t)seq * C.table_stride;
+            bool missing = false;
+            // page of position t; -1: none, or t not below t_hi
+            auto page_at = [&](int t) {
+                if (t >= t_hi) return -1;
+                const int p = table[t >> C.page_shift];
+                if ((unsigned)p < (unsigned)C.num_pages) return p;
+                missing = true;
+                return -1;
+            };
+            // row of the pools' arrays (2^32 rows are more than a GPU holds); absent pages read page 0, masked later
+            auto row_at = [&](int page, int t) { return (((uint32_t)max(page, 0) * C.n_head_kv + kvh) << C.page_shift) + (t & (ps - 1)); };
+            KRow<kHD> k[4];
+            VRow<kHD> v[8];
+            float4 sk[2], sv[2];
+            auto fetch_k = [&](int t0, int page) {
+                const int8_t* row = C.k + (size_t)row_at(page, t0 + 4 * g) * kHD;
 #pragma unroll
-                for (int i = 0; i < kHD / 32; i++) v[i] = r < rows ? q[i * 32 + lane] : 0.f;
-                uint32_t bits = 0;                                 // of magnitudes: a NaN is the largest
+                for (int u = 0; u < 4; u++) load_k<kHD>(k[u], row + u * kHD, t4);
+            };
+            auto fetch_v = [&](uint32_t at) {
+                const int8_t* row = C.v + (size_t)at * kHD;
 #pragma unroll
-                for (int i = 0; i < kHD / 32; i++) bits = max(bits, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-                bits = __reduce_max_sync(0xFFFFFFFFu, bits);
-                top = __uint_as_float(bits);
-                const bool fine = top >= 1e-30f && bits < 0x7F800000u;   // smaller ones count as zero
-                const float inv = fine ? kDigits / top : 0.f;
-#pragma unroll
-                for (int i = 0; i < kHD / 32; i++) {
-                    const int X = fine ? __float2int_rn(v[i] * inv) : 0, h = (X + 128) >> 8;
-                    digits[0][r][i * 32 + lane] = (int8_t)h; digits[1][r][i * 32 + lane] = (int8_t)(X - 256 * h);
-                }
-                if (lane == 0) factor_s[r] = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : top / kDigits * to_log2;
+                for (int u = 0; u < 8; u++) load_v<kHD>(v[u], row + u * kHD, g);
+            };
+            auto fetch_s = [&](float4 (&s)[2], const float* scales, uint32_t at) {
+                s[0] = *reinterpret_cast<const float4*>(scales + at); s[1] = *reinterpret_cast<const float4*>(scales + at + 4);
+            };
+            int t0 = t_lo + tw * kDecChunk;
+            // a chunk has one page, or two of 16 positions: K rows 4 g + u lie in the half of g >> 2, V rows 8 t4 + u of t4 >> 1
+            const int kt = (g >> 2) * 16, vt = (t4 >> 1) * 16;
+            int pk = page_at(t0 + kt), pv = page_at(t0 + vt), pk_next = page_at(t0 + kUnit + kt), pv_next = page_at(t0 + kUnit + vt);
+            if (t0 < t_hi) {
+                const uint32_t at = row_at(pv, t0 + 8 * t4);
+                fetch_k(t0, pk); fetch_s(sk, C.sk, at); fetch_s(sv, C.sv, at); fetch_v(at);
             }
-            __syncthreads();
+            // ---- q as digits, every warp for itself
             uint32_t qa[kTiles][kSteps][4];
             float factor[kTiles];
             int limit[kTiles];                                     // positions that the lane's row may see
 #pragma unroll
+            for (int i = 0; i < kTiles; i++) factor[i] = 0.f;
+            team_sync();                                           // the last item's digits and sums have been read
+            auto& digits = room_s[warp].q.d;
+#pragma unroll
+            for (int r = 0; r < kRows; r++) {
+                if (r >= rows) break;
+                const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
+                const float* q = P.a.q + (size_t)(lo + tok) * P.a.q_stride + (size_t)(kvh * gqa + head) * kHD + 4 * lane;
+                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (4 * lane < kHD) {
+                    if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) f = *reinterpret_cast<const float4*>(q);
+                    else f = make_float4(q[0], q[1], q[2], q[3]);
+                }
+                const float e[4] = {f.x, f.y, f.z, f.w};
+                uint32_t bits = 0;                                 // of the largest magnitude; a NaN is the largest
+#pragma unroll
+                for (int j = 0; j < 4; j++) bits = max(bits, __float_as_uint(e[j]) & 0x7FFFFFFFu);
+                bits = __reduce_max_sync(0xFFFFFFFFu, bits);
+                const float top = __uint_as_float(bits);
+                const bool fine = top >= 1e-30f && bits < 0x7F800000u;   // rows of smaller ones count as zero
+                const float inv = fine ? kDigits / top : 0.f;
+                uint32_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[j] = __float_as_uint(fmaf(fine ? e[j] : 0.f, inv, 12582912.f + 128.f));   // 256 hi + lo + 128
+                const uint32_t p01 = prmt(y[0], y[1], 0x5140u), p23 = prmt(y[2], y[3], 0x5140u);
+                if (4 * lane < kHD) {
+                    *reinterpret_cast<uint32_t*>(&digits[0][r][4 * lane]) = prmt(p01, p23, 0x7632u);
+                    *reinterpret_cast<uint32_t*>(&digits[1][r][4 * lane]) = prmt(p01, p23, 0x5410u) ^ 0x80808080u;
+                }
+                if ((r & 7) == g) factor[r >> 3] = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : top / kDigits * to_log2;
+            }
+            __syncwarp();
+#pragma unroll
             for (int i = 0; i < kTiles; i++) {
                 const int r = i * 8 + g;
+                const bool there = r < rows;
 #pragma unroll
                 for (int s = 0; s < kSteps; s++) {
                     const uint2 h = *reinterpret_cast<const uint2*>(&digits[0][r][k_dim<kHD>(s, t4)]);
                     const uint2 l = *reinterpret_cast<const uint2*>(&digits[1][r][k_dim<kHD>(s, t4)]);
-                    qa[i][s][0] = h.x; qa[i][s][1] = l.x; qa[i][s][2] = h.y; qa[i][s][3] = l.y;
+                    qa[i][s][0] = there ? h.x : 0u; qa[i][s][1] = there ? l.x : 0u; qa[i][s][2] = there ? h.y : 0u; qa[i][s][3] = there ? l.y : 0u;
                 }
-                factor[i] = factor_s[r];
-                limit[i] = r < rows ? min(len - (hi - lo) + (row_base + r) / gqa + 1, room) : 0;
+                limit[i] = there ? min(before + (row_base + r) / gqa, room) : 0;
             }
-            const int least = min(len - (hi - lo) + row_base / gqa + 1, room);                    // of all rows
-            const int most_seen = min(len - (hi - lo) + (row_base + rows - 1) / gqa + 1, room);
-            const int t_lo = (int)(x - a) * kDecUnit, t_hi = min((int)(end - a) * kDecUnit, most_seen);
             float acc[kTiles][kCols][2], m[kTiles], l[kTiles];
 #pragma unroll
             for (int i = 0; i < kTiles; i++) {
@@ -221,106 +286,71 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
 #pragma unroll
                 for (int j = 0; j < kCols; j++) acc[i][j][0] = acc[i][j][1] = 0.f;
             }
-            const int ps = 1 << C.page_shift;
-            const int* table = C.table + (size_t)seq * C.table_stride;
-            bool missing = false;
-            // page of position t, -1: none
-            auto page_at = [&](int t) {
-                if (t >= t_hi || (t >> C.page_shift) >= C.table_pages) return -1;
-                const int p = table[t >> C.page_shift];
-                if ((unsigned)p < (unsigned)C.num_pages) return p;
-                missing = true;
-                return -1;
-            };
-            KRow<kHD> k[4];
-            VRow<kHD> v[8];
-            float4 sk[2], sv[2];
-            auto fetch_k = [&](int t0, int page) {
-                const size_t at = ((size_t)page * C.n_head_kv + kvh) << C.page_shift;
-                const int8_t* row = C.k + (at + ((t0 + 4 * g) & (ps - 1))) * kHD;
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    if (page >= 0) load_k<kHD>(k[u], row + u * kHD, t4);
-                    else
-#pragma unroll
-                        for (int i = 0; i < kHD / 16; i++) k[u].w[i] = 0;
-                }
-            };
-            auto fetch_v = [&](int t0, int page) {
-                const size_t at = (((size_t)page * C.n_head_kv + kvh) << C.page_shift) + ((t0 + 8 * t4) & (ps - 1));
-#pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    if (page >= 0) load_v<kHD>(v[u], C.v + (at + u) * kHD, g);
-                    else
-#pragma unroll
-                        for (int i = 0; i < kHD / 32; i++) v[u].w[i] = 0;
-                }
-            };
-            auto fetch_s = [&](float4 (&s)[2], const float* scales, int t0, int page) {
-                const size_t at = (((size_t)page * C.n_head_kv + kvh) << C.page_shift) + ((t0 + 8 * t4) & (ps - 1));
-#pragma unroll
-                for (int u = 0; u < 2; u++) s[u] = page >= 0 ? reinterpret_cast<const float4*>(scales + at)[u] : make_float4(0.f, 0.f, 0.f, 0.f);
-            };
-            int t0 = t_lo + warp * kDecChunk;
-            // a chunk has one page, or two of 16 positions: K rows 4 g + u lie in the half of g >> 2, V rows 8 t4 + u of t4 >> 1
-            int pk = page_at(t0 + (g >> 2) * 16), pv = page_at(t0 + (t4 >> 1) * 16);
-            int pk_next = page_at(t0 + kDecUnit + (g >> 2) * 16), pv_next = page_at(t0 + kDecUnit + (t4 >> 1) * 16);
-            fetch_k(t0, pk);
-            fetch_s(sk, C.sk, t0, pv);
-            fetch_s(sv, C.sv, t0, pv);
-            fetch_v(t0, pv);
 #pragma unroll 1
-            for (; t0 < t_hi; t0 += kDecUnit) {
-                const int t_next = t0 + kDecUnit;
-                // ---- scores
-                int c[kTiles][4][4];
-#pragma unroll
-                for (int i = 0; i < kTiles; i++)
-#pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        c[i][u][0] = c[i][u][1] = c[i][u][2] = c[i][u][3] = 0;
-#pragma unroll
-                        for (int s = 0; s < kSteps; s++)
-                            mma_s8(c[i][u], qa[i][s][0], qa[i][s][1], qa[i][s][2], qa[i][s][3], k[u].w[2 * s], k[u].w[2 * s + 1]);
-                    }
-                fetch_k(t_next, pk_next);
-                const float skv[8] = {sk[0].x, sk[0].y, sk[0].z, sk[0].w, sk[1].x, sk[1].y, sk[1].z, sk[1].w};
-                const bool whole = __all_sync(0xFFFFFFFFu, pv >= 0 && t0 + kDecChunk <= least);
-                float s[kTiles][8];                                 // score of position t0 + 8 t4 + i, in powers of two
-#pragma unroll
-                for (int i = 0; i < kTiles; i++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-#pragma unroll
-                        for (int u = 0; u < 4; u++) s[i][4 * e + u] = (float)(256 * c[i][u][e] + c[i][u][2 + e]) * skv[4 * e + u] * factor[i];
-                if (!whole) {
+            for (; t0 < t_hi; t0 += kUnit) {
+                const bool more = t0 + kUnit < t_hi;
+                const uint32_t at_next = row_at(pv_next, t0 + kUnit + 8 * t4);
+                // ---- scores, in powers of two: s[p] of position t0 + 8 t4 + p
+                float s[kTiles][8];
+                {
+                    int c[kTiles][4][4];
 #pragma unroll
                     for (int i = 0; i < kTiles; i++)
 #pragma unroll
-                        for (int p = 0; p < 8; p++) if (pv < 0 || t0 + 8 * t4 + p >= limit[i]) s[i][p] = -INFINITY;
+                        for (int u = 0; u < 4; u++) {
+                            c[i][u][0] = c[i][u][1] = c[i][u][2] = c[i][u][3] = 0;
+#pragma unroll
+                            for (int st = 0; st < kSteps; st++)
+                                mma_s8(c[i][u], qa[i][st][0], qa[i][st][1], qa[i][st][2], qa[i][st][3], k[u].w[2 * st], k[u].w[2 * st + 1]);
+                        }
+                    if (more) fetch_k(t0 + kUnit, pk_next);
+                    const float skv[8] = {sk[0].x, sk[0].y, sk[0].z, sk[0].w, sk[1].x, sk[1].y, sk[1].z, sk[1].w};
+#pragma unroll
+                    for (int i = 0; i < kTiles; i++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+#pragma unroll
+                            for (int u = 0; u < 4; u++) s[i][4 * e + u] = (float)(256 * c[i][u][e] + c[i][u][2 + e]) * (skv[4 * e + u] * factor[i]);
                 }
-                fetch_s(sk, C.sk, t_next, pv_next);
-                // ---- weights: of the chunk's own maximum, times the values' scales, as two digits of the largest such product
+                if (more) fetch_s(sk, C.sk, at_next);
                 const float svv[8] = {sv[0].x, sv[0].y, sv[0].z, sv[0].w, sv[1].x, sv[1].y, sv[1].z, sv[1].w};
+                float odd = 0.f;                                    // NaN where a value's scale is not finite
+#pragma unroll
+                for (int p = 0; p < 8; p++) odd = fmaf(svv[p], 0.f, odd);
+                const bool plain = __all_sync(0xFFFFFFFFu, odd == 0.f && pv >= 0 && t0 + kDecChunk <= least);
+                // ---- weights: of the chunk's own maximum, times the values' scales, as two digits of the largest such product
                 uint32_t pa[kTiles][4];
                 float gain[kTiles];
 #pragma unroll
                 for (int i = 0; i < kTiles; i++) {
+                    if (!plain) {
+#pragma unroll
+                        for (int p = 0; p < 8; p++) if (pv < 0 || t0 + 8 * t4 + p >= limit[i]) s[i][p] = -INFINITY;
+                    }
                     float mx = -1e30f;
 #pragma unroll
                     for (int p = 0; p < 8; p++) mx = fmaxf(mx, s[i][p]);
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
                     float sum = 0.f, top = 0.f, z[8];
+                    if (plain) {
 #pragma unroll
-                    for (int p = 0; p < 8; p++) {
-                        const float w = dec_exp2(s[i][p] - mx);
-                        z[p] = w * svv[p];
-                        float mark = fmaf(svv[p], 0.f, w);          // w, or NaN where the scale is not finite
-                        if (!whole && s[i][p] == -INFINITY) z[p] = mark = 0.f;
-                        sum += mark;
-                        if (!(fabsf(z[p]) < INFINITY)) z[p] = 0.f;
-                        top = fmaxf(top, fabsf(z[p]));
+                        for (int p = 0; p < 8; p++) {
+                            const float w = dec_exp2(s[i][p] - mx);
+                            z[p] = w * svv[p];
+                            sum += w;
+                            top = fmaxf(top, fabsf(z[p]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < 8; p++) {
+                            const float w = dec_exp2(s[i][p] - mx);
+                            const bool masked = s[i][p] == -INFINITY;
+                            z[p] = masked ? 0.f : w * svv[p];
+                            sum += masked ? 0.f : fmaf(svv[p], 0.f, w);   // a scale that is not finite marks the rows that use it
+                            if (!(fabsf(z[p]) < INFINITY)) z[p] = 0.f;
+                            top = fmaxf(top, fabsf(z[p]));
+                        }
                     }
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -343,7 +373,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                         pa[i][2 * e + 1] = prmt(p01, p23, 0x5410u) ^ 0x80808080u;
                     }
                 }
-                fetch_s(sv, C.sv, t_next, pv_next);
+                if (more) fetch_s(sv, C.sv, at_next);
                 // ---- weighted values
 #pragma unroll
                 for (int w = 0; w < kHD / 32; w++) {
@@ -365,85 +395,118 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                             for (int e = 0; e < 2; e++) acc[i][4 * w + d][e] = fmaf((float)(256 * o[e] + o[2 + e]), gain[i], acc[i][4 * w + d][e]);
                         }
                 }
-                fetch_v(t_next, pv_next);
+                if (more) fetch_v(at_next);
                 pk = pk_next; pv = pv_next;
-                pk_next = page_at(t_next + kDecUnit + (g >> 2) * 16); pv_next = page_at(t_next + kDecUnit + (t4 >> 1) * 16);
+                pk_next = page_at(t0 + 2 * kUnit + kt); pv_next = page_at(t0 + 2 * kUnit + vt);
             }
             if (missing) atomicOr(C.status, kStatusPage);
-            // ---- the warps' results meet in shared memory
+            // ---- the team's sums: thread tt has elements 4 (tt + n * threads) of the rows.  A warp alone: its own.
 #pragma unroll
             for (int i = 0; i < kTiles; i++) {
                 l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
                 l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
-                const int r = i * 8 + g;
-                if (t4 == 0) { m_s[warp][r] = m[i]; l_s[warp][r] = l[i]; }
-                float* row = dec_smem + (size_t)(warp * kRows + r) * dec_row_floats(kHD);
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-#pragma unroll
-                    for (int j = 0; j < kCols; j += 4)
-                        *reinterpret_cast<float4*>(row + dec_pad((2 * t4 + e) * kCols + j)) = make_float4(acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]);
             }
-            __syncthreads();
             const bool alone = x == a && end == a + units;
-            const int slot = 2 * cta + (x == a ? 1 : 0);            // at most one part of an item that began before, one of one that goes on
-            float* part = P.slots + (size_t)slot * kDecSlotFloats;
-            for (int i = threadIdx.x; i < rows * (kHD / 4); i += kDecThreads) {
-                const int r = i / (kHD / 4), d = (i - r * (kHD / 4)) * 4;
-                float mm = -1e30f, den = 0.f;
-                float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto out_at = [&](int r, int d) {
+                const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
+                return P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD + d;
+            };
+            float* part = P.slots + (size_t)(2 * team + (x == a ? 1 : 0)) * kSlot;   // a team has at most one part of an item that began before, and one of one that goes on
+            if (kTeam == 1) {
 #pragma unroll
-                for (int w = 0; w < kDecWarps; w++) mm = fmaxf(mm, m_s[w][r]);
+                for (int i = 0; i < kTiles; i++) {
+                    const int r = i * 8 + g;
+                    if (r >= rows) continue;
+                    if (!alone && t4 == 0) { part[kRows * kHD + 2 * r] = m[i]; part[kRows * kHD + 2 * r + 1] = l[i]; }
 #pragma unroll
-                for (int w = 0; w < kDecWarps; w++) {
-                    const float f = dec_exp2(m_s[w][r] - mm);
-                    const float4 y = *reinterpret_cast<const float4*>(dec_smem + (size_t)(w * kRows + r) * dec_row_floats(kHD) + dec_pad(d));
-                    num.x += f * y.x; num.y += f * y.y; num.z += f * y.z; num.w += f * y.w;
-                    den += f * l_s[w][r];
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int j = 0; j < kCols; j += 4) {
+                            const float4 n = make_float4(acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]);
+                            const int d = (2 * t4 + e) * kCols + j;
+                            if (alone) dec_store4(out_at(r, d), n, l[i]);
+                            else *reinterpret_cast<float4*>(part + r * kHD + d) = n;
+                        }
                 }
-                if (!alone) {
+            } else {
+                __syncwarp();                                      // this warp's digits have been read
+#pragma unroll
+                for (int i = 0; i < kTiles; i++) {
+                    const int r = i * 8 + g;
+                    if (t4 == 0) { m_s[tw][r] = m[i]; l_s[tw][r] = l[i]; }
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int j = 0; j < kCols; j += 4)
+                            *reinterpret_cast<float4*>(&room_s[tw].acc[r * kRow + dec_pad((2 * t4 + e) * kCols + j)]) =
+                                make_float4(acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]);
+                }
+                __syncthreads();
+                for (int i = tt; i < rows * (kHD / 4); i += kTeamThreads) {
+                    const int r = i / (kHD / 4), d = (i - r * (kHD / 4)) * 4;
+                    float mm = -1e30f, den = 0.f;
+                    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < kTeam; w++) mm = fmaxf(mm, m_s[w][r]);
+#pragma unroll
+                    for (int w = 0; w < kTeam; w++) {
+                        const float f = dec_exp2(m_s[w][r] - mm);
+                        const float4 y = *reinterpret_cast<const float4*>(&room_s[w].acc[r * kRow + dec_pad(d)]);
+                        num.x += f * y.x; num.y += f * y.y; num.z += f * y.z; num.w += f * y.w;
+                        den += f * l_s[w][r];
+                    }
+                    if (alone) { dec_store4(out_at(r, d), num, den); continue; }
                     *reinterpret_cast<float4*>(part + r * kHD + d) = num;
                     if (d == 0) { part[kRows * kHD + 2 * r] = mm; part[kRows * kHD + 2 * r + 1] = den; }
-                    continue;
                 }
-                const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
-                int16_t* o = P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD + d;
-                const float rd = den == 0.f ? 0.f : 1.f / den;      // no position at all: zero
-                o[0] = paged_bf16_rne(num.x * rd); o[1] = paged_bf16_rne(num.y * rd);
-                o[2] = paged_bf16_rne(num.z * rd); o[3] = paged_bf16_rne(num.w * rd);
             }
             if (!alone) {
-                // CTAs whose ends lie strictly inside this item
-                const long long A = a + tol, B = a + units - tol;
-                const int c_lo = (int)((A * ctas + total - 1) / total), c_hi = (int)(((B + 1) * ctas + total - 1) / total) - 1;
-                const int parts = c_hi - c_lo + 2;
-                unsigned int* counter = P.counters + (size_t)seq * per_seq + item;
-                __threadfence();
-                __syncthreads();
-                if (threadIdx.x == 0) last_s = atomicAdd(counter, 1u) == (unsigned)parts - 1;
-                __syncthreads();
-                if (last_s) {
+                // teams whose starts lie strictly inside this item: c_lo to c_hi; its first part is team c_lo - 1's
+                const long long A = a + W.tol, B = a + units - W.tol;
+                const int c_lo = (int)((A * W.teams + W.total - 1) / W.total), c_hi = (int)(((B + 1) * W.teams + W.total - 1) / W.total) - 1;
+                const int c0 = c_lo - 1, parts = c_hi - c0 + 1, ngroups = (parts + kDecGroup - 1) / kDecGroup;
+                auto slot_of = [&](int n) { return 2 * (c0 + n) + (n == 0 ? 1 : 0); };   // of part n
+                // true in the team that is the last of `n` to come
+                auto last_of = [&](unsigned int* counter, int n) {
                     __threadfence();
-                    if (threadIdx.x == 0) *counter = 0;
-                    for (int i = threadIdx.x; i < rows * (kHD / 4); i += kDecThreads) {
+                    team_sync();
+                    int last = 0;
+                    if (tt == 0) {
+                        last = atomicAdd(counter, 1u) == (unsigned)n - 1;
+                        if (last) *counter = 0;
+                        if (kTeam > 1) last_s = last;
+                    }
+                    team_sync();
+                    last = kTeam > 1 ? last_s : __shfl_sync(0xFFFFFFFFu, last, 0);
+                    __threadfence();
+                    return last != 0;
+                };
+                // adds n parts, or sums of groups (stats: where their statistics lie): to the output, or over the first one
+                auto add_up = [&](int first, int step, int n, int stats, bool finish) {
+                    for (int i = tt; i < rows * (kHD / 4); i += kTeamThreads) {
                         const int r = i / (kHD / 4), d = (i - r * (kHD / 4)) * 4;
-                        auto of = [&](int c) { return P.slots + (size_t)(2 * c + (c == c_lo - 1 ? 1 : 0)) * kDecSlotFloats; };
                         float mm = -1e30f, den = 0.f;
                         float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (int c = c_lo - 1; c <= c_hi; c++) mm = fmaxf(mm, __ldcg(of(c) + kRows * kHD + 2 * r));
-                        for (int c = c_lo - 1; c <= c_hi; c++) {
-                            const float* p = of(c);
-                            const float f = dec_exp2(__ldcg(p + kRows * kHD + 2 * r) - mm);
+#pragma unroll 8
+                        for (int j = 0; j < n; j++) {
+                            const float* p = P.slots + (size_t)slot_of(first + j * step) * kSlot;
+                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + kRows * kHD + stats + 2 * r));
                             const float4 y = __ldcg(reinterpret_cast<const float4*>(p + r * kHD + d));
-                            num.x += f * y.x; num.y += f * y.y; num.z += f * y.z; num.w += f * y.w;
-                            den += f * __ldcg(p + kRows * kHD + 2 * r + 1);
+                            const float mn = fmaxf(mm, ml.x), f0 = dec_exp2(mm - mn), f = dec_exp2(ml.x - mn);
+                            num.x = num.x * f0 + f * y.x; num.y = num.y * f0 + f * y.y; num.z = num.z * f0 + f * y.z; num.w = num.w * f0 + f * y.w;
+                            den = den * f0 + f * ml.y;
+                            mm = mn;
                         }
-                        const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
-                        int16_t* o = P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD + d;
-                        const float rd = den == 0.f ? 0.f : 1.f / den;
-                        o[0] = paged_bf16_rne(num.x * rd); o[1] = paged_bf16_rne(num.y * rd);
-                        o[2] = paged_bf16_rne(num.z * rd); o[3] = paged_bf16_rne(num.w * rd);
+                        if (finish) { dec_store4(out_at(r, d), num, den); continue; }
+                        float* p = P.slots + (size_t)slot_of(first) * kSlot;
+                        *reinterpret_cast<float4*>(p + r * kHD + d) = num;      // read by this thread alone; the statistics by all of the row
+                        if (d == 0) *reinterpret_cast<float2*>(p + kRows * kHD + 2 * kRows + 2 * r) = make_float2(mm, den);
                     }
+                };
+                const int group = (team - c0) / kDecGroup, n_in = min(kDecGroup, parts - group * kDecGroup);
+                if (last_of(P.groups_done + slot_of(group * kDecGroup), n_in)) {
+                    add_up(group * kDecGroup, 1, n_in, 0, ngroups == 1);
+                    if (ngroups > 1 && last_of(P.items_done + (size_t)seq * per_seq + item, ngroups)) add_up(0, kDecGroup, ngroups, 2 * kRows, true);
                 }
             }
         }
@@ -451,31 +514,33 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
         if (end < a + units) break;                                 // the range ends inside the item
     }
 }
-
-static int64_t dec_slot_bytes() { return 2ll * sm_count() * kDecCtasPerSm * kDecSlotFloats * 4; }
-static int dec_groups(int n_head, int n_head_kv, int max_new)
-{
-    const long long rows = (long long)(n_head / n_head_kv) * max_new;
-    return (int)((rows + kDecMaxRows - 1) / kDecMaxRows);
-}
+// the workspace: partial results, then the counters; the same places for every call on a device
+static int64_t dec_teams(int team) { return (int64_t)sm_count() * kDecCtasPerSm * (kDecWarps / team); }
+static int64_t dec_slot_bytes() { return std::max(2 * dec_teams(kDecWarps) * dec_slot_floats(kDecMaxRows), 2 * dec_teams(1) * dec_slot_floats(8)) * 4; }
+static int64_t dec_group_bytes() { return 2 * dec_teams(1) * 4; }
 int64_t paged_decode_workspace_bytes(int n_head, int n_head_kv, int num_seqs, int max_new)
 {
-    return dec_slot_bytes() + (int64_t)num_seqs * n_head_kv * dec_groups(n_head, n_head_kv, max_new) * 4;
+    const long long rows = std::min((long long)(n_head / n_head_kv) * max_new, (long long)kDecMostRows);   // enough for fewer, too
+    return dec_slot_bytes() + dec_group_bytes() + (int64_t)num_seqs * n_head_kv * ((rows + 7) / 8) * 4;
 }
 
-template <int kHD, int kTiles>
-static int decode_launch(const DecodeParams& P, int ctas, void* stream, const char* who)
+template <int kHD, int kTiles, int kTeam>
+static int decode_launch(DecodeParams P, long long units, void* stream, const char* who)
 {
-    constexpr int smem = dec_smem_bytes<kHD, kTiles>();
-    static std::atomic<bool> attr_set[64];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (smem > 40 * 1024 && (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_relaxed))) {
-        const int rc = check_cuda(cudaFuncSetAttribute(paged_decode_kernel<kHD, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
-        if (rc) return rc;
-        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_relaxed);
-    }
-    return launch(paged_decode_kernel<kHD, kTiles>, dim3(ctas), dim3(kDecThreads), smem, stream, who, P);
+    const long long ctas = (units + P.min_units - 1) / P.min_units, most = (long long)sm_count() * kDecCtasPerSm * (kDecWarps / kTeam);
+    const long long teams = std::max(1ll, std::min(ctas, most));
+    return launch(paged_decode_kernel<kHD, kTiles, kTeam>, dim3((unsigned)((teams * kTeam + kDecWarps - 1) / kDecWarps)), dim3(kDecThreads), 0, stream, who, P);
+}
+template <int kHD>
+static int decode_launch_hd(DecodeParams P, int tiles, void* stream, const char* who)
+{
+    const PagedAttn& A = P.a;
+    const long long items = (long long)A.c.num_seqs * A.c.n_head_kv * P.row_groups;
+    auto units = [&](int team) { return items * ((A.max_len + team * kDecChunk - 1) / (team * kDecChunk)); };   // at most, by the caller's bounds
+    P.min_units = env_knob("S12_PAGED_MIN_UNITS", 2);
+    if (tiles == 2) return decode_launch<kHD, 2, kDecWarps>(P, units(kDecWarps), stream, who);
+    if (items >= env_knob("S12_PAGED_ITEMS", 1000)) return decode_launch<kHD, 1, 1>(P, units(1), stream, who);
+    return decode_launch<kHD, 1, kDecWarps>(P, units(kDecWarps), stream, who);
 }
 
 // 1: not a shape of this kernel
@@ -483,23 +548,20 @@ int paged_decode_launch(const PagedAttn& A, void* stream, const char* who)
 {
     const int hd = A.c.head_dim, gqa = A.n_head / A.c.n_head_kv;
     const long long rows = (long long)gqa * A.max_new;
-    if ((hd != 64 && hd != 96 && hd != 128) || rows > 64) return 1;
+    if ((hd != 64 && hd != 96 && hd != 128) || rows > kDecMostRows) return 1;
     const int64_t need = paged_decode_workspace_bytes(A.n_head, A.c.n_head_kv, A.c.num_seqs, A.max_new);
     if (!A.workspace || A.workspace_bytes < need || (reinterpret_cast<uintptr_t>(A.workspace) & 15))
         return fail(S12_ERR_BAD_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
     DecodeParams P = {};
     P.a = A;
     P.slots = (float*)A.workspace;
-    P.counters = (unsigned int*)((char*)A.workspace + dec_slot_bytes());
+    P.groups_done = (unsigned int*)((char*)A.workspace + dec_slot_bytes());
+    P.items_done = P.groups_done + dec_group_bytes() / 4;
     const int tiles = rows <= 8 ? 1 : 2;
-    P.groups = (int)((rows + 8 * tiles - 1) / (8 * tiles));
-    P.min_units = 4;
-    // units that the bounds allow: no more CTAs than that
-    const long long units = (long long)A.c.num_seqs * A.c.n_head_kv * P.groups * ((std::max(A.max_len, 1) + kDecUnit - 1) / kDecUnit);
-    const int ctas = (int)std::max(1ll, std::min((units + P.min_units - 1) / P.min_units, (long long)sm_count() * kDecCtasPerSm));
-    if (hd == 64) return tiles == 1 ? decode_launch<64, 1>(P, ctas, stream, who) : decode_launch<64, 2>(P, ctas, stream, who);
-    if (hd == 96) return tiles == 1 ? decode_launch<96, 1>(P, ctas, stream, who) : decode_launch<96, 2>(P, ctas, stream, who);
-    return tiles == 1 ? decode_launch<128, 1>(P, ctas, stream, who) : decode_launch<128, 2>(P, ctas, stream, who);
+    P.row_groups = (int)((rows + 8 * tiles - 1) / (8 * tiles));
+    if (hd == 64) return decode_launch_hd<64>(P, tiles, stream, who);
+    if (hd == 96) return decode_launch_hd<96>(P, tiles, stream, who);
+    return decode_launch_hd<128>(P, tiles, stream, who);
 }
 
 }  // namespace s12
