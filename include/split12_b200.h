@@ -480,7 +480,8 @@ typedef struct S12PagedKv {
  * q_start[num_seqs] are not read and left as they were.  The three arrays are
  * device int32, so a captured graph serves later steps; the rest is the host's.
  * num_tokens, max_new and max_len are bounds that hold for every replay: rows,
- * new tokens of one sequence, positions of one sequence. */
+ * new tokens of one sequence, positions of one sequence (the attention masks
+ * positions from max_len on; the store looks at neither of the last two). */
 typedef struct S12PagedBatch {
     const int32_t* block_table; /* [num_seqs][table_stride], table_pages entries of a row in use */
     const int32_t* kv_len;      /* [num_seqs] */

@@ -14,6 +14,7 @@ struct PagedArgs {
     unsigned int* status;
     int num_pages, page_shift, n_head_kv, head_dim;
     int num_seqs, table_stride, table_pages, num_tokens;
+    int max_len;                // the caller's bound: positions from it on are masked
 };
 
 #ifdef __CUDACC__
@@ -29,11 +30,11 @@ __device__ __forceinline__ int paged_page(const PagedArgs& P, int s, int t)
     const int page = P.table[(size_t)s * P.table_stride + (t >> P.page_shift)];
     return (unsigned)page < (unsigned)P.num_pages ? page : -1;
 }
-// positions of sequence s that the table can hold
+// positions of sequence s inside the table and the caller's bound
 __device__ __forceinline__ int paged_len(const PagedArgs& P, int s)
 {
     const int n = P.kv_len[s];
-    const long long room = (long long)P.table_pages << P.page_shift;
+    const long long room = min((long long)P.table_pages << P.page_shift, (long long)P.max_len);
     return n < 0 ? 0 : n < room ? n : (int)room;
 }
 // rows [lo, hi) of the packed tokens that belong to sequence s
@@ -70,7 +71,7 @@ struct PagedAttn {
     const float* q; int16_t* out;
     int q_stride, out_stride, n_head;
     float scale;
-    int max_new, max_len;       // the caller's bounds: new tokens and positions of a sequence
+    int max_new;                // the caller's bound on a sequence's new tokens
     void* workspace; int64_t workspace_bytes;
 };
 int64_t paged_decode_workspace_bytes(int n_head, int n_head_kv, int num_seqs, int max_new);

@@ -13,10 +13,10 @@
 //             are the A operand of the second product as they lie, against V's rows in order
 //   dims      column n of PV tile j is dim n * head_dim / 8 + j: a lane reads consecutive bytes of each of eight rows
 //             and turns them by byte permutes
-// Work is cut by the device, which alone knows the lengths: the units of all (sequence, kv head, rows) items follow one
-// another and every team of warps takes an equal range; ends within an eighth of a range of an item's end move there.  An
-// item of several teams leaves its partial results in the workspace; of 16 neighbouring parts the team that comes last adds
-// them in order, and of these sums the last again, so that the result does not depend on who came when.
+// Work is cut by the device, which alone knows the lengths: the positions of a (sequence, kv head, rows) item go in equal
+// parts to teams of warps, as many as are resident together (dec_part_units).  The parts of an item leave their results in
+// the workspace; of 16 neighbouring parts the team that comes last adds them in order, and of these sums the last again, so
+// that the result does not depend on who came when.
 #include "paged.cuh"
 #include <algorithm>
 #include <atomic>
@@ -26,7 +26,8 @@ namespace s12 {
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecChunk = 32;                       // positions of a warp's step
-constexpr int kDecCtasPerSm = 3;
+constexpr int kDecCtasPerSm = 3;                    // resident with 8 rows; 2 with 16
+__host__ __device__ constexpr int dec_ctas_per_sm(int tiles) { return tiles == 1 ? kDecCtasPerSm : 2; }
 constexpr int kDecMaxRows = 16, kDecMaxDim = 128;
 constexpr int kDecMostRows = 64;                    // of a sequence and kv head: in groups of 16
 constexpr int kDecGroup = 16;                       // parts that are added up together
@@ -36,11 +37,12 @@ __host__ __device__ constexpr int64_t dec_slot_floats(int rows) { return (int64_
 
 struct DecodeParams {
     PagedAttn a;
-    float* slots;               // [2 * teams] partial results
-    unsigned int* groups_done;  // [2 * teams] parts of a group that are there, zero between calls
+    float* slots;               // [parts of cut items] partial results
+    unsigned int* groups_done;  // [parts of cut items] parts of a group that are there, zero between calls
     unsigned int* items_done;   // [items] groups of an item that are there, zero between calls
     int row_groups;             // groups of rows of a kv head
-    int min_units;              // units of a team, at least
+    int min_units;              // units of a part, at least
+    int teams;                  // that are resident together
 };
 
 __host__ __device__ constexpr int dec_row_floats(int hd) { return hd + hd / 8; }   // padded: the lanes of a store meet different banks
@@ -96,13 +98,36 @@ __device__ __forceinline__ void load_v(VRow<kHD>& r, const int8_t* row, int g)
 }
 
 
-// what a team does next: units [x, end) of item [a, a + units)
-struct DecodeCut {
-    long long total, tol;
-    int teams;
-    __device__ long long cut(int c) const { return total * c / teams; }                 // a range's end before it moves to an item's
-    __device__ long long snap(long long x, long long a, long long b) const { return x - a < tol ? a : b - x < tol ? b : x; }   // x in item [a, b)
-};
+// units of sequence s, in steps of `unit` positions; a sequence without positions has one
+__device__ __forceinline__ uint32_t dec_units(const PagedArgs& C, int s, int unit)
+{
+    const int n = paged_len(C, s);
+    return n <= 0 ? 1u : (uint32_t)(n + unit - 1) / (uint32_t)unit;
+}
+// The most units of a part: the least that gives all items' parts to resident teams.  With so many items that this would
+// cut nothing or nearly nothing, twice a team's share: only what is far longer than the others is cut.  For a whole warp.
+__device__ __forceinline__ uint32_t dec_part_units(const DecodeParams& P, int unit, int per_seq, uint32_t u_first)
+{
+    const PagedArgs& C = P.a.c;
+    const int lane = threadIdx.x & 31;
+    auto sum = [&](auto f) {                                       // of f(units of a sequence) over all of them
+        unsigned long long n = 0;
+        for (int s0 = 0; s0 < C.num_seqs; s0 += 32) {
+            const uint32_t u = s0 == 0 ? u_first : s0 + lane < C.num_seqs ? dec_units(C, s0 + lane, unit) : 0;
+            n += __reduce_add_sync(0xFFFFFFFFu, u ? f(u) : 0u);
+        }
+        return n * (unsigned long long)per_seq;
+    };
+    const unsigned long long total = sum([](uint32_t u) { return u; }), share = total / P.teams + 1;
+    const unsigned long long items = (unsigned long long)C.num_seqs * per_seq;
+    uint32_t hi = (uint32_t)(2 * share < 0x7FFFFFFF ? 2 * share : 0x7FFFFFFF), lo = hi / 2;   // hi is enough: total / hi + items <= teams
+    if (2 * items <= P.teams)
+        while (hi - lo > 0 && hi > P.min_units) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (sum([&](uint32_t u) { return (u + mid - 1) / mid; }) <= (unsigned long long)P.teams) hi = mid; else lo = mid + 1;
+        }
+    return max(hi, (uint32_t)P.min_units);
+}
 
 // one row's sum and output
 __device__ __forceinline__ void dec_store4(int16_t* o, const float4& n, float den)
@@ -116,7 +141,7 @@ __device__ __forceinline__ void dec_store4(int16_t* o, const float4& n, float de
 
 // A team is one warp (many items: nothing waits for another warp) or the CTA (few, long items).
 template <int kHD, int kTiles, int kTeam>
-__global__ void __launch_bounds__(kDecThreads, kTiles == 1 ? kDecCtasPerSm : 2)
+__global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(kTiles))
 paged_decode_kernel(const __grid_constant__ DecodeParams P)
 {
     constexpr int kRows = 8 * kTiles, kSteps = kHD / 32, kCols = kHD / 8, kUnit = kTeam * kDecChunk, kRow = dec_row_floats(kHD);
@@ -134,58 +159,36 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
     const int team = blockIdx.x * (kDecWarps / kTeam) + warp / kTeam, tw = warp % kTeam, tt = threadIdx.x % kTeamThreads;
     const int gqa = P.a.n_head / C.n_head_kv, per_seq = C.n_head_kv * P.row_groups;
     auto team_sync = [] { if (kTeam > 1) __syncthreads(); else __syncwarp(); };
-    auto units_of = [&](int s) { const int n = paged_len(C, s); return n <= 0 ? 1 : (n + kUnit - 1) / kUnit; };
 
-    // ---- the units of all items, and the sequence that holds this team's start (every warp for itself)
-    DecodeCut W = {};
-    const long long u_first = lane < C.num_seqs ? (long long)units_of(lane) * per_seq : 0;
-    for (int s0 = 0; s0 < C.num_seqs; s0 += 32) {
-        long long u = s0 == 0 ? u_first : s0 + lane < C.num_seqs ? (long long)units_of(s0 + lane) * per_seq : 0;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) u += __shfl_xor_sync(0xFFFFFFFFu, u, off);
-        W.total += u;
-    }
-    const long long most = (W.total + P.min_units - 1) / P.min_units, all = (long long)gridDim.x * (kDecWarps / kTeam);
-    W.teams = (int)(most < all ? most : all);
-    if (team >= W.teams) return;
-    W.tol = max(1ll, W.total / W.teams / 8);
-    long long x = W.cut(team), a = 0;
-    int seq = 0;
-    for (int s0 = 0; s0 < C.num_seqs; s0 += 32) {
-        const long long u = s0 == 0 ? u_first : s0 + lane < C.num_seqs ? (long long)units_of(s0 + lane) * per_seq : 0;
-        long long upto = u;
+    // ---- this team's part: part `part` of `parts` of item `item` of sequence seq; slot0: the item's first slot
+    const uint32_t u_first = lane < C.num_seqs ? dec_units(C, lane, kUnit) : 0;
+    const uint32_t most = dec_part_units(P, kUnit, per_seq, u_first);
+    int seq = -1, parts = 0, slot0 = 0;
+    long long left = team;                                         // teams of the items from here on that come before this one
+    uint32_t units = 0;
+    for (int s0 = 0; s0 < C.num_seqs && seq < 0; s0 += 32) {
+        const uint32_t u = s0 == 0 ? u_first : s0 + lane < C.num_seqs ? dec_units(C, s0 + lane, kUnit) : 0;
+        const uint32_t n = (u + most - 1) / most;                  // parts of an item
+        unsigned long long mine = (unsigned long long)n * per_seq | (unsigned long long)(n > 1 ? n * per_seq : 0) << 32, upto = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const long long o = __shfl_up_sync(0xFFFFFFFFu, upto, off);
+            const unsigned long long o = __shfl_up_sync(0xFFFFFFFFu, upto, off);
             if (lane >= off) upto += o;
         }
-        const unsigned over = __ballot_sync(0xFFFFFFFFu, a + upto > x);
-        if (over) {
-            const int l = __ffs(over) - 1;
-            seq = s0 + l;
-            a += __shfl_sync(0xFFFFFFFFu, upto - u, l);
-            break;
-        }
-        a += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        const unsigned over = __ballot_sync(0xFFFFFFFFu, (long long)(uint32_t)upto > left);
+        const int l = over ? __ffs(over) - 1 : 31;
+        const unsigned long long before = __shfl_sync(0xFFFFFFFFu, over ? upto - mine : upto, l);
+        left -= (uint32_t)before;
+        slot0 += (int)(before >> 32);
+        if (over) { seq = s0 + l; units = __shfl_sync(0xFFFFFFFFu, u, l); parts = (int)__shfl_sync(0xFFFFFFFFu, n, l); }
     }
-    int units = units_of(seq), item = (int)((x - a) / units);      // item of the sequence
-    a += (long long)item * units;                                  // its first unit
-    x = W.snap(x, a, a + units);
-    const long long next = W.cut(team + 1);                        // this team's end lies in, or at the end of, an item met below
+    if (seq < 0) return;                                           // more teams than parts
+    const int item = (int)left / parts, part = (int)left - item * parts;
+    if (parts > 1) slot0 += item * parts;
     const float to_log2 = P.a.scale * 1.4426950408889634f;
     const int ps = 1 << C.page_shift;
-
-    while (true) {
-        if (x >= a + units) {                                      // the start moved to the item's end, or the item is done
-            a += units; x = a;
-            if (++item == per_seq) {
-                if (++seq == C.num_seqs) break;
-                item = 0; units = units_of(seq);
-            }
-        }
-        long long end = a + units;
-        if (next < end) end = W.snap(next, a, end);
-        if (x >= end) break;
+    const bool q_aligned = ((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0;
+    {
         const int kvh = item / P.row_groups, row_base = (item - kvh * P.row_groups) * kRows;
         int lo, hi;
         paged_rows(C, seq, lo, hi);
@@ -193,7 +196,8 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
         if (rows > 0) {
             const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // row r sees min(before + token, room) positions
             const int least = min(before + row_base / gqa, room), most_seen = min(before + (row_base + rows - 1) / gqa, room);
-            const int t_lo = (int)(x - a) * kUnit, t_hi = (int)min((end - a) * kUnit, (long long)most_seen);
+            const int t_lo = (int)((unsigned long long)units * part / parts) * kUnit;
+            const int t_hi = (int)min((long long)((unsigned long long)units * (part + 1) / parts) * kUnit, (long long)most_seen);
             const int* table = C.table + (size_t)seq * C.table_stride;
             bool missing = false;
             // page of position t; -1: none, or t not below t_hi
@@ -226,6 +230,17 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
             // a chunk has one page, or two of 16 positions: K rows 4 g + u lie in the half of g >> 2, V rows 8 t4 + u of t4 >> 1
             const int kt = (g >> 2) * 16, vt = (t4 >> 1) * 16;
             int pk = page_at(t0 + kt), pv = page_at(t0 + vt), pk_next = page_at(t0 + kUnit + kt), pv_next = page_at(t0 + kUnit + vt);
+            float4 qv[kRows];                                      // lane: dims 4 lane .. + 3 of every row
+#pragma unroll
+            for (int r = 0; r < kRows; r++) {
+                qv[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < rows && 4 * lane < kHD) {
+                    const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
+                    const float* q = P.a.q + (size_t)(lo + tok) * P.a.q_stride + (size_t)(kvh * gqa + head) * kHD + 4 * lane;
+                    if (q_aligned) qv[r] = *reinterpret_cast<const float4*>(q);
+                    else qv[r] = make_float4(q[0], q[1], q[2], q[3]);
+                }
+            }
             if (t0 < t_hi) {
                 const uint32_t at = row_at(pv, t0 + 8 * t4);
                 fetch_k(t0, pk); fetch_s(sk, C.sk, at); fetch_s(sv, C.sv, at); fetch_v(at);
@@ -236,19 +251,11 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
             int limit[kTiles];                                     // positions that the lane's row may see
 #pragma unroll
             for (int i = 0; i < kTiles; i++) factor[i] = 0.f;
-            team_sync();                                           // the last item's digits and sums have been read
             auto& digits = room_s[warp].q.d;
 #pragma unroll
             for (int r = 0; r < kRows; r++) {
                 if (r >= rows) break;
-                const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
-                const float* q = P.a.q + (size_t)(lo + tok) * P.a.q_stride + (size_t)(kvh * gqa + head) * kHD + 4 * lane;
-                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (4 * lane < kHD) {
-                    if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) f = *reinterpret_cast<const float4*>(q);
-                    else f = make_float4(q[0], q[1], q[2], q[3]);
-                }
-                const float e[4] = {f.x, f.y, f.z, f.w};
+                const float e[4] = {qv[r].x, qv[r].y, qv[r].z, qv[r].w};
                 uint32_t bits = 0;                                 // of the largest magnitude; a NaN is the largest
 #pragma unroll
                 for (int j = 0; j < 4; j++) bits = max(bits, __float_as_uint(e[j]) & 0x7FFFFFFFu);
@@ -406,18 +413,18 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                 l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
                 l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
             }
-            const bool alone = x == a && end == a + units;
+            const bool alone = parts == 1;
             auto out_at = [&](int r, int d) {
                 const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
                 return P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD + d;
             };
-            float* part = P.slots + (size_t)(2 * team + (x == a ? 1 : 0)) * kSlot;   // a team has at most one part of an item that began before, and one of one that goes on
+            float* mine = P.slots + (size_t)(slot0 + part) * kSlot;
             if (kTeam == 1) {
 #pragma unroll
                 for (int i = 0; i < kTiles; i++) {
                     const int r = i * 8 + g;
                     if (r >= rows) continue;
-                    if (!alone && t4 == 0) { part[kRows * kHD + 2 * r] = m[i]; part[kRows * kHD + 2 * r + 1] = l[i]; }
+                    if (!alone && t4 == 0) { mine[kRows * kHD + 2 * r] = m[i]; mine[kRows * kHD + 2 * r + 1] = l[i]; }
 #pragma unroll
                     for (int e = 0; e < 2; e++)
 #pragma unroll
@@ -425,7 +432,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                             const float4 n = make_float4(acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]);
                             const int d = (2 * t4 + e) * kCols + j;
                             if (alone) dec_store4(out_at(r, d), n, l[i]);
-                            else *reinterpret_cast<float4*>(part + r * kHD + d) = n;
+                            else *reinterpret_cast<float4*>(mine + r * kHD + d) = n;
                         }
                 }
             } else {
@@ -456,22 +463,18 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                         den += f * l_s[w][r];
                     }
                     if (alone) { dec_store4(out_at(r, d), num, den); continue; }
-                    *reinterpret_cast<float4*>(part + r * kHD + d) = num;
-                    if (d == 0) { part[kRows * kHD + 2 * r] = mm; part[kRows * kHD + 2 * r + 1] = den; }
+                    *reinterpret_cast<float4*>(mine + r * kHD + d) = num;
+                    if (d == 0) { mine[kRows * kHD + 2 * r] = mm; mine[kRows * kHD + 2 * r + 1] = den; }
                 }
             }
             if (!alone) {
-                // teams whose starts lie strictly inside this item: c_lo to c_hi; its first part is team c_lo - 1's
-                const long long A = a + W.tol, B = a + units - W.tol;
-                const int c_lo = (int)((A * W.teams + W.total - 1) / W.total), c_hi = (int)(((B + 1) * W.teams + W.total - 1) / W.total) - 1;
-                const int c0 = c_lo - 1, parts = c_hi - c0 + 1, ngroups = (parts + kDecGroup - 1) / kDecGroup;
-                auto slot_of = [&](int n) { return 2 * (c0 + n) + (n == 0 ? 1 : 0); };   // of part n
+                const int ngroups = (parts + kDecGroup - 1) / kDecGroup;
                 // true in the team that is the last of `n` to come
                 auto last_of = [&](unsigned int* counter, int n) {
-                    __threadfence();
                     team_sync();
                     int last = 0;
                     if (tt == 0) {
+                        __threadfence();                            // with the barrier before it: all the team's writes
                         last = atomicAdd(counter, 1u) == (unsigned)n - 1;
                         if (last) *counter = 0;
                         if (kTeam > 1) last_s = last;
@@ -489,7 +492,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                         float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
                         for (int j = 0; j < n; j++) {
-                            const float* p = P.slots + (size_t)slot_of(first + j * step) * kSlot;
+                            const float* p = P.slots + (size_t)(slot0 + first + j * step) * kSlot;
                             const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + kRows * kHD + stats + 2 * r));
                             const float4 y = __ldcg(reinterpret_cast<const float4*>(p + r * kHD + d));
                             const float mn = fmaxf(mm, ml.x), f0 = dec_exp2(mm - mn), f = dec_exp2(ml.x - mn);
@@ -498,23 +501,23 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                             mm = mn;
                         }
                         if (finish) { dec_store4(out_at(r, d), num, den); continue; }
-                        float* p = P.slots + (size_t)slot_of(first) * kSlot;
+                        float* p = P.slots + (size_t)(slot0 + first) * kSlot;
                         *reinterpret_cast<float4*>(p + r * kHD + d) = num;      // read by this thread alone; the statistics by all of the row
                         if (d == 0) *reinterpret_cast<float2*>(p + kRows * kHD + 2 * kRows + 2 * r) = make_float2(mm, den);
                     }
                 };
-                const int group = (team - c0) / kDecGroup, n_in = min(kDecGroup, parts - group * kDecGroup);
-                if (last_of(P.groups_done + slot_of(group * kDecGroup), n_in)) {
+                const int group = part / kDecGroup, n_in = min(kDecGroup, parts - group * kDecGroup);
+                if (last_of(P.groups_done + slot0 + group * kDecGroup, n_in)) {
                     add_up(group * kDecGroup, 1, n_in, 0, ngroups == 1);
                     if (ngroups > 1 && last_of(P.items_done + (size_t)seq * per_seq + item, ngroups)) add_up(0, kDecGroup, ngroups, 2 * kRows, true);
                 }
             }
         }
-        x = end;
-        if (end < a + units) break;                                 // the range ends inside the item
     }
 }
-// the workspace: partial results, then the counters; the same places for every call on a device
+
+// The workspace: partial results, then the counters; the same places for every call on a device.  The parts of cut items
+// are at most 2 * teams: an item of u units has at most 2 u / (units of a part).
 static int64_t dec_teams(int team) { return (int64_t)sm_count() * kDecCtasPerSm * (kDecWarps / team); }
 static int64_t dec_slot_bytes() { return std::max(2 * dec_teams(kDecWarps) * dec_slot_floats(kDecMaxRows), 2 * dec_teams(1) * dec_slot_floats(8)) * 4; }
 static int64_t dec_group_bytes() { return 2 * dec_teams(1) * 4; }
@@ -525,22 +528,25 @@ int64_t paged_decode_workspace_bytes(int n_head, int n_head_kv, int num_seqs, in
 }
 
 template <int kHD, int kTiles, int kTeam>
-static int decode_launch(DecodeParams P, long long units, void* stream, const char* who)
+static int decode_launch(DecodeParams P, void* stream, const char* who)
 {
-    const long long ctas = (units + P.min_units - 1) / P.min_units, most = (long long)sm_count() * kDecCtasPerSm * (kDecWarps / kTeam);
-    const long long teams = std::max(1ll, std::min(ctas, most));
-    return launch(paged_decode_kernel<kHD, kTiles, kTeam>, dim3((unsigned)((teams * kTeam + kDecWarps - 1) / kDecWarps)), dim3(kDecThreads), 0, stream, who, P);
+    // at most, by the caller's bounds: every item whole, and what cutting adds; a grid for less than all resident teams
+    P.teams = (int)dec_teams(kTeam) * dec_ctas_per_sm(kTiles) / kDecCtasPerSm;
+    const long long items = (long long)P.a.c.num_seqs * P.a.c.n_head_kv * P.row_groups;
+    const long long parts = (P.a.c.max_len + (long long)kTeam * kDecChunk * P.min_units - 1) / ((long long)kTeam * kDecChunk * P.min_units);
+    const long long grid = (std::min(items * parts, items + P.teams) * kTeam + kDecWarps - 1) / kDecWarps;
+    if (grid > 0x7FFFFFFF) return fail(S12_ERR_TOO_LARGE, "%s: %lld sequences' heads", who, items);
+    return launch(paged_decode_kernel<kHD, kTiles, kTeam>, dim3((unsigned)grid), dim3(kDecThreads), 0, stream, who, P);
 }
 template <int kHD>
 static int decode_launch_hd(DecodeParams P, int tiles, void* stream, const char* who)
 {
     const PagedAttn& A = P.a;
     const long long items = (long long)A.c.num_seqs * A.c.n_head_kv * P.row_groups;
-    auto units = [&](int team) { return items * ((A.max_len + team * kDecChunk - 1) / (team * kDecChunk)); };   // at most, by the caller's bounds
     P.min_units = env_knob("S12_PAGED_MIN_UNITS", 2);
-    if (tiles == 2) return decode_launch<kHD, 2, kDecWarps>(P, units(kDecWarps), stream, who);
-    if (items >= env_knob("S12_PAGED_ITEMS", 1000)) return decode_launch<kHD, 1, 1>(P, units(1), stream, who);
-    return decode_launch<kHD, 1, kDecWarps>(P, units(kDecWarps), stream, who);
+    if (tiles == 2) return decode_launch<kHD, 2, kDecWarps>(P, stream, who);
+    if (items >= env_knob("S12_PAGED_ITEMS", 1000)) return decode_launch<kHD, 1, 1>(P, stream, who);
+    return decode_launch<kHD, 1, kDecWarps>(P, stream, who);
 }
 
 // 1: not a shape of this kernel
