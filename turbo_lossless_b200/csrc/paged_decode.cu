@@ -43,6 +43,7 @@ struct DecodeParams {
     int row_groups;             // groups of rows of a kv head
     int min_units;              // units of a part, at least
     int teams;                  // that are resident together
+    uint32_t gqa_mul;           // ceil(2^20 / query heads of a kv head): x / that for x below 2^10
 };
 
 __host__ __device__ constexpr int dec_row_floats(int hd) { return hd + hd / 8; }   // padded: the lanes of a store meet different banks
@@ -98,6 +99,8 @@ __device__ __forceinline__ void load_v(VRow<kHD>& r, const int8_t* row, int g)
 }
 
 
+// floor(n / d): 64-bit divisions take long
+__device__ __forceinline__ unsigned long long div_small(unsigned long long n, uint32_t d) { return n >> 32 ? n / d : (uint32_t)n / d; }
 // units of sequence s, in steps of `unit` positions; a sequence without positions has one
 __device__ __forceinline__ uint32_t dec_units(const PagedArgs& C, int s, int unit)
 {
@@ -105,38 +108,45 @@ __device__ __forceinline__ uint32_t dec_units(const PagedArgs& C, int s, int uni
     return n <= 0 ? 1u : (uint32_t)(n + unit - 1) / (uint32_t)unit;
 }
 // The most units of a part: the least that gives all items' parts to resident teams.  With so many items that this would
-// cut nothing or nearly nothing, twice a team's share: only what is far longer than the others is cut.  For a whole warp.
-__device__ __forceinline__ uint32_t dec_part_units(const DecodeParams& P, int unit, int per_seq, uint32_t u_first)
+// cut nothing or nearly nothing, twice a team's share: only what is far longer than the others is cut.  For a whole warp;
+// a lane looks at `per_lane` neighbouring sequences.
+__device__ __forceinline__ uint32_t dec_part_units(const DecodeParams& P, int unit, int per_seq, int per_lane)
 {
     const PagedArgs& C = P.a.c;
-    const int lane = threadIdx.x & 31;
-    auto sum = [&](auto f) {                                       // of f(units of a sequence) over all of them
-        unsigned long long n = 0;
-        for (int s0 = 0; s0 < C.num_seqs; s0 += 32) {
-            const uint32_t u = s0 == 0 ? u_first : s0 + lane < C.num_seqs ? dec_units(C, s0 + lane, unit) : 0;
-            n += __reduce_add_sync(0xFFFFFFFFu, u ? f(u) : 0u);
+    const int first = (threadIdx.x & 31) * per_lane, end = min(first + per_lane, C.num_seqs);
+    auto sum = [&](uint32_t most) {                                // parts of all items; most = 0: their units
+        uint32_t n = 0;
+#pragma unroll 4
+        for (int s = first; s < end; s++) {
+            const uint32_t u = dec_units(C, s, unit);
+            n += most ? (u + most - 1) / most : u;
         }
-        return n * (unsigned long long)per_seq;
+        return (unsigned long long)__reduce_add_sync(0xFFFFFFFFu, n) * (unsigned long long)per_seq;
     };
-    const unsigned long long total = sum([](uint32_t u) { return u; }), share = total / P.teams + 1;
-    const unsigned long long items = (unsigned long long)C.num_seqs * per_seq;
-    uint32_t hi = (uint32_t)(2 * share < 0x7FFFFFFF ? 2 * share : 0x7FFFFFFF), lo = hi / 2;   // hi is enough: total / hi + items <= teams
-    if (2 * items <= P.teams)
-        while (hi - lo > 0 && hi > P.min_units) {
+    const unsigned long long share = div_small(sum(0), P.teams) + 1;
+    uint32_t hi = (uint32_t)min(2 * share, 0x7FFFFFFFull), lo = hi / 2;   // hi is enough: units / hi + items <= teams
+    if (2ull * C.num_seqs * per_seq <= P.teams)
+        while (lo < hi && hi > P.min_units) {
             const uint32_t mid = (lo + hi) / 2;
-            if (sum([&](uint32_t u) { return (u + mid - 1) / mid; }) <= (unsigned long long)P.teams) hi = mid; else lo = mid + 1;
+            if (sum(mid) <= (unsigned long long)P.teams) hi = mid; else lo = mid + 1;
         }
     return max(hi, (uint32_t)P.min_units);
 }
 
-// one row's sum and output
-__device__ __forceinline__ void dec_store4(int16_t* o, const float4& n, float den)
+// four values over their sum as bf16
+__device__ __forceinline__ uint2 dec_bf16x4(const float4& n, float rd)
 {
-    const float rd = den == 0.f ? 0.f : 1.f / den;                 // no position at all: zero
-    const uint32_t lo = (uint16_t)paged_bf16_rne(n.x * rd) | (uint32_t)(uint16_t)paged_bf16_rne(n.y * rd) << 16;
-    const uint32_t hi = (uint16_t)paged_bf16_rne(n.z * rd) | (uint32_t)(uint16_t)paged_bf16_rne(n.w * rd) << 16;
-    if ((reinterpret_cast<uintptr_t>(o) & 7) == 0) *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
-    else { o[0] = (int16_t)lo; o[1] = (int16_t)(lo >> 16); o[2] = (int16_t)hi; o[3] = (int16_t)(hi >> 16); }
+    uint32_t lo, hi;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(n.y * rd), "f"(n.x * rd));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(n.w * rd), "f"(n.z * rd));
+    return make_uint2(lo, hi);
+}
+__device__ __forceinline__ float dec_over(float den) { return den == 0.f ? 0.f : 1.f / den; }   // no position at all: zeros
+__device__ __forceinline__ void dec_store4(int16_t* o, const float4& n, float rd, bool aligned)
+{
+    const uint2 y = dec_bf16x4(n, rd);
+    if (aligned) *reinterpret_cast<uint2*>(o) = y;
+    else { o[0] = (int16_t)y.x; o[1] = (int16_t)(y.x >> 16); o[2] = (int16_t)y.y; o[3] = (int16_t)(y.y >> 16); }
 }
 
 // A team is one warp (many items: nothing waits for another warp) or the CTA (few, long items).
@@ -161,32 +171,47 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
     auto team_sync = [] { if (kTeam > 1) __syncthreads(); else __syncwarp(); };
 
     // ---- this team's part: part `part` of `parts` of item `item` of sequence seq; slot0: the item's first slot
-    const uint32_t u_first = lane < C.num_seqs ? dec_units(C, lane, kUnit) : 0;
-    const uint32_t most = dec_part_units(P, kUnit, per_seq, u_first);
+    const int per_lane = (C.num_seqs + 31) >> 5;
+    const uint32_t most = dec_part_units(P, kUnit, per_seq, per_lane);
     int seq = -1, parts = 0, slot0 = 0;
-    long long left = team;                                         // teams of the items from here on that come before this one
-    uint32_t units = 0;
-    for (int s0 = 0; s0 < C.num_seqs && seq < 0; s0 += 32) {
-        const uint32_t u = s0 == 0 ? u_first : s0 + lane < C.num_seqs ? dec_units(C, s0 + lane, kUnit) : 0;
-        const uint32_t n = (u + most - 1) / most;                  // parts of an item
-        unsigned long long mine = (unsigned long long)n * per_seq | (unsigned long long)(n > 1 ? n * per_seq : 0) << 32, upto = mine;
+    uint32_t units = 0, left = team;                               // left: teams of the sequences from here on that come before this one
+    // the lane whose sequences hold the team, then the sequence: two scans, each of (teams, slots) of a lane's sequences
+    for (int s0 = 0, per = per_lane, n_seqs = C.num_seqs; ; ) {
+        uint32_t n = 0, cut = 0, u = 0, parts_of = 0;
+#pragma unroll 4
+        for (int s = s0 + lane * per; s < min(s0 + (lane + 1) * per, n_seqs); s++) {
+            u = dec_units(C, s, kUnit);
+            parts_of = (u + most - 1) / most;
+            n += parts_of; cut += parts_of > 1 ? parts_of : 0;
+        }
+        unsigned long long mine = (unsigned long long)(n * per_seq) | (unsigned long long)(cut * per_seq) << 32, upto = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const unsigned long long o = __shfl_up_sync(0xFFFFFFFFu, upto, off);
             if (lane >= off) upto += o;
         }
-        const unsigned over = __ballot_sync(0xFFFFFFFFu, (long long)(uint32_t)upto > left);
+        const unsigned over = __ballot_sync(0xFFFFFFFFu, (uint32_t)upto > left);
         const int l = over ? __ffs(over) - 1 : 31;
         const unsigned long long before = __shfl_sync(0xFFFFFFFFu, over ? upto - mine : upto, l);
-        left -= (uint32_t)before;
-        slot0 += (int)(before >> 32);
-        if (over) { seq = s0 + l; units = __shfl_sync(0xFFFFFFFFu, u, l); parts = (int)__shfl_sync(0xFFFFFFFFu, n, l); }
+        if (over || per == 1) { left -= (uint32_t)before; slot0 += (int)(before >> 32); }
+        if (per == 1) {
+            if (over) { seq = s0 + l; units = __shfl_sync(0xFFFFFFFFu, u, l); parts = (int)__shfl_sync(0xFFFFFFFFu, parts_of, l); break; }
+            s0 += 32;
+            if (s0 >= n_seqs) break;
+            continue;
+        }
+        if (!over) break;
+        s0 += l * per;
+        n_seqs = min(s0 + per, n_seqs);
+        per = 1;
     }
     if (seq < 0) return;                                           // more teams than parts
-    const int item = (int)left / parts, part = (int)left - item * parts;
+    const int item = (int)(left / (uint32_t)parts), part = (int)left - item * parts;
     if (parts > 1) slot0 += item * parts;
+    auto token_of = [&](int row) { return (int)((uint32_t)row * P.gqa_mul >> 20); };
     const float to_log2 = P.a.scale * 1.4426950408889634f;
     const int ps = 1 << C.page_shift;
+    const bool out_aligned = ((reinterpret_cast<uintptr_t>(P.a.out) & 7) | (P.a.out_stride & 3)) == 0;
     const bool q_aligned = ((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0;
     {
         const int kvh = item / P.row_groups, row_base = (item - kvh * P.row_groups) * kRows;
@@ -195,7 +220,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
         const int rows = min(kRows, (hi - lo) * gqa - row_base);   // rows of this item; 0 or less: none
         if (rows > 0) {
             const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // row r sees min(before + token, room) positions
-            const int least = min(before + row_base / gqa, room), most_seen = min(before + (row_base + rows - 1) / gqa, room);
+            const int least = min(before + token_of(row_base), room), most_seen = min(before + token_of(row_base + rows - 1), room);
             const int t_lo = (int)((unsigned long long)units * part / parts) * kUnit;
             const int t_hi = (int)min((long long)((unsigned long long)units * (part + 1) / parts) * kUnit, (long long)most_seen);
             const int* table = C.table + (size_t)seq * C.table_stride;
@@ -235,7 +260,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
             for (int r = 0; r < kRows; r++) {
                 qv[r] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (r < rows && 4 * lane < kHD) {
-                    const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
+                    const int tok = token_of(row_base + r), head = row_base + r - tok * gqa;
                     const float* q = P.a.q + (size_t)(lo + tok) * P.a.q_stride + (size_t)(kvh * gqa + head) * kHD + 4 * lane;
                     if (q_aligned) qv[r] = *reinterpret_cast<const float4*>(q);
                     else qv[r] = make_float4(q[0], q[1], q[2], q[3]);
@@ -262,7 +287,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                 bits = __reduce_max_sync(0xFFFFFFFFu, bits);
                 const float top = __uint_as_float(bits);
                 const bool fine = top >= 1e-30f && bits < 0x7F800000u;   // rows of smaller ones count as zero
-                const float inv = fine ? kDigits / top : 0.f;
+                const float inv = fine ? __fdividef(kDigits, top) : 0.f;
                 uint32_t y[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) y[j] = __float_as_uint(fmaf(fine ? e[j] : 0.f, inv, 12582912.f + 128.f));   // 256 hi + lo + 128
@@ -271,7 +296,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                     *reinterpret_cast<uint32_t*>(&digits[0][r][4 * lane]) = prmt(p01, p23, 0x7632u);
                     *reinterpret_cast<uint32_t*>(&digits[1][r][4 * lane]) = prmt(p01, p23, 0x5410u) ^ 0x80808080u;
                 }
-                if ((r & 7) == g) factor[r >> 3] = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : top / kDigits * to_log2;
+                if ((r & 7) == g) factor[r >> 3] = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : top * (1.f / kDigits) * to_log2;
             }
             __syncwarp();
 #pragma unroll
@@ -284,7 +309,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                     const uint2 l = *reinterpret_cast<const uint2*>(&digits[1][r][k_dim<kHD>(s, t4)]);
                     qa[i][s][0] = there ? h.x : 0u; qa[i][s][1] = there ? l.x : 0u; qa[i][s][2] = there ? h.y : 0u; qa[i][s][3] = there ? l.y : 0u;
                 }
-                limit[i] = there ? min(before + (row_base + r) / gqa, room) : 0;
+                limit[i] = there ? min(before + token_of(row_base + r), room) : 0;
             }
             float acc[kTiles][kCols][2], m[kTiles], l[kTiles];
 #pragma unroll
@@ -415,7 +440,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
             }
             const bool alone = parts == 1;
             auto out_at = [&](int r, int d) {
-                const int tok = (row_base + r) / gqa, head = row_base + r - tok * gqa;
+                const int tok = token_of(row_base + r), head = row_base + r - tok * gqa;
                 return P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD + d;
             };
             float* mine = P.slots + (size_t)(slot0 + part) * kSlot;
@@ -424,6 +449,8 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                 for (int i = 0; i < kTiles; i++) {
                     const int r = i * 8 + g;
                     if (r >= rows) continue;
+                    const float rd = dec_over(l[i]);
+                    int16_t* o = out_at(r, 0);
                     if (!alone && t4 == 0) { mine[kRows * kHD + 2 * r] = m[i]; mine[kRows * kHD + 2 * r + 1] = l[i]; }
 #pragma unroll
                     for (int e = 0; e < 2; e++)
@@ -431,7 +458,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                         for (int j = 0; j < kCols; j += 4) {
                             const float4 n = make_float4(acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]);
                             const int d = (2 * t4 + e) * kCols + j;
-                            if (alone) dec_store4(out_at(r, d), n, l[i]);
+                            if (alone) dec_store4(o + d, n, rd, out_aligned);
                             else *reinterpret_cast<float4*>(mine + r * kHD + d) = n;
                         }
                 }
@@ -462,7 +489,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                         num.x += f * y.x; num.y += f * y.y; num.z += f * y.z; num.w += f * y.w;
                         den += f * l_s[w][r];
                     }
-                    if (alone) { dec_store4(out_at(r, d), num, den); continue; }
+                    if (alone) { dec_store4(out_at(r, d), num, dec_over(den), out_aligned); continue; }
                     *reinterpret_cast<float4*>(mine + r * kHD + d) = num;
                     if (d == 0) { mine[kRows * kHD + 2 * r] = mm; mine[kRows * kHD + 2 * r + 1] = den; }
                 }
@@ -500,7 +527,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                             den = den * f0 + f * ml.y;
                             mm = mn;
                         }
-                        if (finish) { dec_store4(out_at(r, d), num, den); continue; }
+                        if (finish) { dec_store4(out_at(r, d), num, dec_over(den), out_aligned); continue; }
                         float* p = P.slots + (size_t)(slot0 + first) * kSlot;
                         *reinterpret_cast<float4*>(p + r * kHD + d) = num;      // read by this thread alone; the statistics by all of the row
                         if (d == 0) *reinterpret_cast<float2*>(p + kRows * kHD + 2 * kRows + 2 * r) = make_float2(mm, den);
@@ -543,7 +570,7 @@ static int decode_launch_hd(DecodeParams P, int tiles, void* stream, const char*
 {
     const PagedAttn& A = P.a;
     const long long items = (long long)A.c.num_seqs * A.c.n_head_kv * P.row_groups;
-    P.min_units = env_knob("S12_PAGED_MIN_UNITS", 2);
+    P.min_units = env_knob("S12_PAGED_MIN_UNITS", 4);
     if (tiles == 2) return decode_launch<kHD, 2, kDecWarps>(P, stream, who);
     if (items >= env_knob("S12_PAGED_ITEMS", 1000)) return decode_launch<kHD, 1, 1>(P, stream, who);
     return decode_launch<kHD, 1, kDecWarps>(P, stream, who);
@@ -564,6 +591,7 @@ int paged_decode_launch(const PagedAttn& A, void* stream, const char* who)
     P.groups_done = (unsigned int*)((char*)A.workspace + dec_slot_bytes());
     P.items_done = P.groups_done + dec_group_bytes() / 4;
     const int tiles = rows <= 8 ? 1 : 2;
+    P.gqa_mul = (uint32_t)(((1 << 20) + gqa - 1) / gqa);
     P.row_groups = (int)((rows + 8 * tiles - 1) / (8 * tiles));
     if (hd == 64) return decode_launch_hd<64>(P, tiles, stream, who);
     if (hd == 96) return decode_launch_hd<96>(P, tiles, stream, who);
