@@ -8,10 +8,10 @@ import sys
 _PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_PKG, "csrc")
 LIB_PATH = os.path.join(_PKG, "libsplit12_b200.so")
-SOURCES = ["runtime.cu", "decompress.cu", "patches.cu", "gemv.cu", "gemv_stream.cu", "gemm.cu", "gemm_tc.cu", "gemm_stream.cu", "pack.cu", "comm.cu", "step.cu", "loader.cu", "moe.cu", "paged.cu", "paged_decode.cu", "host.cpp"]
+SOURCES = ["runtime.cu", "decompress.cu", "patches.cu", "gemv.cu", "gemv_stream.cu", "gemm.cu", "gemm_tc.cu", "gemm_stream.cu", "pack.cu", "comm.cu", "step.cu", "loader.cu", "moe.cu", "paged.cu", "paged_decode.cu", "paged_prompt.cu", "host.cpp"]
 # sources compiled without --use_fast_math: the decode-step kernels use sincosf / expf / division on values
 # where the fast intrinsics lose digits (RoPE angles of hundreds of radians)
-ACCURATE_MATH = {"step.cu", "moe.cu", "paged.cu", "paged_decode.cu"}
+ACCURATE_MATH = {"step.cu", "moe.cu", "paged.cu", "paged_decode.cu", "paged_prompt.cu"}
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default", "--use_fast_math"]
 

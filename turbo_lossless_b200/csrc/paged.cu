@@ -331,7 +331,7 @@ int s12_attention_paged_async(const float* q, int q_stride, const S12PagedKv* kv
     if ((rc = paged_status(P.c, who)) != S12_OK) return rc;
     P.q = q; P.out = (int16_t*)out_bf16; P.q_stride = q_stride; P.out_stride = out_stride; P.n_head = n_head; P.scale = scale;
     P.max_new = batch->max_new; P.c.max_len = batch->max_len; P.workspace = workspace; P.workspace_bytes = workspace_bytes;
-    if ((rc = paged_decode_launch(P, stream, who)) <= 0) return rc;
+    if ((rc = paged_decode_launch(P, stream, who)) <= 0 || (rc = paged_prompt_launch(P, stream, who)) <= 0) return rc;
     return launch(paged_attention_general_kernel, dim3(batch->num_tokens, n_head), dim3(kGenWarps * 32), 0, stream, who, P);
 }
 

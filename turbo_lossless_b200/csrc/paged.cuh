@@ -76,5 +76,6 @@ struct PagedAttn {
 };
 int64_t paged_decode_workspace_bytes(int n_head, int n_head_kv, int num_seqs, int max_new);
 int paged_decode_launch(const PagedAttn& A, void* stream, const char* who);
+int paged_prompt_launch(const PagedAttn& A, void* stream, const char* who);
 
 }  // namespace s12

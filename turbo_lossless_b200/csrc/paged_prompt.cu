@@ -1,0 +1,544 @@
+// Causal attention of prompts and chunks of prompts over the paged INT8 cache on the 5th-generation tensor cores
+// (tcgen05.mma, scores, weights and sums in tensor memory), head_dim 64 / 96 / 128.
+//
+// Bound: the two products, 4 * head_dim FLOP per (row, position), and as much time of the exponentials: 16 a clock of an SM
+// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.
+//
+// A CTA has 256 rows of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
+// products and softmax take turns.  It walks the positions in tiles of 128.
+//   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row: scores from tensor memory, running maximum and sum,
+//                    weights back to tensor memory as bf16 in the place of the scores; the output at the end
+//   warps 8-11       int8 codes from global memory to swizzled shared memory: K to f16, which holds a code exactly, V times
+//                    its scale to bf16; the next tile's loads are in flight meanwhile
+//   warp 12          issues the MMAs from one thread: S = Q K^T (both from shared memory), O += P V (P from tensor memory,
+//                    V with the dims contiguous)
+// Numbers: q is f16 after a power of two of its row takes its largest element to 2^14..2^15 (11 significant bits; a row of
+// bf16 would lose three more); K's scales multiply the scores in 32 bits.  Weights and values are bf16, whose range no
+// scale leaves; sums are 32-bit.  The maximum follows a row's scores only when they exceed it by 2^8, since the sums have
+// to be multiplied then.
+// A position that a row may not see gets weight 0, and its value must be finite for that: values behind the sequence's end
+// are zeros, and one whose scale is not finite is zero with its K scale made NaN, which marks the rows that see it.
+#include "paged.cuh"
+#include <algorithm>
+#include <atomic>
+
+namespace s12 {
+
+constexpr int kPrRows = 128;                        // rows of an MMA
+constexpr int kPrTile = 128;                        // positions of a step
+constexpr int kPrThreads = 512;
+constexpr int kPrScaleStages = 4;
+constexpr unsigned int kPrSite = 0x200000u;         // a wait of this kernel gave up
+constexpr float kPrMostScale = 2e36f;               // times 127 a finite bf16
+constexpr float kPrSlack = 8.f;                     // a maximum may be exceeded by 2^8 before the sums are scaled
+
+__host__ __device__ constexpr int pr_tile_bytes(int hd) { return (hd + 63) / 64 * kPrRows * 128; }   // blocks of 64 dims: [128 rows][128 bytes]
+__host__ __device__ constexpr int pr_smem_bytes(int hd) { return 6 * pr_tile_bytes(hd) + 1024; }
+
+struct PrBars { uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done; };
+
+__device__ __forceinline__ uint32_t pr_elect()
+{
+    uint32_t leader;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+    return leader;
+}
+__device__ __forceinline__ void pr_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pr_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pr_commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pr_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pr_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pr_ld32(uint32_t at, float (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+                   "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+                   "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+                   "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+                 : "r"(at) : "memory");
+}
+__device__ __forceinline__ void pr_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pr_st32(uint32_t at, const uint32_t (&u)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]),
+                   "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]),
+                   "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]),
+                   "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+                 : "memory");
+}
+__device__ __forceinline__ void pr_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float pr_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pr_bf16x2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pr_f16x2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// two at a time
+struct Pair { float x, y; };
+__device__ __forceinline__ Pair mul2(Pair a, Pair b)
+{
+    Pair r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b)
+{
+    Pair r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
+{
+    Pair r;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
+// Operand tiles: blocks of 64 dims, each [128 rows][128 bytes] with the 128-byte swizzle (16-byte chunk c of row r sits at
+// c ^ (r & 7)).  For Q and K the rows are the MMA's M and N and the dims its K (K-major); for V the rows are its K and the
+// dims its N (MN-major: 8-row groups 1024 bytes apart, blocks of 64 dims 16384 apart).
+__device__ __forceinline__ uint32_t pr_chunk(int row, int chunk) { return (uint32_t)((chunk >> 3) * (kPrRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); }
+__device__ __forceinline__ uint64_t pr_desc(uint32_t at, uint32_t lead)
+{
+    return (uint64_t)((at >> 4) & 0x3FFF) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+struct PromptParams { PagedAttn a; int tile_rows; };               // rows of a CTA: 128 or 256
+
+template <int kHD>
+__global__ void __launch_bounds__(kPrThreads, 1)
+paged_prompt_kernel(const __grid_constant__ PromptParams P)
+{
+    constexpr int kTileBytes = pr_tile_bytes(kHD), kPieces = kHD / 16;
+    extern __shared__ __align__(16) uint8_t pr_smem[];
+    __shared__ PrBars bars;
+    __shared__ __align__(16) float sk_s[kPrScaleStages][kPrTile];
+    __shared__ uint32_t absent_s[kPrScaleStages];                  // bit i: positions 16 i .. 16 i + 15 of the tile have no page
+    __shared__ float factor_s[2 * kPrRows];
+    __shared__ uint32_t tmem_s;
+    __shared__ int s_abort;
+    uint8_t* smem = pr_smem + ((1024u - (smem_addr(pr_smem) & 1023u)) & 1023u);
+    uint8_t* q_s = smem, *k_s = smem + 2 * kTileBytes, *v_s = smem + 4 * kTileBytes;
+    const PagedArgs& C = P.a.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int gqa = P.a.n_head / C.n_head_kv;
+    grid_launch_dependents();
+    grid_dependency_wait();
+
+    // ---- this CTA's rows: tiles of all sequences counted from the last, a kv head after the other
+    const int kvh = blockIdx.x % C.n_head_kv;
+    int seq = -1, lo = 0, hi = 0, tile = (int)(blockIdx.x / C.n_head_kv);
+    for (int s1 = C.num_seqs; s1 > 0 && seq < 0; s1 -= 32) {       // sequence s1 - 1 - lane
+        const int s = s1 - 1 - lane;
+        int a = 0, b = 0, n = 0;
+        if (s >= 0) { paged_rows(C, s, a, b); n = b > a ? (int)(((long long)(b - a) * gqa + P.tile_rows - 1) / P.tile_rows) : 0; }
+        int upto = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xFFFFFFFFu, upto, off); if (lane >= off) upto += o; }
+        const unsigned over = __ballot_sync(0xFFFFFFFFu, upto > tile);
+        if (over) {
+            const int l = __ffs(over) - 1;
+            seq = s1 - 1 - l; lo = __shfl_sync(0xFFFFFFFFu, a, l); hi = __shfl_sync(0xFFFFFFFFu, b, l);
+            tile = __shfl_sync(0xFFFFFFFFu, upto, l) - 1 - tile;   // the sequence's last tile, which sees most, comes first
+        } else {
+            tile -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+        }
+    }
+    if (seq < 0) return;                                           // more CTAs than tiles
+    const int row0 = tile * P.tile_rows, rows = min(P.tile_rows, (hi - lo) * gqa - row0);
+    const int n_q = rows > kPrRows ? 2 : 1;                        // row tiles
+    const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // token t sees min(before + t, room) positions
+    const int seen = max(0, min(before + (row0 + rows - 1) / gqa, room)), n = max(1, (seen + kPrTile - 1) / kPrTile);
+
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_addr(&bars.k_full[i]), 4); mbar_init(smem_addr(&bars.v_full[i]), 4);
+            mbar_init(smem_addr(&bars.k_empty[i]), 1); mbar_init(smem_addr(&bars.v_empty[i]), 1);
+            mbar_init(smem_addr(&bars.s_full[i]), 1); mbar_init(smem_addr(&bars.p_full[i]), 4);
+        }
+        mbar_init(smem_addr(&bars.done), 1);
+        mbar_fence_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // ---- q as f16: a warp per row, four dims a lane
+    {
+        const bool q_aligned = ((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0;
+        const float to_log2 = fabsf(P.a.scale) * 1.4426950408889634f, sign = P.a.scale < 0.f ? -1.f : 1.f;
+        constexpr int kFlight = 8;
+        for (int r0 = warp; r0 < n_q * kPrRows; r0 += 16 * kFlight) {
+            float4 v[kFlight];
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) {
+                const int r = r0 + 16 * i, t = (row0 + r) / gqa, head = row0 + r - t * gqa;
+                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < rows && 4 * lane < kHD) {
+                    const float* q = P.a.q + (size_t)(lo + t) * P.a.q_stride + (size_t)(kvh * gqa + head) * kHD + 4 * lane;
+                    if (q_aligned) v[i] = *reinterpret_cast<const float4*>(q);
+                    else v[i] = make_float4(q[0], q[1], q[2], q[3]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) {
+                const int r = r0 + 16 * i;
+                if (r >= n_q * kPrRows) break;
+                const uint32_t a = __float_as_uint(v[i].x) & 0x7FFFFFFFu, b = __float_as_uint(v[i].y) & 0x7FFFFFFFu;
+                const uint32_t c = __float_as_uint(v[i].z) & 0x7FFFFFFFu, d = __float_as_uint(v[i].w) & 0x7FFFFFFFu;
+                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d)));   // a NaN is the largest
+                const int e = (int)(top >> 23) - 127;              // the largest is 2^e and more
+                const bool fine = e >= -100 && e < 128;            // rows of smaller ones count as zero
+                // 2^(14 - e) in two factors, each a normal number
+                const float up = fine ? sign * __uint_as_float((uint32_t)(127 + (14 - e) / 2) << 23) : 0.f;
+                const float up2 = __uint_as_float((uint32_t)(127 + (14 - e) - (14 - e) / 2) << 23);
+                if (!fine) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (4 * lane < kHD)
+                    *reinterpret_cast<uint2*>(q_s + (r / kPrRows) * kTileBytes + pr_chunk(r % kPrRows, lane >> 1) + (lane & 1) * 8) =
+                        make_uint2(pr_f16x2(v[i].x * up * up2, v[i].y * up * up2), pr_f16x2(v[i].z * up * up2, v[i].w * up * up2));
+                if (lane == 0) factor_s[r] = e == 128 ? __uint_as_float(0x7FC00000u) : fine ? fmaxf(ldexpf(to_log2, e - 14), 1e-37f) : 1e-37f;   // above 0: a masked score stays -infinity
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what ordinary stores wrote
+    }
+    pr_fence_before();
+    __syncthreads();
+    pr_fence_after();
+    const uint32_t tmem = tmem_s;
+    auto bar = [](const uint64_t& b) { return smem_addr(&b); };
+    auto wait = [&](const uint64_t& b, int phase) { mbar_wait(smem_addr(&b), (uint32_t)phase & 1, C.status, kPrSite, &s_abort); };
+
+    if (warp < 8) {
+        // ------------------------------ softmax -------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        const int i = warp >> 2, r = i * kPrRows + (warp & 3) * 32 + lane;   // row tile, row of the CTA
+        if (i < n_q) {
+            const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            const uint32_t s_at = mine + i * kPrTile, o_at = mine + 2 * kPrTile + i * 128;
+            const int tok = (row0 + r) / gqa, head = row0 + r - tok * gqa;
+            const int limit = r < rows ? min(before + tok, room) : 0;       // positions that this row sees
+            const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
+            const float factor = factor_s[r];
+            float m = -1e30f;
+            Pair l = {0.f, 0.f};
+            for (int j = 0; j < n; j++) {
+                wait(bars.s_full[i], j);                            // and the tile before it is in the sums
+                pr_fence_after();
+                float x[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; c++) pr_ld32(s_at + 32 * c, x[c]);
+                pr_ld_wait();
+                const float4* sk = reinterpret_cast<const float4*>(sk_s[j % kPrScaleStages]);
+#pragma unroll
+                for (int c = 0; c < kPrTile / 4; c++) {
+                    const float4 k = sk[c];
+                    float (&y)[32] = x[c / 8];
+                    const int e = c % 8 * 4;
+                    const Pair a = mul2({y[e], y[e + 1]}, {k.x, k.y}), b = mul2({y[e + 2], y[e + 3]}, {k.z, k.w});
+                    y[e] = a.x; y[e + 1] = a.y; y[e + 2] = b.x; y[e + 3] = b.y;
+                }
+                const int left = limit - j * kPrTile;               // positions of the tile that the row sees
+                const uint32_t absent = absent_s[j % kPrScaleStages];
+                if (least - j * kPrTile < kPrTile || absent) {
+#pragma unroll
+                    for (int c = 0; c < kPrTile; c++) if (c >= left || (absent >> (c / 16) & 1)) x[c / 32][c % 32] = -INFINITY;
+                }
+                float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < kPrTile; c += 8) {
+                    const float* y = x[c / 32];
+                    const int e = c % 32;
+                    t0 = fmaxf(t0, fmaxf(y[e], y[e + 1])); t1 = fmaxf(t1, fmaxf(y[e + 2], y[e + 3]));
+                    t2 = fmaxf(t2, fmaxf(y[e + 4], y[e + 5])); t3 = fmaxf(t3, fmaxf(y[e + 6], y[e + 7]));
+                }
+                const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * factor;
+                const bool rise = top > m + kPrSlack;
+                if (__any_sync(0xFFFFFFFFu, rise)) {
+                    const float mn = rise ? top : m, f = pr_exp2(m - mn);
+                    m = mn;
+                    l = mul2(l, {f, f});
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < kHD; c += 32) {
+                            float o[32];
+                            pr_ld32(o_at + c, o);
+                            pr_ld_wait();
+                            uint32_t u[32];
+#pragma unroll
+                            for (int d = 0; d < 32; d++) u[d] = __float_as_uint(o[d] * f);
+                            pr_st32(o_at + c, u);
+                        }
+                    }
+                }
+                const Pair fac = {factor, factor}, neg = {-m, -m};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int c = 0; c < 32; c++) {
+                        Pair y = fma2({x[2 * h + c / 16][2 * c % 32], x[2 * h + c / 16][2 * c % 32 + 1]}, fac, neg);
+                        y.x = pr_exp2(y.x); y.y = pr_exp2(y.y);
+                        l = add2(l, y);
+                        p[c] = pr_bf16x2(y.x, y.y);
+                    }
+                    pr_st32(s_at + 32 * h, p);
+                }
+                pr_st_wait();
+                pr_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(bars.p_full[i]));
+            }
+            // ---- the output
+            wait(bars.done, 0);
+            pr_fence_after();
+            const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : 1.f / sum;   // no position at all: zeros
+            int16_t* out = P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD;
+            const bool aligned = ((reinterpret_cast<uintptr_t>(P.a.out) & 15) | (P.a.out_stride & 7)) == 0;
+#pragma unroll 1
+            for (int c = 0; c < kHD; c += 32) {
+                float o[32];
+                pr_ld32(o_at + c, o);
+                pr_ld_wait();
+                if (r >= rows) continue;
+#pragma unroll
+                for (int d = 0; d < 32; d += 8) {
+                    const uint4 y = make_uint4(pr_bf16x2(o[d] * rd, o[d + 1] * rd), pr_bf16x2(o[d + 2] * rd, o[d + 3] * rd),
+                                               pr_bf16x2(o[d + 4] * rd, o[d + 5] * rd), pr_bf16x2(o[d + 6] * rd, o[d + 7] * rd));
+                    if (aligned) {
+                        *reinterpret_cast<uint4*>(out + c + d) = y;
+                    } else {
+                        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int e = 0; e < 8; e++) out[c + d + e] = (int16_t)(w[e >> 1] >> (16 * (e & 1)));
+                    }
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ------------------------------ codes to operands ---------------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        const int t = threadIdx.x - 256, cw = warp - 8;
+        // thread: piece (16 codes) of rows it * rows_at + row_of; a row's pieces side by side in a warp
+        constexpr int kLanes = kHD == 64 ? 4 : 8, kRowsAt = 128 / kLanes, kIts = kPrTile / kRowsAt;
+        const int piece = t % kLanes, row_of = t / kLanes;
+        const bool live = piece < kPieces;
+        const int* table = C.table + (size_t)seq * C.table_stride;
+        const int ps = 1 << C.page_shift;
+        bool missing = false;
+        // page of the 16 positions from j * 128 + 16 * (lane & 7) on
+        auto page_of = [&](int j) {
+            const int p = j * kPrTile + 16 * (lane & 7);
+            if (p >= seen) return -1;
+            const int page = table[p >> C.page_shift];
+            if ((unsigned)page < (unsigned)C.num_pages) return page;
+            missing = true;
+            return -1;
+        };
+        auto row_at = [&](int page, int p) { return (((uint32_t)page * C.n_head_kv + kvh) << C.page_shift) + (p & (ps - 1)); };
+        uint4 k[kIts], v[kIts];
+        float scale[kIts], sk = 0.f, sv = 0.f;                      // value scales of this thread's rows; both of position t
+        auto fetch = [&](uint4 (&to)[kIts], const int8_t* codes, int j, int pages) {
+#pragma unroll
+            for (int it = 0; it < kIts; it++) {
+                const int r = it * kRowsAt + row_of, page = __shfl_sync(0xFFFFFFFFu, pages, r >> 4);
+                to[it] = make_uint4(0, 0, 0, 0);
+                if (page >= 0 && live) to[it] = *reinterpret_cast<const uint4*>(codes + (size_t)row_at(page, j * kPrTile + r) * kHD + 16 * piece);
+            }
+        };
+        auto fetch_scales = [&](int j, int pages) {
+            const int page = __shfl_sync(0xFFFFFFFFu, pages, t >> 4);
+            const bool there = page >= 0 && j * kPrTile + t < seen;
+            const uint32_t at = there ? row_at(page, j * kPrTile + t) : 0;
+            sk = there ? C.sk[at] : 0.f;
+            sv = there ? C.sv[at] : 0.f;
+        };
+        auto fetch_rows = [&](int j, int pages) {
+#pragma unroll
+            for (int it = 0; it < kIts; it++) {
+                const int r = it * kRowsAt + row_of, page = __shfl_sync(0xFFFFFFFFu, pages, r >> 4);
+                scale[it] = page >= 0 && j * kPrTile + r < seen ? C.sv[row_at(page, j * kPrTile + r)] : 0.f;
+            }
+        };
+        int pages = page_of(0), next = n > 1 ? page_of(1) : -1;
+        fetch_scales(0, pages);
+        fetch(k, C.k, 0, pages);
+        fetch_rows(0, pages);
+        fetch(v, C.v, 0, pages);
+        for (int j = 0; j < n; j++) {
+            const int st = j & 1;
+            const uint32_t absent = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
+            const float key_scale = fabsf(sv) <= kPrMostScale ? sk : __uint_as_float(0x7FC00000u);
+            // ---- K
+            if (j >= 2) wait(bars.k_empty[st], (j >> 1) - 1);
+            sk_s[j % kPrScaleStages][t] = key_scale;
+            if (t == 0) absent_s[j % kPrScaleStages] = absent;
+#pragma unroll
+            for (int it = 0; it < kIts; it++) {
+                if (!live) break;
+                const int r = it * kRowsAt + row_of;
+                const uint32_t w[4] = {k[it].x, k[it].y, k[it].z, k[it].w};
+                uint32_t y[8];
+#pragma unroll
+                for (int d = 0; d < 4; d++) {
+                    // a code + 128 in the low bits of 1024 as f16, minus 1152
+                    const uint32_t u = w[d] ^ 0x80808080u, a = prmt(u, 0x64646464u, 0x4140u), b = prmt(u, 0x64646464u, 0x4342u);
+                    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y[2 * d]) : "r"(a), "r"(0x64806480u));
+                    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y[2 * d + 1]) : "r"(b), "r"(0x64806480u));
+                }
+                uint8_t* to = k_s + st * kTileBytes;
+                const int odd = piece >> 2;                         // the blocks' halves in turn: other banks
+                *reinterpret_cast<uint4*>(to + pr_chunk(r, 2 * piece + odd)) = odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(to + pr_chunk(r, 2 * piece + 1 - odd)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(bars.k_full[st]));
+            const int next2 = j + 2 < n ? page_of(j + 2) : -1;
+            if (j + 1 < n) { fetch_scales(j + 1, next); fetch(k, C.k, j + 1, next); }
+            // ---- V
+            if (j >= 2) wait(bars.v_empty[st], (j >> 1) - 1);
+#pragma unroll
+            for (int it = 0; it < kIts; it++) {
+                if (!live) break;
+                const int r = it * kRowsAt + row_of;
+                const uint32_t w[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
+                const float f = fabsf(scale[it]) <= kPrMostScale ? scale[it] : 0.f;
+                uint32_t y[8];
+#pragma unroll
+                for (int d = 0; d < 4; d++) {
+                    const Pair a = mul2({(float)(int8_t)w[d], (float)(int8_t)(w[d] >> 8)}, {f, f});
+                    const Pair b = mul2({(float)(int8_t)(w[d] >> 16), (float)((int)w[d] >> 24)}, {f, f});
+                    y[2 * d] = pr_bf16x2(a.x, a.y); y[2 * d + 1] = pr_bf16x2(b.x, b.y);
+                }
+                uint8_t* to = v_s + st * kTileBytes;
+                const int odd = piece >> 2;
+                *reinterpret_cast<uint4*>(to + pr_chunk(r, 2 * piece + odd)) = odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(to + pr_chunk(r, 2 * piece + 1 - odd)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(bars.v_full[st]));
+            if (j + 1 < n) { fetch_rows(j + 1, next); fetch(v, C.v, j + 1, next); }
+            pages = next; next = next2;
+        }
+        if (missing) atomicOr(C.status, kStatusPage);
+    } else {
+        // ------------------------------ MMAs ----------------------------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 12) {
+            const uint32_t idesc_s = 1u << 4 | (uint32_t)(kPrTile >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;                        // f16 x f16
+            const uint32_t idesc_o = 1u << 4 | 1u << 7 | 1u << 10 | 1u << 16 | (uint32_t)(kHD >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;   // bf16 x bf16, B with N contiguous
+            const uint64_t qd = pr_desc(smem_addr(q_s), 16), kd = pr_desc(smem_addr(k_s), 16), vd = pr_desc(smem_addr(v_s), kPrRows * 128);
+            auto scores = [&](int i, int st) {
+#pragma unroll
+                for (int s = 0; s < kHD / 16; s++) {
+                    const uint32_t off = (uint32_t)((s >> 2) * (kPrRows * 128) + (s & 3) * 32) >> 4;
+                    pr_mma_ss(tmem + i * kPrTile, qd + (i * kTileBytes >> 4) + off, kd + (st * kTileBytes >> 4) + off, idesc_s, s > 0);
+                }
+            };
+            wait(bars.k_full[0], 0);
+            pr_fence_after();
+            __syncwarp();
+            if (pr_elect()) {
+                for (int i = 0; i < n_q; i++) { scores(i, 0); pr_commit(bar(bars.s_full[i])); }
+                pr_commit(bar(bars.k_empty[0]));
+            }
+            __syncwarp();
+            for (int j = 0; j < n; j++) {
+                const int st = j & 1, st_next = (j + 1) & 1;
+                const bool more = j + 1 < n;
+                wait(bars.v_full[st], j >> 1);
+                if (more) wait(bars.k_full[st_next], (j + 1) >> 1);
+                for (int i = 0; i < n_q; i++) {
+                    wait(bars.p_full[i], j);
+                    pr_fence_after();
+                    __syncwarp();
+                    if (pr_elect()) {
+#pragma unroll
+                        for (int s = 0; s < kPrTile / 16; s++)      // 16 positions: 8 columns of weights, 16 rows of values
+                            pr_mma_ts(tmem + 2 * kPrTile + i * 128, tmem + i * kPrTile + 8 * s, vd + (st * kTileBytes >> 4) + (uint32_t)(s * 16 * 128 >> 4), idesc_o,
+                                      j > 0 || s > 0);
+                        if (i == n_q - 1) pr_commit(bar(bars.v_empty[st]));
+                        // the next scores take the weights' place: MMAs of one thread are executed in order
+                        if (more) {
+                            scores(i, st_next);
+                            pr_commit(bar(bars.s_full[i]));
+                            if (i == n_q - 1) pr_commit(bar(bars.k_empty[st_next]));
+                        } else if (i == n_q - 1) {
+                            pr_commit(bar(bars.done));
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+    if (*(volatile int*)&s_abort)                                  // a wait gave up: MMAs in flight finish before tensor memory goes
+        for (int i = 0; i < 256; i++) __nanosleep(1000);
+    pr_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        pr_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+template <int kHD>
+static int prompt_launch(const PromptParams& P, long long grid, void* stream, const char* who)
+{
+    static std::atomic<bool> attr_set[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_relaxed)) {
+        const int rc = check_cuda(cudaFuncSetAttribute(paged_prompt_kernel<kHD>, cudaFuncAttributeMaxDynamicSharedMemorySize, pr_smem_bytes(kHD)), who);
+        if (rc) return rc;
+        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_relaxed);
+    }
+    return launch(paged_prompt_kernel<kHD>, dim3((unsigned)grid), dim3(kPrThreads), pr_smem_bytes(kHD), stream, who, P);
+}
+
+// 1: not a shape of this kernel
+int paged_prompt_launch(const PagedAttn& A, void* stream, const char* who)
+{
+    const int hd = A.c.head_dim, gqa = A.n_head / A.c.n_head_kv;
+    if (hd != 64 && hd != 96 && hd != 128) return 1;
+    PromptParams P = {A, 2 * kPrRows};
+    // every sequence's last tile may be a part of one
+    const long long tiles = (long long)A.c.num_tokens * gqa / P.tile_rows + std::min(A.c.num_seqs, A.c.num_tokens), grid = tiles * A.c.n_head_kv;
+    if (grid > 0x7FFFFFFF) return fail(S12_ERR_TOO_LARGE, "%s: %d tokens", who, A.c.num_tokens);
+    return hd == 64 ? prompt_launch<64>(P, grid, stream, who) : hd == 96 ? prompt_launch<96>(P, grid, stream, who) : prompt_launch<128>(P, grid, stream, who);
+}
+
+}  // namespace s12
