@@ -52,8 +52,9 @@ def attention(c, scale, absent=()):
       the output to bf16: 2^-8 of the value;
       q to 11 significant bits of its row's power of two, or 15 bits of its largest: a score is off by at most
         d = scale * (2^-11 sum |q||k| + 2^-15 max|q| sum |k|), a weight by (e^(2d) - 1) of itself, numerator and sum alike;
-      a weight and a value to bf16: 2^-8 + 2^-8 of |p v|; or a weight times its value's scale to 15 bits of the largest of
-        32 neighbours: 2^-15 * 127 of that largest, for each of the 32;
+      a weight, a value's scale and their product to f16: 3 * 2^-11 of |p v|, and below f16's normal numbers 2^-25 of the
+        largest scale for each |code| and 2^-32 of the largest weight; or a weight times its value's scale to 15 bits of the
+        largest of 32 neighbours: 2^-15 * 127 of that largest, for each of the 32;
       sums in 32 bits: 2^-20 of the sum of magnitudes, up to 16 additions deep after the matrix products."""
     hd, gqa = c.hd, c.n_head // c.n_kv
     out = torch.zeros(c.tokens, c.n_head * hd, dtype=torch.float64, device=c.q.device)
@@ -85,7 +86,8 @@ def attention(c, scale, absent=()):
             d = torch.where(seen, d, 0).amax(1, keepdim=True)
             size = p @ v.abs() / den
             top = torch.nn.functional.pad(p * sv, (0, -n % 32)).view(new, -(-n // 32), 32).amax(2).sum(1, keepdim=True) / den
-            err = size * (torch.expm1(2 * d) + 2 * 2.0 ** -8 + 2.0 ** -20) + 32 * 2.0 ** -15 * 127 * top
+            floor = 2.0 ** -25 * 127 * sv.abs().amax() + 2.0 ** -32 * v.abs().sum(0)[None] / den
+            err = size * (torch.expm1(2 * d) + 3 * 2.0 ** -11 + 2.0 ** -20) + 32 * 2.0 ** -15 * 127 * top + floor
             out[row:row + new, h * hd:(h + 1) * hd] = o
             bound[row:row + new, h * hd:(h + 1) * hd] = 2.0 ** -8 * (o.abs() + err) + err
         row += new

@@ -7,20 +7,23 @@
 // A CTA has 256 rows of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
 // products and softmax take turns.  It walks the positions in tiles of 128.
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row: scores from tensor memory, running maximum and sum,
-//                    weights back to tensor memory as bf16 in the place of the scores; the output at the end
-//   warps 8-11       int8 codes from global memory to swizzled shared memory: K to f16, which holds a code exactly, V times
-//                    its scale to bf16; the next tile's loads are in flight meanwhile
+//                    weights back to tensor memory as f16 in the place of the scores; the output at the end
+//   warps 8-11       int8 codes from global memory to f16 in swizzled shared memory; the next tile's loads are in flight
+//                    meanwhile
 //   warp 12          issues the MMAs from one thread: S = Q K^T (both from shared memory), O += P V (P from tensor memory,
 //                    V with the dims contiguous)
-// Numbers: q is f16 after a power of two of its row takes its largest element to 2^14..2^15 (11 significant bits; a row of
-// bf16 would lose three more); K's scales multiply the scores in 32 bits.  Weights and values are bf16, whose range no
-// scale leaves; sums are 32-bit.  The maximum follows a row's scores only when they exceed it by 2^8, since the sums have
-// to be multiplied then.
+// Numbers: all operands are f16 (11 significant bits; bf16 would round a weight and a value to 8).  q is multiplied by a
+// power of two that takes its row's largest element to 2^14..2^15.  A K operand is the code, exactly; K's scales multiply
+// the scores in 32 bits.  A weight is at most 2^15: 2^7 times its distance from the row's maximum, which follows the scores
+// only when they exceed it by 2^8, since the sums have to be multiplied then.  A V operand is code * scale / 2^E with one E
+// for all: what the largest scale so far asks for, and six binary orders of room; when that is not enough the sums are
+// multiplied, too.  Sums are 32-bit.
 // A position that a row may not see gets weight 0, and its value must be finite for that: values behind the sequence's end
 // are zeros, and one whose scale is not finite is zero with its K scale made NaN, which marks the rows that see it.
 #include "paged.cuh"
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace s12 {
 
@@ -29,7 +32,7 @@ constexpr int kPrTile = 128;                        // positions of a step
 constexpr int kPrThreads = 512;
 constexpr int kPrScaleStages = 4;
 constexpr unsigned int kPrSite = 0x200000u;         // a wait of this kernel gave up
-constexpr float kPrMostScale = 2e36f;               // times 127 a finite bf16
+constexpr float kPrLift = 7.f;                       // weights are multiplied by 2^7: 2^15 at most
 constexpr float kPrSlack = 8.f;                     // a maximum may be exceeded by 2^8 before the sums are scaled
 
 __host__ __device__ constexpr int pr_tile_bytes(int hd) { return (hd + 63) / 64 * kPrRows * 128; }   // blocks of 64 dims: [128 rows][128 bytes]
@@ -89,6 +92,12 @@ __device__ __forceinline__ float pr_exp2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float pr_max3(float a, float b, float c)
+{
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
 __device__ __forceinline__ uint32_t pr_bf16x2(float lo, float hi)
 {
     uint32_t r;
@@ -101,29 +110,18 @@ __device__ __forceinline__ uint32_t pr_f16x2(float lo, float hi)
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// four codes as f16, exactly: code + 128 in the low bits of 1024, minus 1152
+__device__ __forceinline__ void pr_codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi)
+{
+    const uint32_t u = w ^ 0x80808080u, a = prmt(u, 0x64646464u, 0x4140u), b = prmt(u, 0x64646464u, 0x4342u);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+}
 // two at a time
-struct Pair { float x, y; };
-__device__ __forceinline__ Pair mul2(Pair a, Pair b)
-{
-    Pair r;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b)
-{
-    Pair r;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
-{
-    Pair r;
-    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
+typedef float2 Pair;
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { return __ffma2_rn(a, b, c); }
 
 // Operand tiles: blocks of 64 dims, each [128 rows][128 bytes] with the 128-byte swizzle (16-byte chunk c of row r sits at
 // c ^ (r & 7)).  For Q and K the rows are the MMA's M and N and the dims its K (K-major); for V the rows are its K and the
@@ -144,7 +142,10 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     extern __shared__ __align__(16) uint8_t pr_smem[];
     __shared__ PrBars bars;
     __shared__ __align__(16) float sk_s[kPrScaleStages][kPrTile];
-    __shared__ uint32_t absent_s[kPrScaleStages];                  // bit i: positions 16 i .. 16 i + 15 of the tile have no page
+    __shared__ float shift_s[kPrScaleStages];                      // 2^(E before - E) of the tile
+    __shared__ uint32_t top_s[2][4];                               // the converters' largest scale of a tile
+    __shared__ float unit_s;                                       // 2^E at the end
+    __shared__ __align__(4) uint8_t absent_s[kPrScaleStages][4];   // byte i, bit h: the 16 positions from 32 i + 16 h on have no page
     __shared__ float factor_s[2 * kPrRows];
     __shared__ uint32_t tmem_s;
     __shared__ int s_abort;
@@ -270,22 +271,22 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                     y[e] = a.x; y[e + 1] = a.y; y[e + 2] = b.x; y[e + 3] = b.y;
                 }
                 const int left = limit - j * kPrTile;               // positions of the tile that the row sees
-                const uint32_t absent = absent_s[j % kPrScaleStages];
+                const uint32_t absent = *reinterpret_cast<const uint32_t*>(absent_s[j % kPrScaleStages]);
                 if (least - j * kPrTile < kPrTile || absent) {
 #pragma unroll
-                    for (int c = 0; c < kPrTile; c++) if (c >= left || (absent >> (c / 16) & 1)) x[c / 32][c % 32] = -INFINITY;
+                    for (int c = 0; c < kPrTile; c++) if (c >= left || (absent >> (c / 32 * 8 + c / 16 % 2) & 1)) x[c / 32][c % 32] = -INFINITY;
                 }
-                float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+                float t0 = x[0][0], t1 = x[0][1], t2 = x[0][2], t3 = x[0][3];
 #pragma unroll
-                for (int c = 0; c < kPrTile; c += 8) {
-                    const float* y = x[c / 32];
-                    const int e = c % 32;
-                    t0 = fmaxf(t0, fmaxf(y[e], y[e + 1])); t1 = fmaxf(t1, fmaxf(y[e + 2], y[e + 3]));
-                    t2 = fmaxf(t2, fmaxf(y[e + 4], y[e + 5])); t3 = fmaxf(t3, fmaxf(y[e + 6], y[e + 7]));
+                for (int c = 4; c + 8 <= kPrTile; c += 8) {
+                    auto at = [&](int e) { return x[e / 32][e % 32]; };
+                    t0 = pr_max3(t0, at(c), at(c + 1)); t1 = pr_max3(t1, at(c + 2), at(c + 3));
+                    t2 = pr_max3(t2, at(c + 4), at(c + 5)); t3 = pr_max3(t3, at(c + 6), at(c + 7));
                 }
-                const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * factor;
+                const float top = pr_max3(fmaxf(t0, t1), pr_max3(t2, x[3][28], x[3][29]), pr_max3(t3, x[3][30], x[3][31])) * factor;
                 const bool rise = top > m + kPrSlack;
-                if (__any_sync(0xFFFFFFFFu, rise)) {
+                const float shift = shift_s[j % kPrScaleStages];
+                if (__any_sync(0xFFFFFFFFu, rise) || shift != 1.f) {
                     const float mn = rise ? top : m, f = pr_exp2(m - mn);
                     m = mn;
                     l = mul2(l, {f, f});
@@ -297,12 +298,12 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                             pr_ld_wait();
                             uint32_t u[32];
 #pragma unroll
-                            for (int d = 0; d < 32; d++) u[d] = __float_as_uint(o[d] * f);
+                            for (int d = 0; d < 32; d++) u[d] = __float_as_uint(o[d] * (f * shift));
                             pr_st32(o_at + c, u);
                         }
                     }
                 }
-                const Pair fac = {factor, factor}, neg = {-m, -m};
+                const Pair fac = {factor, factor}, neg = {kPrLift - m, kPrLift - m};
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     uint32_t p[32];
@@ -311,7 +312,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                         Pair y = fma2({x[2 * h + c / 16][2 * c % 32], x[2 * h + c / 16][2 * c % 32 + 1]}, fac, neg);
                         y.x = pr_exp2(y.x); y.y = pr_exp2(y.y);
                         l = add2(l, y);
-                        p[c] = pr_bf16x2(y.x, y.y);
+                        p[c] = pr_f16x2(y.x, y.y);
                     }
                     pr_st32(s_at + 32 * h, p);
                 }
@@ -323,7 +324,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             // ---- the output
             wait(bars.done, 0);
             pr_fence_after();
-            const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : 1.f / sum;   // no position at all: zeros
+            const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : unit_s / sum;   // no position at all: zeros
             int16_t* out = P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD;
             const bool aligned = ((reinterpret_cast<uintptr_t>(P.a.out) & 15) | (P.a.out_stride & 7)) == 0;
 #pragma unroll 1
@@ -348,160 +349,189 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
         }
     } else if (warp < 12) {
         // ------------------------------ codes to operands ---------------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-        const int t = threadIdx.x - 256, cw = warp - 8;
-        // thread: piece (16 codes) of rows it * rows_at + row_of; a row's pieces side by side in a warp
-        constexpr int kLanes = kHD == 64 ? 4 : 8, kRowsAt = 128 / kLanes, kIts = kPrTile / kRowsAt;
-        const int piece = t % kLanes, row_of = t / kLanes;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        // A warp has 32 rows of the tile, four (eight at head_dim 64) at a time: a lane 16 codes of one of them.  Lanes 0-7 of
+        // a store have two neighbouring rows, whose chunks the swizzle puts on different banks.  Lane l has the scales of row l.
+        const int cw = warp - 8;
+        constexpr int kRowsAt = kHD == 64 ? 8 : 4, kIts = 32 / kRowsAt;
+        const int row_of = kHD == 64 ? lane >> 2 : (lane >> 4) << 1 | (lane >> 2 & 1), piece = kHD == 64 ? lane & 3 : (lane >> 3 & 1) * 4 + (lane & 3);
         const bool live = piece < kPieces;
         const int* table = C.table + (size_t)seq * C.table_stride;
-        const int ps = 1 << C.page_shift;
+        const int ps = 1 << C.page_shift, mine = cw * 32 + lane;
         bool missing = false;
-        // page of the 16 positions from j * 128 + 16 * (lane & 7) on
-        auto page_of = [&](int j) {
-            const int p = j * kPrTile + 16 * (lane & 7);
-            if (p >= seen) return -1;
+        // the pools' row of position p, and whether there is one; -1 where the table has no page or no row sees p
+        auto row_at = [&](int p) {
+            if (p >= seen) return -1ll;
             const int page = table[p >> C.page_shift];
-            if ((unsigned)page < (unsigned)C.num_pages) return page;
-            missing = true;
-            return -1;
+            if ((unsigned)page >= (unsigned)C.num_pages) { missing = true; return -1ll; }
+            return (long long)((((uint32_t)page * C.n_head_kv + kvh) << C.page_shift) + (p & (ps - 1)));
         };
-        auto row_at = [&](int page, int p) { return (((uint32_t)page * C.n_head_kv + kvh) << C.page_shift) + (p & (ps - 1)); };
+        const int8_t* k_at = C.k + row_of * kHD + 16 * piece, *v_at = C.v + row_of * kHD + 16 * piece;
         uint4 k[kIts], v[kIts];
-        float scale[kIts], sk = 0.f, sv = 0.f;                      // value scales of this thread's rows; both of position t
-        auto fetch = [&](uint4 (&to)[kIts], const int8_t* codes, int j, int pages) {
+        float sk = 0.f, sv = 0.f;
+        // 16 rows lie together; absent ones read row 0 and are masked later
+        auto fetch = [&](uint4 (&to)[kIts], const int8_t* at, long long row) {
+            const uint32_t r = (uint32_t)max(row, 0ll);
+            const int8_t* half[2] = {at + (size_t)__shfl_sync(0xFFFFFFFFu, r, 0) * kHD, at + (size_t)__shfl_sync(0xFFFFFFFFu, r, 16) * kHD};
 #pragma unroll
-            for (int it = 0; it < kIts; it++) {
-                const int r = it * kRowsAt + row_of, page = __shfl_sync(0xFFFFFFFFu, pages, r >> 4);
-                to[it] = make_uint4(0, 0, 0, 0);
-                if (page >= 0 && live) to[it] = *reinterpret_cast<const uint4*>(codes + (size_t)row_at(page, j * kPrTile + r) * kHD + 16 * piece);
-            }
+            for (int it = 0; it < kIts; it++)
+                if (live) to[it] = *reinterpret_cast<const uint4*>(half[it / (kIts / 2)] + it % (kIts / 2) * kRowsAt * kHD);
         };
-        auto fetch_scales = [&](int j, int pages) {
-            const int page = __shfl_sync(0xFFFFFFFFu, pages, t >> 4);
-            const bool there = page >= 0 && j * kPrTile + t < seen;
-            const uint32_t at = there ? row_at(page, j * kPrTile + t) : 0;
-            sk = there ? C.sk[at] : 0.f;
-            sv = there ? C.sv[at] : 0.f;
+        auto fetch_scales = [&](long long row) { sk = row >= 0 ? C.sk[row] : 0.f; sv = row >= 0 ? C.sv[row] : 0.f; };
+        // Where a lane's chunks go: row + 4 changes bit 2 of the chunk
+        const uint32_t to0 = pr_chunk(cw * 32 + row_of, 2 * piece);
+        auto store = [&](uint8_t* tile, int it, const uint32_t (&y)[8]) {
+            const uint32_t to = (kRowsAt == 4 && (it & 1) ? to0 ^ 64u : to0) + it * kRowsAt * 128;
+            *reinterpret_cast<uint4*>(tile + to) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(tile + (to ^ 16u)) = make_uint4(y[4], y[5], y[6], y[7]);
         };
-        auto fetch_rows = [&](int j, int pages) {
-#pragma unroll
-            for (int it = 0; it < kIts; it++) {
-                const int r = it * kRowsAt + row_of, page = __shfl_sync(0xFFFFFFFFu, pages, r >> 4);
-                scale[it] = page >= 0 && j * kPrTile + r < seen ? C.sv[row_at(page, j * kPrTile + r)] : 0.f;
-            }
-        };
-        int pages = page_of(0), next = n > 1 ? page_of(1) : -1;
-        fetch_scales(0, pages);
-        fetch(k, C.k, 0, pages);
-        fetch_rows(0, pages);
-        fetch(v, C.v, 0, pages);
+        long long row = row_at(mine), row_next = n > 1 ? row_at(kPrTile + mine) : -1;
+        fetch_scales(row);
+        fetch(k, k_at, row);
+        fetch(v, v_at, row);
+        int E = 0;
         for (int j = 0; j < n; j++) {
             const int st = j & 1;
-            const uint32_t absent = __ballot_sync(0xFFFFFFFFu, pages < 0) & 0xFFu;
-            const float key_scale = fabsf(sv) <= kPrMostScale ? sk : __uint_as_float(0x7FC00000u);
+            const bool absent = row < 0;
+            // the values' unit 2^E
+            const uint32_t bits = __float_as_uint(sv) & 0x7FFFFFFFu;
+            const bool fine = bits < 0x7F800000u;
+            const uint32_t top_w = __reduce_max_sync(0xFFFFFFFFu, fine ? bits : 0u);
+            if (lane == 0) top_s[st][cw] = top_w;
+            named_bar_sync(1, 128);
+            const uint32_t top = max(max(top_s[st][0], top_s[st][1]), max(top_s[st][2], top_s[st][3]));
+            const int e_top = (int)(top >> 23) - 126;               // scales are below 2^e_top
+            float shift = 1.f;
+            if (j == 0 || e_top > E + 8) {
+                const int old = E;
+                E = max(e_top - 2, -120);
+                if (j > 0) shift = old - E < -126 ? 0.f : __uint_as_float((uint32_t)(127 + old - E) << 23);
+            }
+            const float unit = __uint_as_float((uint32_t)(127 - E) << 23);   // 2^-E
+            const float key_scale = fine ? sk : __uint_as_float(0x7FC00000u);
             // ---- K
             if (j >= 2) wait(bars.k_empty[st], (j >> 1) - 1);
-            sk_s[j % kPrScaleStages][t] = key_scale;
-            if (t == 0) absent_s[j % kPrScaleStages] = absent;
+            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, absent);   // a whole half, or rows that nobody sees
+            sk_s[j % kPrScaleStages][mine] = key_scale;
+            if (lane == 0) absent_s[j % kPrScaleStages][cw] = (uint8_t)((gone & 1u) | (gone >> 16 & 1u) << 1);
+            if (mine == 0) {
+                shift_s[j % kPrScaleStages] = shift;
+                if (j == n - 1) unit_s = __uint_as_float((uint32_t)(127 + E) << 23);
+            }
 #pragma unroll
             for (int it = 0; it < kIts; it++) {
                 if (!live) break;
-                const int r = it * kRowsAt + row_of;
                 const uint32_t w[4] = {k[it].x, k[it].y, k[it].z, k[it].w};
                 uint32_t y[8];
 #pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    // a code + 128 in the low bits of 1024 as f16, minus 1152
-                    const uint32_t u = w[d] ^ 0x80808080u, a = prmt(u, 0x64646464u, 0x4140u), b = prmt(u, 0x64646464u, 0x4342u);
-                    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y[2 * d]) : "r"(a), "r"(0x64806480u));
-                    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y[2 * d + 1]) : "r"(b), "r"(0x64806480u));
-                }
-                uint8_t* to = k_s + st * kTileBytes;
-                const int odd = piece >> 2;                         // the blocks' halves in turn: other banks
-                *reinterpret_cast<uint4*>(to + pr_chunk(r, 2 * piece + odd)) = odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<uint4*>(to + pr_chunk(r, 2 * piece + 1 - odd)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+                for (int d = 0; d < 4; d++) pr_codes_f16(w[d], y[2 * d], y[2 * d + 1]);
+                store(k_s + st * kTileBytes, it, y);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(bars.k_full[st]));
-            const int next2 = j + 2 < n ? page_of(j + 2) : -1;
-            if (j + 1 < n) { fetch_scales(j + 1, next); fetch(k, C.k, j + 1, next); }
+            const float scale = fine ? sv * unit : 0.f;
+            const uint32_t scale2 = pr_f16x2(scale, scale);
+            const long long row_next2 = j + 2 < n ? row_at((j + 2) * kPrTile + mine) : -1;
+            if (j + 1 < n) { fetch_scales(row_next); fetch(k, k_at, row_next); }
             // ---- V
             if (j >= 2) wait(bars.v_empty[st], (j >> 1) - 1);
 #pragma unroll
             for (int it = 0; it < kIts; it++) {
-                if (!live) break;
-                const int r = it * kRowsAt + row_of;
+                const uint32_t f2 = __shfl_sync(0xFFFFFFFFu, scale2, it * kRowsAt + row_of);
+                if (!live) continue;
                 const uint32_t w[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
-                const float f = fabsf(scale[it]) <= kPrMostScale ? scale[it] : 0.f;
                 uint32_t y[8];
 #pragma unroll
                 for (int d = 0; d < 4; d++) {
-                    const Pair a = mul2({(float)(int8_t)w[d], (float)(int8_t)(w[d] >> 8)}, {f, f});
-                    const Pair b = mul2({(float)(int8_t)(w[d] >> 16), (float)((int)w[d] >> 24)}, {f, f});
-                    y[2 * d] = pr_bf16x2(a.x, a.y); y[2 * d + 1] = pr_bf16x2(b.x, b.y);
+                    pr_codes_f16(w[d], y[2 * d], y[2 * d + 1]);
+                    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(y[2 * d]) : "r"(f2));
+                    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(y[2 * d + 1]) : "r"(f2));
                 }
-                uint8_t* to = v_s + st * kTileBytes;
-                const int odd = piece >> 2;
-                *reinterpret_cast<uint4*>(to + pr_chunk(r, 2 * piece + odd)) = odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<uint4*>(to + pr_chunk(r, 2 * piece + 1 - odd)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+                store(v_s + st * kTileBytes, it, y);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(bars.v_full[st]));
-            if (j + 1 < n) { fetch_rows(j + 1, next); fetch(v, C.v, j + 1, next); }
-            pages = next; next = next2;
+            if (j + 1 < n) fetch(v, v_at, row_next);
+            row = row_next; row_next = row_next2;
         }
         if (missing) atomicOr(C.status, kStatusPage);
     } else {
         // ------------------------------ MMAs ----------------------------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 12) {
             const uint32_t idesc_s = 1u << 4 | (uint32_t)(kPrTile >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;                        // f16 x f16
-            const uint32_t idesc_o = 1u << 4 | 1u << 7 | 1u << 10 | 1u << 16 | (uint32_t)(kHD >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;   // bf16 x bf16, B with N contiguous
-            const uint64_t qd = pr_desc(smem_addr(q_s), 16), kd = pr_desc(smem_addr(k_s), 16), vd = pr_desc(smem_addr(v_s), kPrRows * 128);
-            auto scores = [&](int i, int st) {
+            const uint32_t idesc_o = 1u << 4 | 1u << 16 | (uint32_t)(kHD >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;   // the same, B with N contiguous
+            // Everything that an MMA needs is a constant away from one value: with the row tile or the stage as variables the
+            // descriptors are put together anew for each, which takes longer than the MMA.
+            uint64_t qd = pr_desc(smem_addr(q_s), 16), kd = pr_desc(smem_addr(k_s), 16), vd = pr_desc(smem_addr(v_s), kPrRows * 128);
+            auto scores = [&](auto row_tile, auto stage) {
+                constexpr int i = row_tile.value, st = stage.value;
 #pragma unroll
                 for (int s = 0; s < kHD / 16; s++) {
                     const uint32_t off = (uint32_t)((s >> 2) * (kPrRows * 128) + (s & 3) * 32) >> 4;
-                    pr_mma_ss(tmem + i * kPrTile, qd + (i * kTileBytes >> 4) + off, kd + (st * kTileBytes >> 4) + off, idesc_s, s > 0);
+                    pr_mma_ss(tmem + i * kPrTile, qd + (uint32_t)(i * kTileBytes >> 4) + off, kd + (uint32_t)(st * kTileBytes >> 4) + off, idesc_s, s > 0);
                 }
+                pr_commit(bar(bars.s_full[i]));
+            };
+            auto sums = [&](auto row_tile, auto stage, uint32_t accumulate) {
+                constexpr int i = row_tile.value, st = stage.value;
+#pragma unroll
+                for (int s = 0; s < kPrTile / 16; s++)              // 16 positions: 8 columns of weights, 16 rows of values
+                    pr_mma_ts(tmem + 2 * kPrTile + i * 128, tmem + i * kPrTile + 8 * s, vd + (uint32_t)((st * kTileBytes + s * 16 * 128) >> 4), idesc_o, s > 0 ? 1u : accumulate);
+            };
+            std::integral_constant<int, 0> zero;
+            std::integral_constant<int, 1> one;
+            auto step = [&](int j, auto stage, auto stage_next) {   // tile j's sums and tile j + 1's scores
+                constexpr int st = stage.value, st_next = stage_next.value;
+                const bool more = j + 1 < n;
+                asm volatile("" : "+l"(qd), "+l"(kd), "+l"(vd));     // or the compiler keeps all the descriptors, in local memory
+                wait(bars.v_full[st], j >> 1);
+                wait(bars.p_full[0], j);
+                pr_fence_after();
+                __syncwarp();
+                if (pr_elect()) {
+                    sums(zero, stage, j > 0);
+                    if (n_q == 1) pr_commit(bar(bars.v_empty[st]));
+                }
+                if (more) { wait(bars.k_full[st_next], (j + 1) >> 1); pr_fence_after(); }
+                __syncwarp();
+                // the next scores take the weights' place: MMAs of one thread are executed in order
+                if (more && pr_elect()) {
+                    scores(zero, stage_next);
+                    if (n_q == 1) pr_commit(bar(bars.k_empty[st_next]));
+                }
+                __syncwarp();
+                if (n_q > 1) {
+                    wait(bars.p_full[1], j);
+                    pr_fence_after();
+                    __syncwarp();
+                    if (pr_elect()) {
+                        sums(one, stage, j > 0);
+                        pr_commit(bar(bars.v_empty[st]));
+                        if (more) {
+                            scores(one, stage_next);
+                            pr_commit(bar(bars.k_empty[st_next]));
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (!more && pr_elect()) pr_commit(bar(bars.done));
+                __syncwarp();
             };
             wait(bars.k_full[0], 0);
             pr_fence_after();
             __syncwarp();
             if (pr_elect()) {
-                for (int i = 0; i < n_q; i++) { scores(i, 0); pr_commit(bar(bars.s_full[i])); }
+                scores(zero, zero);
+                if (n_q > 1) scores(one, zero);
                 pr_commit(bar(bars.k_empty[0]));
             }
             __syncwarp();
-            for (int j = 0; j < n; j++) {
-                const int st = j & 1, st_next = (j + 1) & 1;
-                const bool more = j + 1 < n;
-                wait(bars.v_full[st], j >> 1);
-                if (more) wait(bars.k_full[st_next], (j + 1) >> 1);
-                for (int i = 0; i < n_q; i++) {
-                    wait(bars.p_full[i], j);
-                    pr_fence_after();
-                    __syncwarp();
-                    if (pr_elect()) {
-#pragma unroll
-                        for (int s = 0; s < kPrTile / 16; s++)      // 16 positions: 8 columns of weights, 16 rows of values
-                            pr_mma_ts(tmem + 2 * kPrTile + i * 128, tmem + i * kPrTile + 8 * s, vd + (st * kTileBytes >> 4) + (uint32_t)(s * 16 * 128 >> 4), idesc_o,
-                                      j > 0 || s > 0);
-                        if (i == n_q - 1) pr_commit(bar(bars.v_empty[st]));
-                        // the next scores take the weights' place: MMAs of one thread are executed in order
-                        if (more) {
-                            scores(i, st_next);
-                            pr_commit(bar(bars.s_full[i]));
-                            if (i == n_q - 1) pr_commit(bar(bars.k_empty[st_next]));
-                        } else if (i == n_q - 1) {
-                            pr_commit(bar(bars.done));
-                        }
-                    }
-                    __syncwarp();
-                }
+            for (int j = 0; j < n; j += 2) {
+                step(j, zero, one);
+                if (j + 1 < n) step(j + 1, one, zero);
             }
         }
     }
