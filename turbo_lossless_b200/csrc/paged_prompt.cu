@@ -10,8 +10,9 @@
 //                    weights back to tensor memory as f16 in the place of the scores; the output at the end
 //   warps 8-11       int8 codes from global memory to f16 in swizzled shared memory; the next tile's loads are in flight
 //                    meanwhile
-//   warp 12          issues the MMAs from one thread: S = Q K^T (both from shared memory), O += P V (P from tensor memory,
-//                    V with the dims contiguous)
+//   warps 12, 13     issue the MMAs of row tile 0 / 1, one thread each: S = Q K^T (both from shared memory), O += P V (P from
+//                    tensor memory, V with the dims contiguous), 64 positions at a time: the next 64 scores are there
+//                    when the softmax has done with these
 // Numbers: all operands are f16 (11 significant bits; bf16 would round a weight and a value to 8).  q is multiplied by a
 // power of two that takes its row's largest element to 2^14..2^15.  A K operand is the code, exactly; K's scales multiply
 // the scores in 32 bits.  A weight is at most 2^15: 2^7 times its distance from the row's maximum, which follows the scores
@@ -28,7 +29,8 @@
 namespace s12 {
 
 constexpr int kPrRows = 128;                        // rows of an MMA
-constexpr int kPrTile = 128;                        // positions of a step
+constexpr int kPrTile = 128;                        // positions of a conversion step
+constexpr int kPrHalf = 64;                         // positions of an MMA and softmax step
 constexpr int kPrThreads = 512;
 constexpr int kPrScaleStages = 4;
 constexpr unsigned int kPrSite = 0x200000u;         // a wait of this kernel gave up
@@ -38,7 +40,7 @@ constexpr float kPrSlack = 8.f;                     // a maximum may be exceeded
 __host__ __device__ constexpr int pr_tile_bytes(int hd) { return (hd + 63) / 64 * kPrRows * 128; }   // blocks of 64 dims: [128 rows][128 bytes]
 __host__ __device__ constexpr int pr_smem_bytes(int hd) { return 6 * pr_tile_bytes(hd) + 1024; }
 
-struct PrBars { uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done; };
+struct PrBars { uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], sums_done[2]; };
 
 __device__ __forceinline__ uint32_t pr_elect()
 {
@@ -74,6 +76,15 @@ __device__ __forceinline__ void pr_ld32(uint32_t at, float (&r)[32])
                  : "r"(at) : "memory");
 }
 __device__ __forceinline__ void pr_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// After a wait: r is what the loads brought.  Between a load and this no branch may define r: the compiler takes the load's
+// registers for ready and might copy them.
+__device__ __forceinline__ void pr_ready(float (&r)[32])
+{
+    asm volatile("" : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                 "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+                 "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]));
+}
 __device__ __forceinline__ void pr_st32(uint32_t at, const uint32_t (&u)[32])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -180,16 +191,16 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     const int row0 = tile * P.tile_rows, rows = min(P.tile_rows, (hi - lo) * gqa - row0);
     const int n_q = rows > kPrRows ? 2 : 1;                        // row tiles
     const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // token t sees min(before + t, room) positions
-    const int seen = max(0, min(before + (row0 + rows - 1) / gqa, room)), n = max(1, (seen + kPrTile - 1) / kPrTile);
+    const int seen = max(0, min(before + (row0 + rows - 1) / gqa, room)), halves = max(1, (seen + kPrHalf - 1) / kPrHalf), n = (halves + 1) / 2;
 
     if (threadIdx.x == 0) {
         s_abort = 0;
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_addr(&bars.k_full[i]), 4); mbar_init(smem_addr(&bars.v_full[i]), 4);
-            mbar_init(smem_addr(&bars.k_empty[i]), 1); mbar_init(smem_addr(&bars.v_empty[i]), 1);
-            mbar_init(smem_addr(&bars.s_full[i]), 1); mbar_init(smem_addr(&bars.p_full[i]), 4);
+            mbar_init(smem_addr(&bars.k_empty[i]), n_q); mbar_init(smem_addr(&bars.v_empty[i]), n_q);
+            for (int b = 0; b < 2; b++) { mbar_init(smem_addr(&bars.s_full[i][b]), 1); mbar_init(smem_addr(&bars.p_full[i][b]), 4); }
+            mbar_init(smem_addr(&bars.sums_done[i]), 1);
         }
-        mbar_init(smem_addr(&bars.done), 1);
         mbar_fence_init();
     }
     if (warp == 12) {
@@ -247,50 +258,56 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
         const int i = warp >> 2, r = i * kPrRows + (warp & 3) * 32 + lane;   // row tile, row of the CTA
         if (i < n_q) {
             const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            const uint32_t s_at = mine + i * kPrTile, o_at = mine + 2 * kPrTile + i * 128;
+            const uint32_t s_at = mine + i * 2 * kPrHalf, o_at = mine + 4 * kPrHalf + i * 128;
             const int tok = (row0 + r) / gqa, head = row0 + r - tok * gqa;
             const int limit = r < rows ? min(before + tok, room) : 0;       // positions that this row sees
             const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
             const float factor = factor_s[r];
             float m = -1e30f;
             Pair l = {0.f, 0.f};
-            for (int j = 0; j < n; j++) {
-                wait(bars.s_full[i], j);                            // and the tile before it is in the sums
+#pragma unroll 1
+            for (int h = 0; h < halves; h++) {
+                const int j = (h >> 1) % kPrScaleStages, b = h & 1;
+                float x[2][32];
+                wait(bars.s_full[i][b], h >> 1);                    // then half h - 2 is in the sums
                 pr_fence_after();
-                float x[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; c++) pr_ld32(s_at + 32 * c, x[c]);
+                pr_ld32(s_at + b * kPrHalf, x[0]);
+                pr_ld32(s_at + b * kPrHalf + 32, x[1]);
                 pr_ld_wait();
-                const float4* sk = reinterpret_cast<const float4*>(sk_s[j % kPrScaleStages]);
+                pr_ready(x[0]);
+                pr_ready(x[1]);
+                const float4* sk = reinterpret_cast<const float4*>(sk_s[j] + b * kPrHalf);
 #pragma unroll
-                for (int c = 0; c < kPrTile / 4; c++) {
+                for (int c = 0; c < kPrHalf / 4; c++) {
                     const float4 k = sk[c];
                     float (&y)[32] = x[c / 8];
                     const int e = c % 8 * 4;
-                    const Pair a = mul2({y[e], y[e + 1]}, {k.x, k.y}), b = mul2({y[e + 2], y[e + 3]}, {k.z, k.w});
-                    y[e] = a.x; y[e + 1] = a.y; y[e + 2] = b.x; y[e + 3] = b.y;
+                    const Pair u = mul2({y[e], y[e + 1]}, {k.x, k.y}), v = mul2({y[e + 2], y[e + 3]}, {k.z, k.w});
+                    y[e] = u.x; y[e + 1] = u.y; y[e + 2] = v.x; y[e + 3] = v.y;
                 }
-                const int left = limit - j * kPrTile;               // positions of the tile that the row sees
-                const uint32_t absent = *reinterpret_cast<const uint32_t*>(absent_s[j % kPrScaleStages]);
-                if (least - j * kPrTile < kPrTile || absent) {
+                const int left = limit - h * kPrHalf;               // positions of the half that the row sees
+                const uint32_t absent = *reinterpret_cast<const uint16_t*>(&absent_s[j][2 * b]);
+                if (least - h * kPrHalf < kPrHalf || absent) {
 #pragma unroll
-                    for (int c = 0; c < kPrTile; c++) if (c >= left || (absent >> (c / 32 * 8 + c / 16 % 2) & 1)) x[c / 32][c % 32] = -INFINITY;
+                    for (int c = 0; c < kPrHalf; c++) if (c >= left || (absent >> (c / 32 * 8 + c / 16 % 2) & 1)) x[c / 32][c % 32] = -INFINITY;
                 }
                 float t0 = x[0][0], t1 = x[0][1], t2 = x[0][2], t3 = x[0][3];
+                auto at = [&](int e) { return x[e / 32][e % 32]; };
 #pragma unroll
-                for (int c = 4; c + 8 <= kPrTile; c += 8) {
-                    auto at = [&](int e) { return x[e / 32][e % 32]; };
+                for (int c = 4; c + 8 <= kPrHalf; c += 8) {
                     t0 = pr_max3(t0, at(c), at(c + 1)); t1 = pr_max3(t1, at(c + 2), at(c + 3));
                     t2 = pr_max3(t2, at(c + 4), at(c + 5)); t3 = pr_max3(t3, at(c + 6), at(c + 7));
                 }
-                const float top = pr_max3(fmaxf(t0, t1), pr_max3(t2, x[3][28], x[3][29]), pr_max3(t3, x[3][30], x[3][31])) * factor;
+                const float top = pr_max3(fmaxf(t0, t1), pr_max3(t2, at(kPrHalf - 4), at(kPrHalf - 3)), pr_max3(t3, at(kPrHalf - 2), at(kPrHalf - 1))) * factor;
                 const bool rise = top > m + kPrSlack;
-                const float shift = shift_s[j % kPrScaleStages];
+                const float shift = b == 0 ? shift_s[j] : 1.f;
                 if (__any_sync(0xFFFFFFFFu, rise) || shift != 1.f) {
                     const float mn = rise ? top : m, f = pr_exp2(m - mn);
                     m = mn;
                     l = mul2(l, {f, f});
-                    if (j > 0) {
+                    if (h > 0) {
+                        wait(bars.sums_done[i], h - 1);                 // the half before it, too
+                        pr_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < kHD; c += 32) {
                             float o[32];
@@ -304,25 +321,23 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                     }
                 }
                 const Pair fac = {factor, factor}, neg = {kPrLift - m, kPrLift - m};
+                uint32_t p[32];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int c = 0; c < 32; c++) {
-                        Pair y = fma2({x[2 * h + c / 16][2 * c % 32], x[2 * h + c / 16][2 * c % 32 + 1]}, fac, neg);
-                        y.x = pr_exp2(y.x); y.y = pr_exp2(y.y);
-                        l = add2(l, y);
-                        p[c] = pr_f16x2(y.x, y.y);
-                    }
-                    pr_st32(s_at + 32 * h, p);
+                for (int c = 0; c < 32; c++) {
+                    Pair y = fma2({x[c / 16][2 * c % 32], x[c / 16][2 * c % 32 + 1]}, fac, neg);
+                    y.x = pr_exp2(y.x); y.y = pr_exp2(y.y);
+                    l = add2(l, y);
+                    p[c] = pr_f16x2(y.x, y.y);
                 }
+                pr_st32(s_at + b * kPrHalf, p);
                 pr_st_wait();
                 pr_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(bars.p_full[i]));
+                if (lane == 0) mbar_arrive(bar(bars.p_full[i][b]));
             }
             // ---- the output
-            wait(bars.done, 0);
+            if (halves > 1) wait(bars.sums_done[i], halves - 2);    // one after the other: a wait tells odd from even only
+            wait(bars.sums_done[i], halves - 1);
             pr_fence_after();
             const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : unit_s / sum;   // no position at all: zeros
             int16_t* out = P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD;
@@ -460,78 +475,58 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     } else {
         // ------------------------------ MMAs ----------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12) {
-            const uint32_t idesc_s = 1u << 4 | (uint32_t)(kPrTile >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;                        // f16 x f16
+        if (warp - 12 < n_q) {                                     // a warp per row tile
+            const int i = warp - 12;
+            const uint32_t idesc_s = 1u << 4 | (uint32_t)(kPrHalf >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;                        // f16 x f16
             const uint32_t idesc_o = 1u << 4 | 1u << 16 | (uint32_t)(kHD >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;   // the same, B with N contiguous
-            // Everything that an MMA needs is a constant away from one value: with the row tile or the stage as variables the
-            // descriptors are put together anew for each, which takes longer than the MMA.
-            uint64_t qd = pr_desc(smem_addr(q_s), 16), kd = pr_desc(smem_addr(k_s), 16), vd = pr_desc(smem_addr(v_s), kPrRows * 128);
-            auto scores = [&](auto row_tile, auto stage) {
-                constexpr int i = row_tile.value, st = stage.value;
+            const uint64_t qd = pr_desc(smem_addr(q_s) + i * kTileBytes, 16), kd = pr_desc(smem_addr(k_s), 16), vd = pr_desc(smem_addr(v_s), kPrRows * 128);
+            const uint32_t s_at = tmem + i * 2 * kPrHalf, o_at = tmem + 4 * kPrHalf + i * 128;
+            // scores of half h; the tile's keys have been used with its last half
+            auto scores = [&](int h) {
+                const uint64_t k = kd + (uint32_t)((h >> 1 & 1) * (kTileBytes >> 4) + (h & 1) * (kPrHalf * 128 >> 4));
+                const uint32_t d = s_at + (h & 1) * kPrHalf;
 #pragma unroll
                 for (int s = 0; s < kHD / 16; s++) {
                     const uint32_t off = (uint32_t)((s >> 2) * (kPrRows * 128) + (s & 3) * 32) >> 4;
-                    pr_mma_ss(tmem + i * kPrTile, qd + (uint32_t)(i * kTileBytes >> 4) + off, kd + (uint32_t)(st * kTileBytes >> 4) + off, idesc_s, s > 0);
+                    pr_mma_ss(d, qd + off, k + off, idesc_s, s > 0);
                 }
-                pr_commit(bar(bars.s_full[i]));
-            };
-            auto sums = [&](auto row_tile, auto stage, uint32_t accumulate) {
-                constexpr int i = row_tile.value, st = stage.value;
-#pragma unroll
-                for (int s = 0; s < kPrTile / 16; s++)              // 16 positions: 8 columns of weights, 16 rows of values
-                    pr_mma_ts(tmem + 2 * kPrTile + i * 128, tmem + i * kPrTile + 8 * s, vd + (uint32_t)((st * kTileBytes + s * 16 * 128) >> 4), idesc_o, s > 0 ? 1u : accumulate);
-            };
-            std::integral_constant<int, 0> zero;
-            std::integral_constant<int, 1> one;
-            auto step = [&](int j, auto stage, auto stage_next) {   // tile j's sums and tile j + 1's scores
-                constexpr int st = stage.value, st_next = stage_next.value;
-                const bool more = j + 1 < n;
-                asm volatile("" : "+l"(qd), "+l"(kd), "+l"(vd));     // or the compiler keeps all the descriptors, in local memory
-                wait(bars.v_full[st], j >> 1);
-                wait(bars.p_full[0], j);
-                pr_fence_after();
-                __syncwarp();
-                if (pr_elect()) {
-                    sums(zero, stage, j > 0);
-                    if (n_q == 1) pr_commit(bar(bars.v_empty[st]));
-                }
-                if (more) { wait(bars.k_full[st_next], (j + 1) >> 1); pr_fence_after(); }
-                __syncwarp();
-                // the next scores take the weights' place: MMAs of one thread are executed in order
-                if (more && pr_elect()) {
-                    scores(zero, stage_next);
-                    if (n_q == 1) pr_commit(bar(bars.k_empty[st_next]));
-                }
-                __syncwarp();
-                if (n_q > 1) {
-                    wait(bars.p_full[1], j);
-                    pr_fence_after();
-                    __syncwarp();
-                    if (pr_elect()) {
-                        sums(one, stage, j > 0);
-                        pr_commit(bar(bars.v_empty[st]));
-                        if (more) {
-                            scores(one, stage_next);
-                            pr_commit(bar(bars.k_empty[st_next]));
-                        }
-                    }
-                    __syncwarp();
-                }
-                if (!more && pr_elect()) pr_commit(bar(bars.done));
-                __syncwarp();
+                pr_commit(bar(bars.s_full[i][h & 1]));
+                if ((h & 1) || h + 1 == halves) pr_commit(bar(bars.k_empty[h >> 1 & 1]));
             };
             wait(bars.k_full[0], 0);
             pr_fence_after();
             __syncwarp();
             if (pr_elect()) {
-                scores(zero, zero);
-                if (n_q > 1) scores(one, zero);
-                pr_commit(bar(bars.k_empty[0]));
+                scores(0);
+                if (halves > 1) scores(1);
             }
             __syncwarp();
-            for (int j = 0; j < n; j += 2) {
-                step(j, zero, one);
-                if (j + 1 < n) step(j + 1, one, zero);
+#pragma unroll 1
+            for (int h = 0; h < halves; h++) {
+                const int b = h & 1, st = h >> 1 & 1;
+                if (b == 0) wait(bars.v_full[st], h >> 2);
+                wait(bars.p_full[i][b], h >> 1);
+                const bool more = h + 2 < halves;
+                if (more && b == 0) wait(bars.k_full[st ^ 1], (h + 2) >> 2);
+                pr_fence_after();
+                __syncwarp();
+                if (pr_elect()) {
+                    const uint64_t v = vd + (uint32_t)((st * kTileBytes + b * kPrHalf * 128) >> 4);
+                    const uint32_t p = s_at + b * kPrHalf;
+#pragma unroll
+                    for (int s = 0; s < kPrHalf / 16; s++)          // 16 positions: 8 columns of weights, 16 rows of values
+                        pr_mma_ts(o_at, p + 8 * s, v + (uint32_t)(s * 16 * 128 >> 4), idesc_o, h > 0 || s > 0);
+                    if (b == 1 || h + 1 == halves) pr_commit(bar(bars.v_empty[st]));
+                    pr_commit(bar(bars.sums_done[i]));
+                }
+                __syncwarp();
+                if (more) {                                         // in the weights' place, when they have been read
+                    wait(bars.sums_done[i], h);
+                    pr_fence_after();
+                    __syncwarp();
+                    if (pr_elect()) scores(h + 2);
+                    __syncwarp();
+                }
             }
         }
     }
