@@ -40,7 +40,7 @@ constexpr float kPrSlack = 8.f;                     // a maximum may be exceeded
 __host__ __device__ constexpr int pr_tile_bytes(int hd) { return (hd + 63) / 64 * kPrRows * 128; }   // blocks of 64 dims: [128 rows][128 bytes]
 __host__ __device__ constexpr int pr_smem_bytes(int hd) { return 6 * pr_tile_bytes(hd) + 1024; }
 
-struct PrBars { uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], sums_done[2]; };
+struct PrBars { uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], sums_done[2]; };
 
 __device__ __forceinline__ uint32_t pr_elect()
 {
@@ -143,7 +143,11 @@ __device__ __forceinline__ uint64_t pr_desc(uint32_t at, uint32_t lead)
     return (uint64_t)((at >> 4) & 0x3FFF) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-struct PromptParams { PagedAttn a; int tile_rows; };               // rows of a CTA: 128 or 256
+struct PromptParams {
+    PagedAttn a;
+    int tile_rows;              // rows of a CTA: 128 or 256
+    uint32_t gqa_mul;           // ceil(2^32 / query heads of a kv head), 0 for one: divides what is below 2^32 / that number
+};
 
 template <int kHD>
 __global__ void __launch_bounds__(kPrThreads, 1)
@@ -165,6 +169,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     const PagedArgs& C = P.a.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int gqa = P.a.n_head / C.n_head_kv;
+    auto token_of = [&](int row) { return P.gqa_mul ? (int)__umulhi((uint32_t)row, P.gqa_mul) : row; };
     grid_launch_dependents();
     grid_dependency_wait();
 
@@ -191,10 +196,11 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     const int row0 = tile * P.tile_rows, rows = min(P.tile_rows, (hi - lo) * gqa - row0);
     const int n_q = rows > kPrRows ? 2 : 1;                        // row tiles
     const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // token t sees min(before + t, room) positions
-    const int seen = max(0, min(before + (row0 + rows - 1) / gqa, room)), halves = max(1, (seen + kPrHalf - 1) / kPrHalf), n = (halves + 1) / 2;
+    const int seen = max(0, min(before + token_of(row0 + rows - 1), room)), halves = max(1, (seen + kPrHalf - 1) / kPrHalf), n = (halves + 1) / 2;
 
     if (threadIdx.x == 0) {
         s_abort = 0;
+        mbar_init(smem_addr(&bars.q_full), 12);
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_addr(&bars.k_full[i]), 4); mbar_init(smem_addr(&bars.v_full[i]), 4);
             mbar_init(smem_addr(&bars.k_empty[i]), n_q); mbar_init(smem_addr(&bars.v_empty[i]), n_q);
@@ -207,44 +213,6 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // ---- q as f16: a warp per row, four dims a lane
-    {
-        const bool q_aligned = ((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0;
-        const float to_log2 = fabsf(P.a.scale) * 1.4426950408889634f, sign = P.a.scale < 0.f ? -1.f : 1.f;
-        constexpr int kFlight = 8;
-        for (int r0 = warp; r0 < n_q * kPrRows; r0 += 16 * kFlight) {
-            float4 v[kFlight];
-#pragma unroll
-            for (int i = 0; i < kFlight; i++) {
-                const int r = r0 + 16 * i, t = (row0 + r) / gqa, head = row0 + r - t * gqa;
-                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < rows && 4 * lane < kHD) {
-                    const float* q = P.a.q + (size_t)(lo + t) * P.a.q_stride + (size_t)(kvh * gqa + head) * kHD + 4 * lane;
-                    if (q_aligned) v[i] = *reinterpret_cast<const float4*>(q);
-                    else v[i] = make_float4(q[0], q[1], q[2], q[3]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kFlight; i++) {
-                const int r = r0 + 16 * i;
-                if (r >= n_q * kPrRows) break;
-                const uint32_t a = __float_as_uint(v[i].x) & 0x7FFFFFFFu, b = __float_as_uint(v[i].y) & 0x7FFFFFFFu;
-                const uint32_t c = __float_as_uint(v[i].z) & 0x7FFFFFFFu, d = __float_as_uint(v[i].w) & 0x7FFFFFFFu;
-                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d)));   // a NaN is the largest
-                const int e = (int)(top >> 23) - 127;              // the largest is 2^e and more
-                const bool fine = e >= -100 && e < 128;            // rows of smaller ones count as zero
-                // 2^(14 - e) in two factors, each a normal number
-                const float up = fine ? sign * __uint_as_float((uint32_t)(127 + (14 - e) / 2) << 23) : 0.f;
-                const float up2 = __uint_as_float((uint32_t)(127 + (14 - e) - (14 - e) / 2) << 23);
-                if (!fine) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (4 * lane < kHD)
-                    *reinterpret_cast<uint2*>(q_s + (r / kPrRows) * kTileBytes + pr_chunk(r % kPrRows, lane >> 1) + (lane & 1) * 8) =
-                        make_uint2(pr_f16x2(v[i].x * up * up2, v[i].y * up * up2), pr_f16x2(v[i].z * up * up2, v[i].w * up * up2));
-                if (lane == 0) factor_s[r] = e == 128 ? __uint_as_float(0x7FC00000u) : fine ? fmaxf(ldexpf(to_log2, e - 14), 1e-37f) : 1e-37f;   // above 0: a masked score stays -infinity
-            }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what ordinary stores wrote
-    }
     pr_fence_before();
     __syncthreads();
     pr_fence_after();
@@ -252,14 +220,60 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     auto bar = [](const uint64_t& b) { return smem_addr(&b); };
     auto wait = [&](const uint64_t& b, int phase) { mbar_wait(smem_addr(&b), (uint32_t)phase & 1, C.status, kPrSite, &s_abort); };
 
+    // q as f16: a warp per row, four dims a lane, by all warps but the converters, which have begun meanwhile
+    auto q_rows = [&](auto in_flight) {
+        constexpr int kFlight = in_flight.value, kWarps = 12;
+        const bool q_aligned = ((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0;
+        const float to_log2 = fabsf(P.a.scale) * 1.4426950408889634f, sign = P.a.scale < 0.f ? -1.f : 1.f;
+        const float* q0 = P.a.q + (size_t)lo * P.a.q_stride + (size_t)kvh * gqa * kHD + 4 * lane;
+#pragma unroll 1
+        for (int r0 = warp < 8 ? warp : warp - 4; r0 < n_q * kPrRows; r0 += kWarps * kFlight) {
+            float4 v[kFlight];
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) {
+                const int r = r0 + kWarps * i, t = token_of(row0 + r), head = row0 + r - t * gqa;
+                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < rows && 4 * lane < kHD) {
+                    const float* q = q0 + (size_t)t * P.a.q_stride + head * kHD;
+                    if (q_aligned) v[i] = *reinterpret_cast<const float4*>(q);
+                    else v[i] = make_float4(q[0], q[1], q[2], q[3]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) {
+                const int r = r0 + kWarps * i;
+                if (r >= n_q * kPrRows) break;
+                const uint32_t a = __float_as_uint(v[i].x) & 0x7FFFFFFFu, b = __float_as_uint(v[i].y) & 0x7FFFFFFFu;
+                const uint32_t c = __float_as_uint(v[i].z) & 0x7FFFFFFFu, d = __float_as_uint(v[i].w) & 0x7FFFFFFFu;
+                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d)));   // a NaN is the largest
+                const int e = (int)(top >> 23) - 127;              // the largest is 2^e and more
+                const bool fine = e >= -100 && e < 128;            // rows of smaller ones count as zero
+                // 2^(14 - e) in two factors, each a normal number
+                const int up = (14 - e) / 2, up2 = 14 - e - up;
+                const float f = fine ? sign * __uint_as_float((uint32_t)(127 + up) << 23) : 0.f, f2 = __uint_as_float((uint32_t)(127 + up2) << 23);
+                if (!fine) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (4 * lane < kHD)
+                    *reinterpret_cast<uint2*>(q_s + r / kPrRows * kTileBytes + pr_chunk(r % kPrRows, lane >> 1) + (lane & 1) * 8) =
+                        make_uint2(pr_f16x2(v[i].x * f * f2, v[i].y * f * f2), pr_f16x2(v[i].z * f * f2, v[i].w * f * f2));
+                // above 0: a masked score stays -infinity
+                const float factor = to_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * __uint_as_float((uint32_t)(127 - up2) << 23);
+                if (lane == 0) factor_s[r] = e == 128 ? __uint_as_float(0x7FC00000u) : fine ? fmaxf(factor, 1e-37f) : 1e-37f;
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what ordinary stores wrote
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(bars.q_full));
+    };
     if (warp < 8) {
         // ------------------------------ softmax -------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        q_rows(std::integral_constant<int, 11>());
+        wait(bars.q_full, 0);                                       // the rows' factors come from all warps
         const int i = warp >> 2, r = i * kPrRows + (warp & 3) * 32 + lane;   // row tile, row of the CTA
         if (i < n_q) {
             const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
             const uint32_t s_at = mine + i * 2 * kPrHalf, o_at = mine + 4 * kPrHalf + i * 128;
-            const int tok = (row0 + r) / gqa, head = row0 + r - tok * gqa;
+            const int tok = token_of(row0 + r), head = row0 + r - tok * gqa;
             const int limit = r < rows ? min(before + tok, room) : 0;       // positions that this row sees
             const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
             const float factor = factor_s[r];
@@ -475,6 +489,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     } else {
         // ------------------------------ MMAs ----------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        q_rows(std::integral_constant<int, 4>());
         if (warp - 12 < n_q) {                                     // a warp per row tile
             const int i = warp - 12;
             const uint32_t idesc_s = 1u << 4 | (uint32_t)(kPrHalf >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;                        // f16 x f16
@@ -493,6 +508,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 pr_commit(bar(bars.s_full[i][h & 1]));
                 if ((h & 1) || h + 1 == halves) pr_commit(bar(bars.k_empty[h >> 1 & 1]));
             };
+            wait(bars.q_full, 0);
             wait(bars.k_full[0], 0);
             pr_fence_after();
             __syncwarp();
@@ -559,7 +575,9 @@ int paged_prompt_launch(const PagedAttn& A, void* stream, const char* who)
 {
     const int hd = A.c.head_dim, gqa = A.n_head / A.c.n_head_kv;
     if (hd != 64 && hd != 96 && hd != 128) return 1;
-    PromptParams P = {A, 2 * kPrRows};
+    // rows as far as the division by multiplication holds
+    if ((long long)A.c.num_tokens * gqa + 2 * kPrRows >= (1ll << 32) / gqa) return 1;
+    PromptParams P = {A, 2 * kPrRows, gqa == 1 ? 0u : (uint32_t)(((1ull << 32) + gqa - 1) / gqa)};
     // every sequence's last tile may be a part of one
     const long long tiles = (long long)A.c.num_tokens * gqa / P.tile_rows + std::min(A.c.num_seqs, A.c.num_tokens), grid = tiles * A.c.n_head_kv;
     if (grid > 0x7FFFFFFF) return fail(S12_ERR_TOO_LARGE, "%s: %d tokens", who, A.c.num_tokens);
