@@ -229,35 +229,49 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
 #pragma unroll 1
         for (int r0 = warp < 8 ? warp : warp - 4; r0 < n_q * kPrRows; r0 += kWarps * kFlight) {
             float4 v[kFlight];
+            uint32_t top[kFlight];
+            auto row_of = [&](int i) {
+                const int r = r0 + kWarps * i, t = token_of(row0 + r), head = row0 + r - t * gqa;
+                return q0 + (size_t)t * P.a.q_stride + head * kHD;
+            };
+#pragma unroll
+            for (int i = 0; i < kFlight; i++) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (q_aligned) {
+#pragma unroll
+                for (int i = 0; i < kFlight; i++) if (r0 + kWarps * i < rows && 4 * lane < kHD) v[i] = *reinterpret_cast<const float4*>(row_of(i));
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < kFlight; i++) {
+                    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r0 + kWarps * i < rows && 4 * lane < kHD) { const float* q = row_of(i); u = make_float4(q[0], q[1], q[2], q[3]); }
+#pragma unroll
+                    for (int c = 0; c < kFlight; c++) if (c == i) v[c] = u;
+                }
+            }
+            // no branch from here on: the rows' chains of instructions run side by side
 #pragma unroll
             for (int i = 0; i < kFlight; i++) {
-                const int r = r0 + kWarps * i, t = token_of(row0 + r), head = row0 + r - t * gqa;
-                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < rows && 4 * lane < kHD) {
-                    const float* q = q0 + (size_t)t * P.a.q_stride + head * kHD;
-                    if (q_aligned) v[i] = *reinterpret_cast<const float4*>(q);
-                    else v[i] = make_float4(q[0], q[1], q[2], q[3]);
-                }
+                const uint32_t a = __float_as_uint(v[i].x) & 0x7FFFFFFFu, b = __float_as_uint(v[i].y) & 0x7FFFFFFFu;
+                const uint32_t c = __float_as_uint(v[i].z) & 0x7FFFFFFFu, d = __float_as_uint(v[i].w) & 0x7FFFFFFFu;
+                top[i] = __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d)));   // a NaN is the largest
             }
 #pragma unroll
             for (int i = 0; i < kFlight; i++) {
                 const int r = r0 + kWarps * i;
-                if (r >= n_q * kPrRows) break;
-                const uint32_t a = __float_as_uint(v[i].x) & 0x7FFFFFFFu, b = __float_as_uint(v[i].y) & 0x7FFFFFFFu;
-                const uint32_t c = __float_as_uint(v[i].z) & 0x7FFFFFFFu, d = __float_as_uint(v[i].w) & 0x7FFFFFFFu;
-                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d)));   // a NaN is the largest
-                const int e = (int)(top >> 23) - 127;              // the largest is 2^e and more
+                const int e = (int)(top[i] >> 23) - 127;           // the largest is 2^e and more
                 const bool fine = e >= -100 && e < 128;            // rows of smaller ones count as zero
                 // 2^(14 - e) in two factors, each a normal number
                 const int up = (14 - e) / 2, up2 = 14 - e - up;
                 const float f = fine ? sign * __uint_as_float((uint32_t)(127 + up) << 23) : 0.f, f2 = __uint_as_float((uint32_t)(127 + up2) << 23);
-                if (!fine) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (4 * lane < kHD)
-                    *reinterpret_cast<uint2*>(q_s + r / kPrRows * kTileBytes + pr_chunk(r % kPrRows, lane >> 1) + (lane & 1) * 8) =
-                        make_uint2(pr_f16x2(v[i].x * f * f2, v[i].y * f * f2), pr_f16x2(v[i].z * f * f2, v[i].w * f * f2));
+                const float4 u = fine ? v[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+                const uint2 y = make_uint2(pr_f16x2(u.x * f * f2, u.y * f * f2), pr_f16x2(u.z * f * f2, u.w * f * f2));
                 // above 0: a masked score stays -infinity
                 const float factor = to_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * __uint_as_float((uint32_t)(127 - up2) << 23);
-                if (lane == 0) factor_s[r] = e == 128 ? __uint_as_float(0x7FC00000u) : fine ? fmaxf(factor, 1e-37f) : 1e-37f;
+                const float kept = e == 128 ? __uint_as_float(0x7FC00000u) : fine ? fmaxf(factor, 1e-37f) : 1e-37f;
+                if (r < n_q * kPrRows && 4 * lane < kHD) {
+                    *reinterpret_cast<uint2*>(q_s + r / kPrRows * kTileBytes + pr_chunk(r % kPrRows, lane >> 1) + (lane & 1) * 8) = y;
+                    if (lane == 0) factor_s[r] = kept;
+                }
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what ordinary stores wrote
@@ -273,7 +287,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
         if (i < n_q) {
             const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
             const uint32_t s_at = mine + i * 2 * kPrHalf, o_at = mine + 4 * kPrHalf + i * 128;
-            const int tok = token_of(row0 + r), head = row0 + r - tok * gqa;
+            const int tok = token_of(row0 + r);
             const int limit = r < rows ? min(before + tok, room) : 0;       // positions that this row sees
             const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
             const float factor = factor_s[r];
@@ -354,25 +368,39 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             wait(bars.sums_done[i], halves - 1);
             pr_fence_after();
             const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : unit_s / sum;   // no position at all: zeros
-            int16_t* out = P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD;
-            const bool aligned = ((reinterpret_cast<uintptr_t>(P.a.out) & 15) | (P.a.out_stride & 7)) == 0;
+            // A row as one piece: by way of shared memory, where this row tile's q has been read.  Row of 256 bytes, its
+            // 16-byte chunks permuted so that the lanes of a store and of a load meet different banks.
+            uint8_t* stage = q_s + i * kTileBytes + (warp & 3) * (kTileBytes / 4);
+            constexpr int kRowBytes = kHD == 64 ? 128 : 256, kChunks = kHD / 8;
+            auto chunk_at = [&](int row, int c) { return stage + row * kRowBytes + ((c ^ (row & 7)) << 4); };
 #pragma unroll 1
             for (int c = 0; c < kHD; c += 32) {
                 float o[32];
                 pr_ld32(o_at + c, o);
                 pr_ld_wait();
-                if (r >= rows) continue;
+                pr_ready(o);
 #pragma unroll
-                for (int d = 0; d < 32; d += 8) {
-                    const uint4 y = make_uint4(pr_bf16x2(o[d] * rd, o[d + 1] * rd), pr_bf16x2(o[d + 2] * rd, o[d + 3] * rd),
-                                               pr_bf16x2(o[d + 4] * rd, o[d + 5] * rd), pr_bf16x2(o[d + 6] * rd, o[d + 7] * rd));
-                    if (aligned) {
-                        *reinterpret_cast<uint4*>(out + c + d) = y;
-                    } else {
-                        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+                for (int d = 0; d < 32; d += 8)
+                    *reinterpret_cast<uint4*>(chunk_at(lane, (c + d) / 8)) =
+                        make_uint4(pr_bf16x2(o[d] * rd, o[d + 1] * rd), pr_bf16x2(o[d + 2] * rd, o[d + 3] * rd),
+                                   pr_bf16x2(o[d + 4] * rd, o[d + 5] * rd), pr_bf16x2(o[d + 6] * rd, o[d + 7] * rd));
+            }
+            __syncwarp();
+            const bool aligned = ((reinterpret_cast<uintptr_t>(P.a.out) & 15) | (P.a.out_stride & 7)) == 0;
+            const int first = i * kPrRows + (warp & 3) * 32;       // this warp's rows
+            int16_t* out0 = P.a.out + (size_t)lo * P.a.out_stride + (size_t)kvh * gqa * kHD;
+#pragma unroll 4
+            for (int x = lane; x < 32 * kChunks; x += 32) {
+                const int row = x / kChunks, c = x - row * kChunks, t = token_of(row0 + first + row), hd = row0 + first + row - t * gqa;
+                if (first + row >= rows) break;
+                const uint4 y = *reinterpret_cast<const uint4*>(chunk_at(row, c));
+                int16_t* out = out0 + (size_t)t * P.a.out_stride + hd * kHD + c * 8;
+                if (aligned) {
+                    *reinterpret_cast<uint4*>(out) = y;
+                } else {
+                    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                        for (int e = 0; e < 8; e++) out[c + d + e] = (int16_t)(w[e >> 1] >> (16 * (e & 1)));
-                    }
+                    for (int e = 0; e < 8; e++) out[e] = (int16_t)(w[e >> 1] >> (16 * (e & 1)));
                 }
             }
         }
