@@ -24,7 +24,6 @@
 #include "paged.cuh"
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 namespace s12 {
 
@@ -200,7 +199,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
 
     if (threadIdx.x == 0) {
         s_abort = 0;
-        mbar_init(smem_addr(&bars.q_full), 12);
+        mbar_init(smem_addr(&bars.q_full), 8);
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_addr(&bars.k_full[i]), 4); mbar_init(smem_addr(&bars.v_full[i]), 4);
             mbar_init(smem_addr(&bars.k_empty[i]), n_q); mbar_init(smem_addr(&bars.v_empty[i]), n_q);
@@ -220,69 +219,57 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     auto bar = [](const uint64_t& b) { return smem_addr(&b); };
     auto wait = [&](const uint64_t& b, int phase) { mbar_wait(smem_addr(&b), (uint32_t)phase & 1, C.status, kPrSite, &s_abort); };
 
-    // q as f16: a warp per row, four dims a lane, by all warps but the converters, which have begun meanwhile
-    auto q_rows = [&](auto in_flight) {
-        constexpr int kFlight = in_flight.value, kWarps = 12;
-        const bool q_aligned = ((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0;
-        const float to_log2 = fabsf(P.a.scale) * 1.4426950408889634f, sign = P.a.scale < 0.f ? -1.f : 1.f;
-        const float* q0 = P.a.q + (size_t)lo * P.a.q_stride + (size_t)kvh * gqa * kHD + 4 * lane;
-#pragma unroll 1
-        for (int r0 = warp < 8 ? warp : warp - 4; r0 < n_q * kPrRows; r0 += kWarps * kFlight) {
-            float4 v[kFlight];
-            uint32_t top[kFlight];
-            auto row_of = [&](int i) {
-                const int r = r0 + kWarps * i, t = token_of(row0 + r), head = row0 + r - t * gqa;
-                return q0 + (size_t)t * P.a.q_stride + head * kHD;
-            };
-#pragma unroll
-            for (int i = 0; i < kFlight; i++) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (q_aligned) {
-#pragma unroll
-                for (int i = 0; i < kFlight; i++) if (r0 + kWarps * i < rows && 4 * lane < kHD) v[i] = *reinterpret_cast<const float4*>(row_of(i));
-            } else {
-#pragma unroll 1
-                for (int i = 0; i < kFlight; i++) {
-                    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r0 + kWarps * i < rows && 4 * lane < kHD) { const float* q = row_of(i); u = make_float4(q[0], q[1], q[2], q[3]); }
-#pragma unroll
-                    for (int c = 0; c < kFlight; c++) if (c == i) v[c] = u;
-                }
-            }
-            // no branch from here on: the rows' chains of instructions run side by side
-#pragma unroll
-            for (int i = 0; i < kFlight; i++) {
-                const uint32_t a = __float_as_uint(v[i].x) & 0x7FFFFFFFu, b = __float_as_uint(v[i].y) & 0x7FFFFFFFu;
-                const uint32_t c = __float_as_uint(v[i].z) & 0x7FFFFFFFu, d = __float_as_uint(v[i].w) & 0x7FFFFFFFu;
-                top[i] = __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d)));   // a NaN is the largest
-            }
-#pragma unroll
-            for (int i = 0; i < kFlight; i++) {
-                const int r = r0 + kWarps * i;
-                const int e = (int)(top[i] >> 23) - 127;           // the largest is 2^e and more
-                const bool fine = e >= -100 && e < 128;            // rows of smaller ones count as zero
-                // 2^(14 - e) in two factors, each a normal number
-                const int up = (14 - e) / 2, up2 = 14 - e - up;
-                const float f = fine ? sign * __uint_as_float((uint32_t)(127 + up) << 23) : 0.f, f2 = __uint_as_float((uint32_t)(127 + up2) << 23);
-                const float4 u = fine ? v[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-                const uint2 y = make_uint2(pr_f16x2(u.x * f * f2, u.y * f * f2), pr_f16x2(u.z * f * f2, u.w * f * f2));
-                // above 0: a masked score stays -infinity
-                const float factor = to_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * __uint_as_float((uint32_t)(127 - up2) << 23);
-                const float kept = e == 128 ? __uint_as_float(0x7FC00000u) : fine ? fmaxf(factor, 1e-37f) : 1e-37f;
-                if (r < n_q * kPrRows && 4 * lane < kHD) {
-                    *reinterpret_cast<uint2*>(q_s + r / kPrRows * kTileBytes + pr_chunk(r % kPrRows, lane >> 1) + (lane & 1) * 8) = y;
-                    if (lane == 0) factor_s[r] = kept;
-                }
-            }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what ordinary stores wrote
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(bars.q_full));
-    };
     if (warp < 8) {
         // ------------------------------ softmax -------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-        q_rows(std::integral_constant<int, 11>());
-        wait(bars.q_full, 0);                                       // the rows' factors come from all warps
+        // ---- q as f16: warp w takes rows w, w + 8, ..., all of them in flight together, a lane four dims of each; the
+        // converters have begun meanwhile
+        {
+            const float to_log2 = fabsf(P.a.scale) * 1.4426950408889634f;
+            const float* q0 = P.a.q + (size_t)lo * P.a.q_stride + (size_t)kvh * gqa * kHD + 4 * lane;
+            const bool in_row = 4 * lane < kHD;
+            uint8_t* to = q_s + pr_chunk(warp, lane >> 1) + (lane & 1) * 8;
+            auto row_of = [&](int r) {
+                const int t = token_of(row0 + r);
+                return q0 + (size_t)t * P.a.q_stride + (row0 + r - t * gqa) * kHD;
+            };
+            auto put = [&](int i, const float4& v) {                // row warp + 8 i
+                const uint32_t a = __float_as_uint(v.x) & 0x7FFFFFFFu, b = __float_as_uint(v.y) & 0x7FFFFFFFu;
+                const uint32_t c = __float_as_uint(v.z) & 0x7FFFFFFFu, d = __float_as_uint(v.w) & 0x7FFFFFFFu;
+                // 2^e of the largest, e >= -100, or nothing: rows of smaller ones count as zero, and a NaN or an infinity, the
+                // largest of all, becomes a NaN
+                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d))) & 0x7F800000u;
+                const bool fine = top - (27u << 23) < (228u << 23);
+                const float up = fine ? __uint_as_float((268u << 23) - top ^ (P.a.scale < 0.f ? 0x80000000u : 0u)) : 0.f;   // 2^(14 - e)
+                if (in_row) *reinterpret_cast<uint2*>(to + i / 16 * kTileBytes + i % 16 * 1024) = make_uint2(pr_f16x2(v.x * up, v.y * up), pr_f16x2(v.z * up, v.w * up));
+                // above 0: a masked score stays -infinity
+                if (lane == 0) factor_s[warp + 8 * i] = fine ? fmaxf(to_log2 * __uint_as_float(top - (14u << 23)), 1e-37f) : 1e-37f;
+            };
+            if (((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0) {
+                float4 v[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (warp + 8 * i < rows && in_row) v[i] = *reinterpret_cast<const float4*>(row_of(warp + 8 * i));
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) put(i, v[i]);
+                if (n_q > 1)
+#pragma unroll
+                    for (int i = 16; i < 32; i++) put(i, v[i]);
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 16 * n_q; i++) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (warp + 8 * i < rows && in_row) { const float* q = row_of(warp + 8 * i); v = make_float4(q[0], q[1], q[2], q[3]); }
+                    put(i, v);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what ordinary stores wrote
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(bars.q_full));
+            wait(bars.q_full, 0);                                   // the rows' factors come from all warps
+        }
         const int i = warp >> 2, r = i * kPrRows + (warp & 3) * 32 + lane;   // row tile, row of the CTA
         if (i < n_q) {
             const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -517,7 +504,6 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     } else {
         // ------------------------------ MMAs ----------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        q_rows(std::integral_constant<int, 4>());
         if (warp - 12 < n_q) {                                     // a warp per row tile
             const int i = warp - 12;
             const uint32_t idesc_s = 1u << 4 | (uint32_t)(kPrHalf >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;                        // f16 x f16
