@@ -23,12 +23,14 @@ struct StoreParams {
     PagedArgs c;
     const float* q; const float* k; const float* v; float* q_out;
     int q_stride, kv_stride, q_out_stride, n_head;
-    int heads_per_warp;
+    int heads_per_warp;         // paged_store_kernel
+    int group_shift;            // paged_store_rows_kernel: 2^this lanes have a head
 };
 struct HalfTurns { double f[128]; };                            // theta^(-2 d / head_dim) / pi
 
 constexpr int kStoreWarps = 8;
 constexpr int kStoreThreads = kStoreWarps * 32;
+constexpr int kStorePasses = 3;
 
 __device__ __forceinline__ unsigned long long abs_bits(double x) { return (unsigned long long)__double_as_longlong(x) & 0x7FFFFFFFFFFFFFFFull; }
 
@@ -91,6 +93,87 @@ paged_store_kernel(const __grid_constant__ StoreParams P, const __grid_constant_
             if (d < half) { dst[d] = code(lo[i]); dst[d + half] = code(hi[i]); }
         }
         if (lane == 0) (is_v ? P.c.sv : P.c.sk)[at] = (float)(amax / 127.0);
+    }
+}
+
+// The same for rows on 16-byte boundaries and head_dim a multiple of 8.  Bound: HBM, 4 bytes an element in, 4 or 1 out.
+// A group of lanes has a head, a lane four neighbouring elements of each half, so that a pair lies in one lane; a warp takes
+// kPasses times as many heads as it has groups, all of their loads in flight while the angles are computed, once a CTA.
+template <int kPasses>
+__global__ void __launch_bounds__(kStoreThreads)
+paged_store_rows_kernel(const __grid_constant__ StoreParams P, const __grid_constant__ HalfTurns F)
+{
+    __shared__ __align__(16) double cos_s[128], sin_s[128];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x;
+    const int hd = P.c.head_dim, half = hd >> 1, hkv = P.c.n_head_kv, heads = P.n_head + 2 * hkv;
+    const int group = lane >> P.group_shift, d = (lane & ((1 << P.group_shift) - 1)) * 4;   // the lane's head of a pass, its elements
+    const int per_pass = kStoreWarps * (32 >> P.group_shift);
+    const int h0 = blockIdx.y * kPasses * per_pass + warp * (32 >> P.group_shift) + group;
+    const int seq = paged_seq_of(P.c, row);
+    if (seq < 0) return;                                          // a row behind the last sequence
+    float4 lo[kPasses], hi[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; i++) {
+        const int h = h0 + i * per_pass;
+        if (h >= heads || d >= half) continue;
+        const float* x = h < P.n_head ? P.q + (size_t)row * P.q_stride + (size_t)h * hd
+                                      : (h < P.n_head + hkv ? P.k + (size_t)(h - P.n_head) * hd : P.v + (size_t)(h - P.n_head - hkv) * hd) + (size_t)row * P.kv_stride;
+        lo[i] = *reinterpret_cast<const float4*>(x + d); hi[i] = *reinterpret_cast<const float4*>(x + d + half);
+    }
+    const int after = P.c.q_start ? P.c.q_start[seq + 1] - row : 1;
+    const int pos = P.c.kv_len[seq] - after;
+    const bool inside = pos >= 0 && (pos >> P.c.page_shift) < P.c.table_pages;
+    const int page = inside ? paged_page(P.c, seq, pos) : -1;     // position below 0: a row of a sequence that is not there
+    if (page < 0 && pos >= 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(P.c.status, kStatusPage);
+    for (int i = threadIdx.x; i < half; i += kStoreThreads) sincospi((double)pos * F.f[i], &sin_s[i], &cos_s[i]);
+    __syncthreads();
+    double c[4], s[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) { c[e] = d < half ? cos_s[d + e] : 0.; s[e] = d < half ? sin_s[d + e] : 0.; }
+#pragma unroll
+    for (int i = 0; i < kPasses; i++) {
+        const int h = h0 + i * per_pass;
+        const bool live = h < heads && d < half;
+        const float a[4] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w}, b[4] = {hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+        if (live && h < P.n_head) {
+            float x[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float cf = (float)c[e], sf = (float)s[e];
+                x[e] = a[e] * cf - b[e] * sf; y[e] = a[e] * sf + b[e] * cf;
+            }
+            float* to = P.q_out + (size_t)row * P.q_out_stride + (size_t)h * hd + d;
+            *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(to + half) = make_float4(y[0], y[1], y[2], y[3]);
+        }
+        if (!__any_sync(0xFFFFFFFFu, live && h >= P.n_head) || page < 0) continue;
+        const bool is_v = h >= P.n_head + hkv, keep = live && h >= P.n_head;
+        double x[8];
+        unsigned long long top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double x0 = a[e], x1 = b[e];
+            x[e] = is_v ? x0 : x0 * c[e] - x1 * s[e]; x[4 + e] = is_v ? x1 : x0 * s[e] + x1 * c[e];
+            if (keep) top = max(top, max(abs_bits(x[e]), abs_bits(x[4 + e])));
+        }
+        for (int off = 1 << P.group_shift >> 1; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+        if (!keep) continue;
+        const double amax = __longlong_as_double((long long)top), inv = 127.0 / amax;   // a NaN counts as the largest
+        const bool fine = top < 0x7FF0000000000000ull && top > 0;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {                             // rounded to nearest by 1.5 * 2^52: the low word holds the code
+            const uint32_t r = fine ? (uint32_t)__double2loint(x[e] * inv + 6755399441055744.0) : 0u;
+            w[e >> 2] |= (r & 0xFFu) << (8 * (e & 3));
+        }
+        const int kvh = h - P.n_head - (is_v ? hkv : 0);
+        const size_t at = ((size_t)page * hkv + kvh) << P.c.page_shift | (size_t)(pos & ((1 << P.c.page_shift) - 1));
+        int8_t* dst = (is_v ? P.c.v : P.c.k) + at * hd + d;
+        *reinterpret_cast<uint32_t*>(dst) = w[0];
+        *reinterpret_cast<uint32_t*>(dst + half) = w[1];
+        if (d == 0) (is_v ? P.c.sv : P.c.sk)[at] = (float)(amax / 127.0);
     }
 }
 
@@ -284,6 +367,16 @@ int s12_rope_store_kv_paged_async(const float* q, int q_stride, const float* k, 
     for (int d = 0; d < hd / 2; d++) F.f[d] = std::pow((double)theta, -2.0 * d / hd) / 3.14159265358979323846;
     P.q = q; P.k = k; P.v = v; P.q_out = q_out;
     P.q_stride = q_stride; P.kv_stride = kv_stride; P.q_out_stride = q_out_stride; P.n_head = n_head;
+    const bool rows16 = hd % 8 == 0 && ((q_stride | kv_stride | q_out_stride) & 3) == 0 &&
+                        ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q_out)) & 15) == 0;
+    if (rows16) {
+        while ((1 << P.group_shift) < hd / 8) P.group_shift++;
+        const int all = n_head + 2 * kv->n_head_kv, per_pass = kStoreWarps * (32 >> P.group_shift);
+        const bool many = batch->num_tokens >= sm_count();
+        const int passes = many ? kStorePasses : 1;
+        return launch(many ? paged_store_rows_kernel<kStorePasses> : paged_store_rows_kernel<1>,
+                      dim3(batch->num_tokens, (all + passes * per_pass - 1) / (passes * per_pass)), dim3(kStoreThreads), 0, stream, who, P, F);
+    }
     P.heads_per_warp = 1;
     const int heads = n_head + 2 * kv->n_head_kv, per = kStoreWarps * P.heads_per_warp;
     return launch(paged_store_kernel, dim3(batch->num_tokens, (heads + per - 1) / per), dim3(kStoreThreads), 0, stream, who, P, F);
