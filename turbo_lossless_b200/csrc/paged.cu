@@ -8,8 +8,8 @@
 //
 // Pages are head-major, [page][kv head][position][head_dim]: what a CTA reads of a page is contiguous.
 #include "paged.cuh"
-#include <atomic>
 #include <cmath>
+#include <mutex>
 
 namespace s12 {
 
@@ -323,6 +323,20 @@ static int paged_cache_args(PagedArgs& C, const S12PagedKv* kv, const char* who)
     while ((1 << C.page_shift) < ps) C.page_shift++;
     return S12_OK;
 }
+// the last table made, for the next call of the same shape
+static void half_turns(int head_dim, float theta, HalfTurns& F)
+{
+    static std::mutex mu;
+    static HalfTurns cached;
+    static int c_dim = 0;
+    static float c_theta = 0.f;
+    std::lock_guard<std::mutex> lk(mu);
+    if (c_dim != head_dim || c_theta != theta) {
+        for (int d = 0; d < head_dim / 2; d++) cached.f[d] = std::pow((double)theta, -2.0 * d / head_dim) / 3.14159265358979323846;
+        c_dim = head_dim; c_theta = theta;
+    }
+    F = cached;
+}
 static int paged_status(PagedArgs& C, const char* who)
 {
     C.status = device_status_word();
@@ -364,7 +378,7 @@ int s12_rope_store_kv_paged_async(const float* q, int q_stride, const float* k, 
         return fail(S12_ERR_BAD_ARG, "%s: a row stride shorter than the row, or theta not above 0", who);
     if ((rc = paged_status(P.c, who)) != S12_OK) return rc;
     HalfTurns F;
-    for (int d = 0; d < hd / 2; d++) F.f[d] = std::pow((double)theta, -2.0 * d / hd) / 3.14159265358979323846;
+    half_turns(hd, theta, F);
     P.q = q; P.k = k; P.v = v; P.q_out = q_out;
     P.q_stride = q_stride; P.kv_stride = kv_stride; P.q_out_stride = q_out_stride; P.n_head = n_head;
     const bool rows16 = hd % 8 == 0 && ((q_stride | kv_stride | q_out_stride) & 3) == 0 &&

@@ -34,6 +34,14 @@ def _stream(stream=None) -> int:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(stream, dev: int) -> int:
+    """As ``_stream``, for the device that the caller has found to be the current one."""
+    return _raw_stream(dev) if stream is None and _raw_stream is not None else _stream(stream)
+
+
 @dataclass
 class CompressedWeight:
     """One packed tensor resident on a device (engine/model.h:21-40)."""
@@ -449,61 +457,66 @@ class Split12Engine:
               "launch_attention_all_heads_batch")
 
     # ---- the paged INT8 cache: codes int8 [pages][kv heads][page size][head dim], scales fp32 without the last -----------
+    # The checks below are written for speed: a decode step makes these calls for every layer.
     @staticmethod
-    def _paged_kv(kv_k, kv_v, scale_k, scale_v) -> S12PagedKv:
-        shape = kv_k.shape[-4:]
-        if not (kv_k.dtype == kv_v.dtype == torch.int8 and scale_k.dtype == scale_v.dtype == torch.float32 and kv_k.dim() >= 4
-                and kv_v.shape == kv_k.shape and scale_k.shape == scale_v.shape == kv_k.shape[:-1]):
+    def _paged_kv(kv_k, kv_v, scale_k, scale_v):
+        """The cache as the library sees it, and its device's index."""
+        shape, scales = kv_k.shape, scale_k.shape
+        if not (kv_k.dtype is kv_v.dtype is torch.int8 and scale_k.dtype is scale_v.dtype is torch.float32 and len(shape) >= 4
+                and kv_v.shape == shape and scale_v.shape == scales == shape[:-1]):
             raise ValueError("a paged cache is int8 [..., pages, kv heads, page size, head dim] twice and fp32 without the last twice")
         if not (kv_k.is_contiguous() and kv_v.is_contiguous() and scale_k.is_contiguous() and scale_v.is_contiguous()):
             raise ValueError("a paged cache must be contiguous")
         dev = kv_k.get_device()
         if dev != torch.cuda.current_device() or not dev == kv_v.get_device() == scale_k.get_device() == scale_v.get_device():
             raise ValueError(f"the cache must be on the current device, cuda:{torch.cuda.current_device()}")
-        return S12PagedKv(kv_k.data_ptr(), kv_v.data_ptr(), scale_k.data_ptr(), scale_v.data_ptr(), *shape[:1], shape[2], shape[1], shape[3])
+        pages, heads, page, dim = shape[-4:]
+        return S12PagedKv(kv_k.data_ptr(), kv_v.data_ptr(), scale_k.data_ptr(), scale_v.data_ptr(), pages, page, heads, dim), dev
 
     @staticmethod
     def _paged_batch(block_table, kv_len, q_start, tokens: int, max_new: int, max_len: int, dev: int) -> S12PagedBatch:
-        seqs = kv_len.numel()
-        if not (block_table.dtype == kv_len.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == seqs
-                and block_table.stride(1) == 1 and kv_len.is_contiguous()):
-            raise ValueError("block_table is int32 [sequences][pages] with dense rows, kv_len int32 [sequences]")
-        if q_start is not None and not (q_start.dtype == torch.int32 and q_start.numel() == seqs + 1 and q_start.is_contiguous()
-                                        and q_start.get_device() == dev):
+        i32, seqs, (rows, pages), (stride, dense) = torch.int32, kv_len.numel(), block_table.shape, block_table.stride()
+        if not (block_table.dtype is kv_len.dtype is i32 and rows == seqs and (dense == 1 or pages == 1) and kv_len.is_contiguous()
+                and block_table.get_device() == dev == kv_len.get_device()):
+            raise ValueError("block_table is int32 [sequences][pages] with dense rows, kv_len int32 [sequences], both on the cache's device")
+        if q_start is None:
+            start = None
+        elif q_start.dtype is i32 and q_start.numel() == seqs + 1 and q_start.is_contiguous() and q_start.get_device() == dev:
+            start = q_start.data_ptr()
+        else:
             raise ValueError("q_start is int32 [sequences + 1], on the cache's device")
-        if block_table.get_device() != dev or kv_len.get_device() != dev:
-            raise ValueError("block_table and kv_len must be on the cache's device")
-        pages = block_table.shape[1]
-        return S12PagedBatch(block_table.data_ptr(), kv_len.data_ptr(), _ptr(q_start), seqs, max(block_table.stride(0), pages), pages,
-                             tokens, max_new, max_len)
+        return S12PagedBatch(block_table.data_ptr(), kv_len.data_ptr(), start, seqs, stride if rows > 1 else pages, pages, tokens, max_new, max_len)
 
     @staticmethod
-    def _rows(dev: int, dtype, width: int, **tensors) -> int:
-        """Checks [rows][at least width] tensors with dense rows; returns the number of rows, the same in all."""
-        rows = -1
-        for name, t in tensors.items():
-            if t.dtype != dtype or t.dim() != 2 or t.shape[1] < width or t.stride(1) != 1 or t.get_device() != dev:
-                raise ValueError(f"{name} must be {dtype} [tokens][{width}] with dense rows, on the cache's device")
-            if rows not in (-1, t.shape[0]):
-                raise ValueError(f"{name} has {t.shape[0]} rows, not {rows}")
-            rows = t.shape[0]
-        return rows
+    def _rows(name: str, t, dtype, width: int, dev: int):
+        """(rows, row stride) of a [rows][at least width] tensor with dense rows."""
+        rows, columns = t.shape
+        stride, dense = t.stride()
+        if t.dtype is not dtype or columns < width or dense != 1 or t.get_device() != dev:
+            raise ValueError(f"{name} must be {dtype} [tokens][{width}] with dense rows, on the cache's device")
+        return rows, stride if rows > 1 else columns
 
     def rope_store_kv_paged(self, q, k, v, kv_k, kv_v, scale_k, scale_v, block_table, kv_len, q_start, n_head: int, theta: float,
                             q_out=None, stream=None) -> None:
         """RoPE of q (into ``q_out``, default in place) and k, INT8 store of k and v, for packed new tokens: rows
         ``q_start[s]:q_start[s+1]`` are the last positions of sequence s, whose length with them is ``kv_len[s]``
         (``q_start`` None: one token per sequence)."""
-        kv = self._paged_kv(kv_k, kv_v, scale_k, scale_v)
-        dev, hd = kv_k.get_device(), kv.head_dim
-        q_out = q if q_out is None else q_out
-        rows = self._rows(dev, torch.float32, n_head * hd, q=q, q_out=q_out)
-        if self._rows(dev, torch.float32, kv.n_head_kv * hd, k=k, v=v) != rows or k.stride(0) != v.stride(0):
-            raise ValueError("k and v must have q's rows and one row stride")
+        kv, dev = self._paged_kv(kv_k, kv_v, scale_k, scale_v)
+        width, f32 = n_head * kv.head_dim, torch.float32
+        rows, q_stride = self._rows("q", q, f32, width, dev)
+        if q_out is None:
+            q_out, out_rows, out_stride = q, rows, q_stride
+        else:
+            out_rows, out_stride = self._rows("q_out", q_out, f32, width, dev)
+        width = kv.n_head_kv * kv.head_dim
+        k_rows, k_stride = self._rows("k", k, f32, width, dev)
+        if not rows == out_rows == k_rows or (k_rows, k_stride) != self._rows("v", v, f32, width, dev):
+            raise ValueError("k, v and q_out must have q's rows, and k and v one row stride")
         b = self._paged_batch(block_table, kv_len, q_start, rows, 1, 1, dev)
-        check(self.lib.s12_rope_store_kv_paged_async(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), k.stride(0), q_out.data_ptr(),
-                                                     q_out.stride(0), C.byref(kv), C.byref(b), n_head, theta, _stream(stream)),
-              "s12_rope_store_kv_paged_async")
+        rc = self.lib.s12_rope_store_kv_paged_async(q.data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), k_stride, q_out.data_ptr(), out_stride,
+                                                    C.byref(kv), C.byref(b), n_head, theta, _stream_of(stream, dev))
+        if rc:
+            check(rc, "s12_rope_store_kv_paged_async")
 
     def attention_paged_workspace(self, n_head: int, n_head_kv: int, head_dim: int, num_seqs: int, max_new: int, device="cuda") -> torch.Tensor:
         """A zeroed workspace for ``attention_paged`` calls of up to these sizes; one for each stream or graph whose calls may overlap."""
@@ -516,32 +529,36 @@ class Split12Engine:
                         max_new: int, max_len: int, workspace: Optional[torch.Tensor] = None, stream=None) -> None:
         """Causal attention of packed new tokens over the pages (rows as in ``rope_store_kv_paged``) into ``out_bf16`` int16.
         ``max_new`` / ``max_len`` bound a sequence's new tokens and length, also for later replays of a captured graph.
-        Without a ``workspace`` one is allocated and cleared by the call."""
-        kv = self._paged_kv(kv_k, kv_v, scale_k, scale_v)
-        dev, hd = kv_k.get_device(), kv.head_dim
-        rows = self._rows(dev, torch.float32, n_head * hd, q=q)
-        if self._rows(dev, torch.int16, n_head * hd, out_bf16=out_bf16) != rows:
+        Without a ``workspace`` (on the current stream only) one is allocated and cleared by the call."""
+        kv, dev = self._paged_kv(kv_k, kv_v, scale_k, scale_v)
+        width = n_head * kv.head_dim
+        rows, q_stride = self._rows("q", q, torch.float32, width, dev)
+        out_rows, out_stride = self._rows("out_bf16", out_bf16, torch.int16, width, dev)
+        if rows != out_rows:
             raise ValueError("out_bf16 must have q's rows")
         b = self._paged_batch(block_table, kv_len, q_start, rows, max_new, max_len, dev)
         if workspace is None:
-            workspace = self.attention_paged_workspace(n_head, kv.n_head_kv, hd, b.num_seqs, max_new, kv_k.device)
+            if stream is not None:
+                raise ValueError("a call on a stream of the caller's needs a workspace")
+            workspace = self.attention_paged_workspace(n_head, kv.n_head_kv, kv.head_dim, b.num_seqs, max_new, kv_k.device)
         elif workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError("the workspace must be contiguous, on the cache's device")
-        check(self.lib.s12_attention_paged_async(q.data_ptr(), q.stride(0), C.byref(kv), C.byref(b), out_bf16.data_ptr(), out_bf16.stride(0),
-                                                 n_head, scale, workspace.data_ptr(), workspace.nbytes, _stream(stream)),
-              "s12_attention_paged_async")
+        rc = self.lib.s12_attention_paged_async(q.data_ptr(), q_stride, C.byref(kv), C.byref(b), out_bf16.data_ptr(), out_stride, n_head, scale,
+                                                workspace.data_ptr(), workspace.nbytes, _stream_of(stream, dev))
+        if rc:
+            check(rc, "s12_attention_paged_async")
 
     def copy_pages(self, kv_k, kv_v, scale_k, scale_v, src, dst, stream=None) -> None:
         """Pages ``src[i]`` to ``dst[i]`` (int32, on the device) in every layer of [layers][pages]... arrays.  The ``dst`` pages
         differ from one another and from all of ``src``."""
-        kv = self._paged_kv(kv_k, kv_v, scale_k, scale_v)
-        dev = kv_k.get_device()
-        if not (src.dtype == dst.dtype == torch.int32 and src.dim() == 1 and src.shape == dst.shape and src.is_contiguous()
+        kv, dev = self._paged_kv(kv_k, kv_v, scale_k, scale_v)
+        if not (src.dtype is dst.dtype is torch.int32 and src.dim() == 1 and src.shape == dst.shape and src.is_contiguous()
                 and dst.is_contiguous() and src.get_device() == dst.get_device() == dev):
             raise ValueError("src and dst are int32 lists of one length, on the cache's device")
         layers = kv_k.numel() // max(1, kv.num_pages * kv.n_head_kv * kv.page_size * kv.head_dim)
-        check(self.lib.s12_copy_pages_async(C.byref(kv), layers, src.data_ptr(), dst.data_ptr(), src.numel(), _stream(stream)),
-              "s12_copy_pages_async")
+        rc = self.lib.s12_copy_pages_async(C.byref(kv), layers, src.data_ptr(), dst.data_ptr(), src.numel(), _stream_of(stream, dev))
+        if rc:
+            check(rc, "s12_copy_pages_async")
 
     def init(self) -> None:
         """Per-device set-up ahead of the first call (s12_init): status word, GEMM workspace, kernel attributes."""
