@@ -30,6 +30,7 @@ constexpr int kDecCtasPerSm = 3;                    // resident with 8 rows; 2 w
 __host__ __device__ constexpr int dec_ctas_per_sm(int tiles) { return tiles == 1 ? kDecCtasPerSm : 2; }
 constexpr int kDecMaxRows = 16, kDecMaxDim = 128;
 constexpr int kDecMostRows = 64;                    // of a sequence and kv head: in groups of 16
+constexpr int kDecWhole = 16;                       // chunks up to which a warp's item is never cut
 constexpr int kDecGroup = 16;                       // parts that are added up together
 constexpr float kDigits = 32512.f;                  // 127 * 256: the high digit stays below 128
 // a partial result: [rows][head_dim], then [rows][max, sum], then the same of a group that begins with this part
@@ -42,6 +43,7 @@ struct DecodeParams {
     unsigned int* items_done;   // [items] groups of an item that are there, zero between calls
     int row_groups;             // groups of rows of a kv head
     int min_units;              // units of a part, at least
+    int whole;                  // no item is cut, whatever its length: a team's item follows from its number
     int teams;                  // that are resident together
     uint32_t gqa_mul;           // ceil(2^20 / query heads of a kv head): x / that for x below 2^10
 };
@@ -171,39 +173,44 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
     auto team_sync = [] { if (kTeam > 1) __syncthreads(); else __syncwarp(); };
 
     // ---- this team's part: part `part` of `parts` of item `item` of sequence seq; slot0: the item's first slot
-    const int per_lane = (C.num_seqs + 31) >> 5;
-    const uint32_t most = dec_part_units(P, kUnit, per_seq, per_lane);
     int seq = -1, parts = 0, slot0 = 0;
-    uint32_t units = 0, left = team;                               // left: teams of the sequences from here on that come before this one
-    // the lane whose sequences hold the team, then the sequence: two scans, each of (teams, slots) of a lane's sequences
-    for (int s0 = 0, per = per_lane, n_seqs = C.num_seqs; ; ) {
-        uint32_t n = 0, cut = 0, u = 0, parts_of = 0;
+    uint32_t units = 0, left = team;
+    if (P.whole) {
+        if (team < C.num_seqs * per_seq) { seq = team / per_seq; left = team - seq * per_seq; parts = 1; }
+    } else {
+        const int per_lane = (C.num_seqs + 31) >> 5;
+        const uint32_t most = dec_part_units(P, kUnit, per_seq, per_lane);
+        // left: teams of the sequences from here on that come before this one
+        // the lane whose sequences hold the team, then the sequence: two scans, each of (teams, slots) of a lane's sequences
+        for (int s0 = 0, per = per_lane, n_seqs = C.num_seqs; ; ) {
+            uint32_t n = 0, cut = 0, u = 0, parts_of = 0;
 #pragma unroll 4
-        for (int s = s0 + lane * per; s < min(s0 + (lane + 1) * per, n_seqs); s++) {
-            u = dec_units(C, s, kUnit);
-            parts_of = (u + most - 1) / most;
-            n += parts_of; cut += parts_of > 1 ? parts_of : 0;
-        }
-        unsigned long long mine = (unsigned long long)(n * per_seq) | (unsigned long long)(cut * per_seq) << 32, upto = mine;
+            for (int s = s0 + lane * per; s < min(s0 + (lane + 1) * per, n_seqs); s++) {
+                u = dec_units(C, s, kUnit);
+                parts_of = (u + most - 1) / most;
+                n += parts_of; cut += parts_of > 1 ? parts_of : 0;
+            }
+            unsigned long long mine = (unsigned long long)(n * per_seq) | (unsigned long long)(cut * per_seq) << 32, upto = mine;
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const unsigned long long o = __shfl_up_sync(0xFFFFFFFFu, upto, off);
-            if (lane >= off) upto += o;
+            for (int off = 1; off < 32; off <<= 1) {
+                const unsigned long long o = __shfl_up_sync(0xFFFFFFFFu, upto, off);
+                if (lane >= off) upto += o;
+            }
+            const unsigned over = __ballot_sync(0xFFFFFFFFu, (uint32_t)upto > left);
+            const int l = over ? __ffs(over) - 1 : 31;
+            const unsigned long long before = __shfl_sync(0xFFFFFFFFu, over ? upto - mine : upto, l);
+            if (over || per == 1) { left -= (uint32_t)before; slot0 += (int)(before >> 32); }
+            if (per == 1) {
+                if (over) { seq = s0 + l; units = __shfl_sync(0xFFFFFFFFu, u, l); parts = (int)__shfl_sync(0xFFFFFFFFu, parts_of, l); break; }
+                s0 += 32;
+                if (s0 >= n_seqs) break;
+                continue;
+            }
+            if (!over) break;
+            s0 += l * per;
+            n_seqs = min(s0 + per, n_seqs);
+            per = 1;
         }
-        const unsigned over = __ballot_sync(0xFFFFFFFFu, (uint32_t)upto > left);
-        const int l = over ? __ffs(over) - 1 : 31;
-        const unsigned long long before = __shfl_sync(0xFFFFFFFFu, over ? upto - mine : upto, l);
-        if (over || per == 1) { left -= (uint32_t)before; slot0 += (int)(before >> 32); }
-        if (per == 1) {
-            if (over) { seq = s0 + l; units = __shfl_sync(0xFFFFFFFFu, u, l); parts = (int)__shfl_sync(0xFFFFFFFFu, parts_of, l); break; }
-            s0 += 32;
-            if (s0 >= n_seqs) break;
-            continue;
-        }
-        if (!over) break;
-        s0 += l * per;
-        n_seqs = min(s0 + per, n_seqs);
-        per = 1;
     }
     if (seq < 0) return;                                           // more teams than parts
     const int item = (int)(left / (uint32_t)parts), part = (int)left - item * parts;
@@ -219,20 +226,25 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
         paged_rows(C, seq, lo, hi);
         const int rows = min(kRows, (hi - lo) * gqa - row_base);   // rows of this item; 0 or less: none
         if (rows > 0) {
+            const int t_lo = P.whole ? 0 : (int)((unsigned long long)units * part / parts) * kUnit;
+            // the first chunks' pages are asked for before the lengths are there
+            const int kt = (g >> 2) * 16, vt = (t4 >> 1) * 16;
+            const int* table = C.table + (size_t)seq * C.table_stride;
+            auto entry_at = [&](int t) { return (t >> C.page_shift) < C.table_pages ? table[t >> C.page_shift] : -1; };
+            int t0 = t_lo + tw * kDecChunk;
+            const int entry[4] = {entry_at(t0 + kt), entry_at(t0 + vt), entry_at(t0 + kUnit + kt), entry_at(t0 + kUnit + vt)};
             const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // row r sees min(before + token, room) positions
             const int least = min(before + token_of(row_base), room), most_seen = min(before + token_of(row_base + rows - 1), room);
-            const int t_lo = (int)((unsigned long long)units * part / parts) * kUnit;
-            const int t_hi = (int)min((long long)((unsigned long long)units * (part + 1) / parts) * kUnit, (long long)most_seen);
-            const int* table = C.table + (size_t)seq * C.table_stride;
+            const int t_hi = P.whole ? most_seen : (int)min((long long)((unsigned long long)units * (part + 1) / parts) * kUnit, (long long)most_seen);
             bool missing = false;
-            // page of position t; -1: none, or t not below t_hi
-            auto page_at = [&](int t) {
+            // the page of position t, whose table entry was read; -1: none, or t not below t_hi
+            auto page_of = [&](int entry, int t) {
                 if (t >= t_hi) return -1;
-                const int p = table[t >> C.page_shift];
-                if ((unsigned)p < (unsigned)C.num_pages) return p;
+                if ((unsigned)entry < (unsigned)C.num_pages) return entry;
                 missing = true;
                 return -1;
             };
+            auto page_at = [&](int t) { return page_of(t < t_hi ? entry_at(t) : -1, t); };
             // row of the pools' arrays (2^32 rows are more than a GPU holds); absent pages read page 0, masked later
             auto row_at = [&](int page, int t) { return (((uint32_t)max(page, 0) * C.n_head_kv + kvh) << C.page_shift) + (t & (ps - 1)); };
             KRow<kHD> k[4];
@@ -251,10 +263,8 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
             auto fetch_s = [&](float4 (&s)[2], const float* scales, uint32_t at) {
                 s[0] = *reinterpret_cast<const float4*>(scales + at); s[1] = *reinterpret_cast<const float4*>(scales + at + 4);
             };
-            int t0 = t_lo + tw * kDecChunk;
             // a chunk has one page, or two of 16 positions: K rows 4 g + u lie in the half of g >> 2, V rows 8 t4 + u of t4 >> 1
-            const int kt = (g >> 2) * 16, vt = (t4 >> 1) * 16;
-            int pk = page_at(t0 + kt), pv = page_at(t0 + vt), pk_next = page_at(t0 + kUnit + kt), pv_next = page_at(t0 + kUnit + vt);
+            int pk = page_of(entry[0], t0 + kt), pv = page_of(entry[1], t0 + vt), pk_next = page_of(entry[2], t0 + kUnit + kt), pv_next = page_of(entry[3], t0 + kUnit + vt);
             float4 qv[kRows];                                      // lane: dims 4 lane .. + 3 of every row
 #pragma unroll
             for (int r = 0; r < kRows; r++) {
@@ -557,11 +567,12 @@ int64_t paged_decode_workspace_bytes(int n_head, int n_head_kv, int num_seqs, in
 template <int kHD, int kTiles, int kTeam>
 static int decode_launch(DecodeParams P, void* stream, const char* who)
 {
+    P.whole = P.a.c.max_len <= kTeam * kDecChunk * (kTeam == 1 ? kDecWhole : P.min_units);
     // at most, by the caller's bounds: every item whole, and what cutting adds; a grid for less than all resident teams
     P.teams = (int)dec_teams(kTeam) * dec_ctas_per_sm(kTiles) / kDecCtasPerSm;
     const long long items = (long long)P.a.c.num_seqs * P.a.c.n_head_kv * P.row_groups;
     const long long parts = (P.a.c.max_len + (long long)kTeam * kDecChunk * P.min_units - 1) / ((long long)kTeam * kDecChunk * P.min_units);
-    const long long grid = (std::min(items * parts, items + P.teams) * kTeam + kDecWarps - 1) / kDecWarps;
+    const long long grid = ((P.whole ? items : std::min(items * parts, items + P.teams)) * kTeam + kDecWarps - 1) / kDecWarps;
     if (grid > 0x7FFFFFFF) return fail(S12_ERR_TOO_LARGE, "%s: %lld sequences' heads", who, items);
     return launch(paged_decode_kernel<kHD, kTiles, kTeam>, dim3((unsigned)grid), dim3(kDecThreads), 0, stream, who, P);
 }
