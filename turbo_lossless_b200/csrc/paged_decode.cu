@@ -110,29 +110,33 @@ __device__ __forceinline__ uint32_t dec_units(const PagedArgs& C, int s, int uni
     return n <= 0 ? 1u : (uint32_t)(n + unit - 1) / (uint32_t)unit;
 }
 // The most units of a part: the least that gives all items' parts to resident teams.  With so many items that this would
-// cut nothing or nearly nothing, twice a team's share: only what is far longer than the others is cut.  For a whole warp;
-// a lane looks at `per_lane` neighbouring sequences.
+// cut nothing or nearly nothing, twice a team's share: only what is far longer than the others is cut (cutting all of 2400
+// items so that they fill two rounds of 1776 teams measured the same).  At least min_units, and a 128th of the longest item:
+// adding up more parts takes longer than they save.  For a whole warp; a lane looks at `per_lane` neighbouring sequences.
 __device__ __forceinline__ uint32_t dec_part_units(const DecodeParams& P, int unit, int per_seq, int per_lane)
 {
     const PagedArgs& C = P.a.c;
     const int first = (threadIdx.x & 31) * per_lane, end = min(first + per_lane, C.num_seqs);
-    auto sum = [&](uint32_t most) {                                // parts of all items; most = 0: their units
-        uint32_t n = 0;
+    uint32_t n = 0, top = 0;
 #pragma unroll 4
-        for (int s = first; s < end; s++) {
-            const uint32_t u = dec_units(C, s, unit);
-            n += most ? (u + most - 1) / most : u;
-        }
-        return (unsigned long long)__reduce_add_sync(0xFFFFFFFFu, n) * (unsigned long long)per_seq;
-    };
-    const unsigned long long share = div_small(sum(0), P.teams) + 1;
-    uint32_t hi = (uint32_t)min(2 * share, 0x7FFFFFFFull), lo = hi / 2;   // hi is enough: units / hi + items <= teams
-    if (2ull * C.num_seqs * per_seq <= P.teams)
-        while (lo < hi && hi > P.min_units) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (sum(mid) <= (unsigned long long)P.teams) hi = mid; else lo = mid + 1;
-        }
-    return max(hi, (uint32_t)P.min_units);
+    for (int s = first; s < end; s++) {
+        const uint32_t u = dec_units(C, s, unit);
+        n += u; top = max(top, u);
+    }
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    const unsigned long long total = (unsigned long long)__reduce_add_sync(0xFFFFFFFFu, n) * (unsigned long long)per_seq;
+    const unsigned long long items = (unsigned long long)C.num_seqs * per_seq, share = div_small(total, P.teams) + 1;
+    const uint32_t least = max((uint32_t)P.min_units, (top + 127) >> 7);
+    if (2 * items > P.teams) return max((uint32_t)min(2 * share, 0x7FFFFFFFull), least);
+    uint32_t lo = max((uint32_t)share, least), hi = max((uint32_t)div_small(total, P.teams - (uint32_t)items) + 1, lo);   // hi is enough: total / hi + items <= teams
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        uint32_t parts = 0;
+#pragma unroll 4
+        for (int s = first; s < end; s++) parts += (dec_units(C, s, unit) + mid - 1) / mid;
+        if ((unsigned long long)__reduce_add_sync(0xFFFFFFFFu, parts) * (unsigned long long)per_seq <= (unsigned long long)P.teams) hi = mid; else lo = mid + 1;
+    }
+    return lo;
 }
 
 // four values over their sum as bf16
@@ -593,7 +597,7 @@ static int decode_launch_hd(DecodeParams P, int tiles, void* stream, const char*
 {
     const PagedAttn& A = P.a;
     const long long items = (long long)A.c.num_seqs * A.c.n_head_kv * P.row_groups;
-    P.min_units = env_knob("S12_PAGED_MIN_UNITS", 4);
+    P.min_units = env_knob("S12_PAGED_MIN_UNITS", 2);
     if (tiles == 2) return decode_launch<kHD, 2, kDecWarps>(P, stream, who);
     if (items >= env_knob("S12_PAGED_ITEMS", 1000)) return decode_launch<kHD, 1, 1>(P, stream, who);
     return decode_launch<kHD, 1, kDecWarps>(P, stream, who);
