@@ -255,7 +255,8 @@ int s12_version(void);
  * the tensor-core GEMM's roles, 0x8000 a peer wait of the all-reduce,
  * 0x10000-0x80000 the streaming small-batch kernel's weight copies,
  * activation copies, consumers and epilogue / hand-over; 0x100000 is no wait
- * but a page of a paged cache that a block table does not have), including
+ * but a page of a paged cache that a block table does not have; 0x200000 the
+ * attention of prompts over a paged cache), including
  * the word of s12_gemm_noalloc_async.  When it was non-zero the GEMM's
  * hand-over counters are zeroed again, so later launches start clean.
  * Synchronises the device. */

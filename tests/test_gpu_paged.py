@@ -12,6 +12,8 @@ KINDS = {
     "one_token": [(0, 1)],
     "decode": [(n - 1, 1) for n in (1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 200, 1000)],
     "long_decode": [(9000, 1), (4095, 1), (0, 1)],
+    "few_tokens": [(500, 4), (0, 3), (90, 1), (33, 0), (1000, 4), (0, 1), (2, 2)],
+    "two_tokens_far": [(6000, 2), (5, 2)],
     "prompt": [(0, 150)],
     "tile_ends": [(0, n) for n in (31, 32, 33, 63, 64, 65)] + [(0, n) for n in (127, 128, 129)],
     "ragged": [(0, 7), (0, 0), (130, 5), (0, 1), (3, 261), (0, 0)],
@@ -265,3 +267,104 @@ def test_wrappers_refuse_what_the_kernels_cannot_take():
     for edit in (dict(q_start=None), dict(n_head=3), dict(max_new=0), dict(max_len=0), dict(n_head=0)):
         with pytest.raises(S12Error):
             e.attention_paged(**{**ok, **edit})
+
+
+def test_pages_beyond_32_bit_offsets():
+    """A pool of 4.6 GB for K and V each, of which the sequences hold the last pages: every path reads and writes there."""
+    from turbo_lossless_b200 import Split12Engine
+    e, pages = Split12Engine(), 70000
+    pool = [torch.empty(pages, 8, 64, 128, dtype=torch.int8, device="cuda") for _ in "kv"] + [torch.empty(pages, 8, 64, device="cuda") for _ in "kv"]
+    for lens in ([(130, 1), (64, 1)], [(70, 80), (0, 9)]):
+        c = PO.Case(lens, 16, 8, 128, 64, seed=21)
+        small = c.codes[0].shape[0]
+        for x, y in zip(pool, c.cache()):
+            x[pages - small:] = y
+        table = torch.where(c.table >= 0, c.table + (pages - small), -1)
+        q_start = None if c.max_new == 1 else c.q_start
+        _, codes, scales = PO.store(c, 10000.0)
+        e.rope_store_kv_paged(c.q, c.k, c.v, *pool, table, c.kv_len, q_start, 16, 10000.0)
+        for x, y in zip(pool, (*codes, *scales)):
+            assert torch.equal(x[pages - small:].nan_to_num(-1), y.nan_to_num(-1)) if x.is_floating_point() else torch.equal(x[pages - small:], y)
+        c.codes, c.scales = codes, scales
+        out = torch.zeros(c.tokens, 16 * 128, dtype=torch.int16, device="cuda")
+        e.attention_paged(c.q, *pool, out, table, c.kv_len, q_start, 16, 0.1, c.max_new, c.max_len)
+        check(out, *PO.attention(c, 0.1))
+        src, dst = table[0, :2].clone(), torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+        e.copy_pages(*pool, src, dst)
+        assert all(torch.equal(x[dst.long()].nan_to_num(-1) if x.is_floating_point() else x[dst.long()], x[src.long()].nan_to_num(-1) if x.is_floating_point() else x[src.long()]) for x in pool)
+    assert e.device_status() == 0
+
+
+def test_one_workspace_serves_calls_of_other_sizes_in_turn():
+    """The workspace is as it was after every call: whatever came before, a call's bits are the same."""
+    from turbo_lossless_b200 import Split12Engine
+    e = Split12Engine()
+    shapes = [([(9000, 1), (4095, 1), (0, 1)], 8, 1), ([(300, 1)] * 40, 32, 8), ([(2000, 4), (31, 3)], 16, 2), ([(100000, 1)], 4, 4)]
+    cases = [PO.Case(lens, h, hkv, 128, 64, seed=31) for lens, h, hkv in shapes]
+    ws = e.attention_paged_workspace(32, 1, 128, 40, 8)
+    outs = []
+    for turn in range(3):
+        for c in cases[::-1] if turn else cases:
+            out, status = run_attention(c, 0.1, workspace=ws)
+            assert status == 0
+            outs.append((c, out))
+    for c in cases:
+        mine = [o for k, o in outs if k is c]
+        assert all(torch.equal(o, mine[0]) for o in mine)
+        check(mine[0], *PO.attention(c, 0.1))
+    assert not ws.view(torch.int32)[-(32 * 1 * 40 * 2) // 4:].any()
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    from turbo_lossless_b200 import Split12Engine
+    e = Split12Engine()
+    cases = [PO.Case([(20000 + i, 1), (5, 1)], 8, 1, 128, 64, seed=40 + i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    spaces = [e.attention_paged_workspace(8, 1, 128, 2, 1) for _ in cases]
+    outs = [torch.zeros(2, 8 * 128, dtype=torch.int16, device="cuda") for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, st, ws, out in zip(cases, streams, spaces, outs):
+            e.attention_paged(c.q, *c.cache(), out, c.table, c.kv_len, None, 8, 0.1, 1, c.max_len, ws, stream=st)
+    torch.cuda.synchronize()
+    for c, out in zip(cases, outs):
+        check(out, *PO.attention(c, 0.1))
+    with pytest.raises(ValueError):
+        e.attention_paged(cases[0].q, *cases[0].cache(), outs[0], cases[0].table, cases[0].kv_len, None, 8, 0.1, 1, 30000, stream=streams[0])
+
+
+def test_dependent_launches_wait_for_one_another():
+    """Store, attention over what it stored, and a page copy, replayed as a graph of dependent launches."""
+    from turbo_lossless_b200 import Split12Engine
+    e = Split12Engine()
+    for lens in ([(200, 1), (63, 1)], [(64, 100), (0, 40)]):
+        c = PO.Case(lens, 8, 2, 128, 64, seed=51)
+        q_start = None if c.max_new == 1 else c.q_start
+        ws = e.attention_paged_workspace(8, 2, 128, 2, c.max_new)
+        q_out, out = torch.zeros_like(c.q), torch.zeros(c.tokens, 8 * 128, dtype=torch.int16, device="cuda")
+        src, dst = c.table[0, :1].clone(), torch.tensor([sorted(set(range(c.codes[0].shape[0])) - set(c.table.flatten().tolist()))[0]], dtype=torch.int32, device="cuda")
+
+        def step():
+            e.rope_store_kv_paged(c.q, c.k, c.v, *c.cache(), c.table, c.kv_len, q_start, 8, 10000.0, q_out=q_out)
+            e.attention_paged(q_out, *c.cache(), out, c.table, c.kv_len, q_start, 8, 0.1, c.max_new, c.max_len, ws)
+            e.copy_pages(*c.cache(), src, dst)
+        step()
+        torch.cuda.synchronize()
+        old = e.set_dependent_launch(True)
+        try:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                for _ in range(4):
+                    step()
+        finally:
+            e.set_dependent_launch(old)
+        for x in (q_out, out):
+            x.zero_()
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        q = c.q
+        c.q = q_out
+        check(out, *PO.attention(c, 0.1))
+        c.q = q
+        assert torch.equal(c.codes[0][dst.long()], c.codes[0][src.long()]) and e.device_status() == 0

@@ -130,8 +130,8 @@ def test_entry_points_refuse_before_any_device_work():
     lib, p = capi.load(), 4096
     store = lambda kv, b, q=p, qs=512, k=p, v=p, ks=256, o=p, os=512, h=4, th=1e4: lib.s12_rope_store_kv_paged_async(  # noqa: E731
         q, qs, k, v, ks, o, os, C.byref(kv) if kv else None, C.byref(b) if b else None, h, th, None)
-    attend = lambda kv, b, q=p, qs=512, o=p, os=512, h=4, ws=p, n=1 << 40: lib.s12_attention_paged_async(  # noqa: E731
-        q, qs, C.byref(kv) if kv else None, C.byref(b) if b else None, o, os, h, 0.1, ws, n, None)
+    attend = lambda kv, b, q=p, qs=512, o=p, os=512, h=4, ws=p, n=1 << 40, sc=0.1: lib.s12_attention_paged_async(  # noqa: E731
+        q, qs, C.byref(kv) if kv else None, C.byref(b) if b else None, o, os, h, sc, ws, n, None)
     copy = lambda kv, layers=2, s=p, d=p, n=1: lib.s12_copy_pages_async(C.byref(kv) if kv else None, layers, s, d, n, None)  # noqa: E731
 
     def refused(rc, name):
@@ -155,7 +155,7 @@ def test_entry_points_refuse_before_any_device_work():
     for edit in (dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(qs=511), dict(os=511), dict(ks=255), dict(h=3), dict(h=1), dict(h=0),
                  dict(th=0.0), dict(th=-1.0), dict(th=float("nan")), dict(th=float("inf"))):
         refused(store(kv, b, **edit), b"s12_rope_store_kv_paged_async")
-    for edit in (dict(q=None), dict(o=None), dict(qs=511), dict(os=511), dict(h=3), dict(h=0)):
+    for edit in (dict(q=None), dict(o=None), dict(qs=511), dict(os=511), dict(h=3), dict(h=0), dict(sc=float("nan")), dict(sc=float("inf"))):
         refused(attend(kv, b, **edit), b"s12_attention_paged_async")
     for f in ("max_new", "max_len"):
         kv, b = good()

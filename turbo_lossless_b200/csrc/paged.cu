@@ -433,8 +433,8 @@ int s12_attention_paged_async(const float* q, int q_stride, const S12PagedKv* kv
     if (!rc) rc = paged_batch_args(P.c, batch, n_head, who);
     if (rc) return rc;
     if (!q || !out_bf16) return fail(S12_ERR_BAD_ARG, "%s: null argument", who);
-    if (q_stride < n_head * kv->head_dim || out_stride < n_head * kv->head_dim || batch->max_new < 1 || batch->max_len < 1)
-        return fail(S12_ERR_BAD_ARG, "%s: a row stride shorter than the row, or max_new or max_len below 1", who);
+    if (q_stride < n_head * kv->head_dim || out_stride < n_head * kv->head_dim || batch->max_new < 1 || batch->max_len < 1 || !std::isfinite(scale))
+        return fail(S12_ERR_BAD_ARG, "%s: a row stride shorter than the row, max_new or max_len below 1, or a scale that is not finite", who);
     if ((rc = paged_status(P.c, who)) != S12_OK) return rc;
     P.q = q; P.out = (int16_t*)out_bf16; P.q_stride = q_stride; P.out_stride = out_stride; P.n_head = n_head; P.scale = scale;
     P.max_new = batch->max_new; P.c.max_len = batch->max_len; P.workspace = workspace; P.workspace_bytes = workspace_bytes;
