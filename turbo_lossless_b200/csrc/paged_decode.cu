@@ -29,7 +29,7 @@ constexpr int kDecChunk = 32;                       // positions of a warp's ste
 constexpr int kDecCtasPerSm = 3;                    // resident with 8 rows; 2 with 16
 __host__ __device__ constexpr int dec_ctas_per_sm(int tiles) { return tiles == 1 ? kDecCtasPerSm : 2; }
 constexpr int kDecMaxRows = 16, kDecMaxDim = 128;
-constexpr int kDecMostRows = 64;                    // of a sequence and kv head: in groups of 16
+constexpr int kDecMostRows = 1024;                  // of a sequence and kv head: in groups of 16
 constexpr int kDecWhole = 16;                       // chunks up to which a warp's item is never cut
 constexpr int kDecGroup = 16;                       // parts that are added up together
 constexpr float kDigits = 32512.f;                  // 127 * 256: the high digit stays below 128
@@ -609,6 +609,12 @@ int paged_decode_launch(const PagedAttn& A, void* stream, const char* who)
     const int hd = A.c.head_dim, gqa = A.n_head / A.c.n_head_kv;
     const long long rows = (long long)gqa * A.max_new;
     if ((hd != 64 && hd != 96 && hd != 128) || rows > kDecMostRows) return 1;
+    // Groups of 16 rows read the cache anew, 256 rows of the other kernel share it, but without cutting the positions.  us here
+    // / there, 8 kv heads of 128: 64 sequences of 8000 positions with 16 rows 288 / 595, 32 rows 552 / 589, 64 rows 957 / 583; one
+    // sequence of 8000 with 128 rows 46 / 120, four 128 / 128, sixteen 529 / 149; one of 128 positions with 128 rows 8.1 / 9.8.
+    const long long groups16 = (rows + 15) / 16 * A.c.num_seqs * A.c.n_head_kv;
+    const int force = env_knob("S12_PAGED_FORCE", 0);              // 1: here, 2: there
+    if (force == 2 || (force == 0 && rows > 32 && groups16 > 192)) return 1;
     const int64_t need = paged_decode_workspace_bytes(A.n_head, A.c.n_head_kv, A.c.num_seqs, A.max_new);
     if (!A.workspace || A.workspace_bytes < need || (reinterpret_cast<uintptr_t>(A.workspace) & 15))
         return fail(S12_ERR_BAD_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
