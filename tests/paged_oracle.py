@@ -50,8 +50,9 @@ def attention(c, scale, absent=()):
 
     The bound counts what the kernels round, each by its half step:
       the output to bf16: 2^-8 of the value;
-      q to 11 significant bits of its row's power of two, or 15 bits of its largest: a score is off by at most
-        d = scale * (2^-11 sum |q||k| + 2^-15 max|q| sum |k|), a weight by (e^(2d) - 1) of itself, numerator and sum alike;
+      q and k to f16, or q to 15 bits of its largest: a score is off by at most
+        d = scale * (2 * 2^-11 sum |q||k| + 2^-15 max|q| sum |k| + 2^-32 max(scale of k) sum |q|), the last for keys below f16's
+        normal numbers; a weight by (e^(2d) - 1) of itself, numerator and sum alike;
       a weight, a value's scale and their product to f16: 3 * 2^-11 of |p v|, and below f16's normal numbers 2^-25 of the
         largest scale for each |code| and 2^-32 of the largest weight; or a weight times its value's scale to 15 bits of the
         largest of 32 neighbours: 2^-15 * 127 of that largest, for each of the 32;
@@ -82,7 +83,8 @@ def attention(c, scale, absent=()):
             den = p.sum(1, keepdim=True)
             den = torch.where(den == 0, 1, den)
             o = p @ v / den
-            d = scale * (2.0 ** -11 * q.abs() @ k.abs().T + 2.0 ** -15 * q.abs().amax(1, keepdim=True) * k.abs().sum(1)[None])
+            d = scale * (2.0 ** -10 * q.abs() @ k.abs().T + 2.0 ** -15 * q.abs().amax(1, keepdim=True) * k.abs().sum(1)[None]
+                         + 2.0 ** -32 * k.abs().amax() * q.abs().sum(1, keepdim=True))
             d = torch.where(seen, d, 0).amax(1, keepdim=True)
             size = p @ v.abs() / den
             top = torch.nn.functional.pad(p * sv, (0, -n % 32)).view(new, -(-n // 32), 32).amax(2).sum(1, keepdim=True) / den

@@ -14,8 +14,9 @@
 //                    tensor memory, V with the dims contiguous), 64 positions at a time: the next 64 scores are there
 //                    when the softmax has done with these
 // Numbers: all operands are f16 (11 significant bits; bf16 would round a weight and a value to 8).  q is multiplied by a
-// power of two that takes its row's largest element to 2^14..2^15.  A K operand is the code, exactly; K's scales multiply
-// the scores in 32 bits.  A weight is at most 2^15: 2^7 times its distance from the row's maximum, which follows the scores
+// power of two that takes its row's largest element to 2^14..2^15.  A K operand is code * scale over a power of two of its
+// tile, rounded once (the scale goes in as two f16 numbers); multiplying the scores by the scales instead took a tenth of the
+// softmax's time.  A weight is at most 2^15: 2^7 times its distance from the row's maximum, which follows the scores
 // only when they exceed it by 2^8, since the sums have to be multiplied then.  A V operand is code * scale / 2^E with one E
 // for all: what the largest scale so far asks for, and six binary orders of room; when that is not enough the sums are
 // multiplied, too.  Sums are 32-bit.
@@ -31,7 +32,7 @@ constexpr int kPrRows = 128;                        // rows of an MMA
 constexpr int kPrTile = 128;                        // positions of a conversion step
 constexpr int kPrHalf = 64;                         // positions of an MMA and softmax step
 constexpr int kPrThreads = 512;
-constexpr int kPrScaleStages = 4;
+constexpr int kPrScaleStages = 4;                    // tiles whose powers of two are kept
 constexpr unsigned int kPrSite = 0x200000u;         // a wait of this kernel gave up
 constexpr float kPrLift = 7.f;                       // weights are multiplied by 2^7: 2^15 at most
 constexpr float kPrSlack = 8.f;                     // a maximum may be exceeded by 2^8 before the sums are scaled
@@ -155,9 +156,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     constexpr int kTileBytes = pr_tile_bytes(kHD), kPieces = kHD / 16;
     extern __shared__ __align__(16) uint8_t pr_smem[];
     __shared__ PrBars bars;
-    __shared__ __align__(16) float sk_s[kPrScaleStages][kPrTile];
-    __shared__ float shift_s[kPrScaleStages];                      // 2^(E before - E) of the tile
-    __shared__ uint32_t top_s[2][4];                               // the converters' largest scale of a tile
+    __shared__ __align__(8) float2 unit_s2[kPrScaleStages];        // of a tile: the power of two of its keys, 2^(E before - E) of its values
+    __shared__ uint2 top_s[2][4];                                  // the converters' largest scales of a tile
     __shared__ float unit_s;                                       // 2^E at the end
     __shared__ __align__(4) uint8_t absent_s[kPrScaleStages][4];   // byte i, bit h: the 16 positions from 32 i + 16 h on have no page
     __shared__ float factor_s[2 * kPrRows];
@@ -242,8 +242,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 const bool fine = top - (27u << 23) < (228u << 23);
                 const float up = fine ? __uint_as_float((268u << 23) - top ^ (P.a.scale < 0.f ? 0x80000000u : 0u)) : 0.f;   // 2^(14 - e)
                 if (in_row) *reinterpret_cast<uint2*>(to + i / 16 * kTileBytes + i % 16 * 1024) = make_uint2(pr_f16x2(v.x * up, v.y * up), pr_f16x2(v.z * up, v.w * up));
-                // above 0: a masked score stays -infinity
-                if (lane == 0) factor_s[warp + 8 * i] = fine ? fmaxf(to_log2 * __uint_as_float(top - (14u << 23)), 1e-37f) : 1e-37f;
+                if (lane == 0) factor_s[warp + 8 * i] = fine ? to_log2 * __uint_as_float(top - (14u << 23)) : 0.f;
             };
             if (((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0) {
                 float4 v[32];
@@ -291,15 +290,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 pr_ld_wait();
                 pr_ready(x[0]);
                 pr_ready(x[1]);
-                const float4* sk = reinterpret_cast<const float4*>(sk_s[j] + b * kPrHalf);
-#pragma unroll
-                for (int c = 0; c < kPrHalf / 4; c++) {
-                    const float4 k = sk[c];
-                    float (&y)[32] = x[c / 8];
-                    const int e = c % 8 * 4;
-                    const Pair u = mul2({y[e], y[e + 1]}, {k.x, k.y}), v = mul2({y[e + 2], y[e + 3]}, {k.z, k.w});
-                    y[e] = u.x; y[e + 1] = u.y; y[e + 2] = v.x; y[e + 3] = v.y;
-                }
+                const float2 unit = unit_s2[j];
+                const float fac = fmaxf(factor * unit.x, 1e-37f);   // above 0: a masked score stays -infinity
                 const int left = limit - h * kPrHalf;               // positions of the half that the row sees
                 const uint32_t absent = *reinterpret_cast<const uint16_t*>(&absent_s[j][2 * b]);
                 if (least - h * kPrHalf < kPrHalf || absent) {
@@ -313,9 +305,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                     t0 = pr_max3(t0, at(c), at(c + 1)); t1 = pr_max3(t1, at(c + 2), at(c + 3));
                     t2 = pr_max3(t2, at(c + 4), at(c + 5)); t3 = pr_max3(t3, at(c + 6), at(c + 7));
                 }
-                const float top = pr_max3(fmaxf(t0, t1), pr_max3(t2, at(kPrHalf - 4), at(kPrHalf - 3)), pr_max3(t3, at(kPrHalf - 2), at(kPrHalf - 1))) * factor;
+                const float top = pr_max3(fmaxf(t0, t1), pr_max3(t2, at(kPrHalf - 4), at(kPrHalf - 3)), pr_max3(t3, at(kPrHalf - 2), at(kPrHalf - 1))) * fac;
                 const bool rise = top > m + kPrSlack;
-                const float shift = b == 0 ? shift_s[j] : 1.f;
+                const float shift = b == 0 ? unit.y : 1.f;
                 if (__any_sync(0xFFFFFFFFu, rise) || shift != 1.f) {
                     const float mn = rise ? top : m, f = pr_exp2(m - mn);
                     m = mn;
@@ -335,11 +327,11 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                         }
                     }
                 }
-                const Pair fac = {factor, factor}, neg = {kPrLift - m, kPrLift - m};
+                const Pair fac2 = {fac, fac}, neg = {kPrLift - m, kPrLift - m};
                 uint32_t p[32];
 #pragma unroll
                 for (int c = 0; c < 32; c++) {
-                    Pair y = fma2({x[c / 16][2 * c % 32], x[c / 16][2 * c % 32 + 1]}, fac, neg);
+                    Pair y = fma2({x[c / 16][2 * c % 32], x[c / 16][2 * c % 32 + 1]}, fac2, neg);
                     y.x = pr_exp2(y.x); y.y = pr_exp2(y.y);
                     l = add2(l, y);
                     p[c] = pr_f16x2(y.x, y.y);
@@ -438,13 +430,14 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             const int st = j & 1;
             const bool absent = row < 0;
             // the values' unit 2^E
-            const uint32_t bits = __float_as_uint(sv) & 0x7FFFFFFFu;
+            const uint32_t bits_k = __float_as_uint(sk) & 0x7FFFFFFFu, bits = __float_as_uint(sv) & 0x7FFFFFFFu;
             const bool fine = bits < 0x7F800000u;
-            const uint32_t top_w = __reduce_max_sync(0xFFFFFFFFu, fine ? bits : 0u);
-            if (lane == 0) top_s[st][cw] = top_w;
+            const uint32_t top_k = __reduce_max_sync(0xFFFFFFFFu, bits_k < 0x7F800000u ? bits_k : 0u), top_v = __reduce_max_sync(0xFFFFFFFFu, fine ? bits : 0u);
+            if (lane == 0) top_s[st][cw] = make_uint2(top_k, top_v);
             named_bar_sync(1, 128);
-            const uint32_t top = max(max(top_s[st][0], top_s[st][1]), max(top_s[st][2], top_s[st][3]));
-            const int e_top = (int)(top >> 23) - 126;               // scales are below 2^e_top
+            const uint2 w0 = top_s[st][0], w1 = top_s[st][1], w2 = top_s[st][2], w3 = top_s[st][3];
+            const int e_top = (int)(max(max(w0.y, w1.y), max(w2.y, w3.y)) >> 23) - 126;   // scales are below 2^e_top
+            const int e_key = min(max((int)(max(max(w0.x, w1.x), max(w2.x, w3.x)) >> 23) - 126 - 8, -100), 100);   // keys below 2^15
             float shift = 1.f;
             if (j == 0 || e_top > E + 8) {
                 const int old = E;
@@ -452,23 +445,35 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 if (j > 0) shift = old - E < -126 ? 0.f : __uint_as_float((uint32_t)(127 + old - E) << 23);
             }
             const float unit = __uint_as_float((uint32_t)(127 - E) << 23);   // 2^-E
-            const float key_scale = fine ? sk : __uint_as_float(0x7FC00000u);
+            const float key_scale = (fine ? sk : __uint_as_float(0x7FC00000u)) * __uint_as_float((uint32_t)(127 - e_key) << 23);
+            const uint32_t key_hi = pr_f16x2(key_scale, 0.f) & 0xFFFFu;       // the scale as a sum of two f16
+            float key_hi_f;
+            asm("{\n\t.reg .b16 h, z;\n\tmov.b32 {h, z}, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(key_hi_f) : "r"(key_hi));
+            const uint32_t key_parts = key_hi | pr_f16x2(0.f, key_scale - key_hi_f);
             // ---- K
             if (j >= 2) wait(bars.k_empty[st], (j >> 1) - 1);
             const uint32_t gone = __ballot_sync(0xFFFFFFFFu, absent);   // a whole half, or rows that nobody sees
-            sk_s[j % kPrScaleStages][mine] = key_scale;
             if (lane == 0) absent_s[j % kPrScaleStages][cw] = (uint8_t)((gone & 1u) | (gone >> 16 & 1u) << 1);
             if (mine == 0) {
-                shift_s[j % kPrScaleStages] = shift;
+                unit_s2[j % kPrScaleStages] = make_float2(__uint_as_float((uint32_t)(127 + e_key) << 23), shift);
                 if (j == n - 1) unit_s = __uint_as_float((uint32_t)(127 + E) << 23);
             }
 #pragma unroll
             for (int it = 0; it < kIts; it++) {
-                if (!live) break;
+                const uint32_t parts = __shfl_sync(0xFFFFFFFFu, key_parts, it * kRowsAt + row_of), f_hi = prmt(parts, parts, 0x1010u), f_lo = prmt(parts, parts, 0x3232u);
+                if (!live) continue;
                 const uint32_t w[4] = {k[it].x, k[it].y, k[it].z, k[it].w};
                 uint32_t y[8];
 #pragma unroll
-                for (int d = 0; d < 4; d++) pr_codes_f16(w[d], y[2 * d], y[2 * d + 1]);
+                for (int d = 0; d < 4; d++) {
+                    pr_codes_f16(w[d], y[2 * d], y[2 * d + 1]);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t low;
+                        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(low) : "r"(y[2 * d + h]), "r"(f_lo));
+                        asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(y[2 * d + h]) : "r"(f_hi), "r"(low));
+                    }
+                }
                 store(k_s + st * kTileBytes, it, y);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
