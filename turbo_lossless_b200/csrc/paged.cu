@@ -30,7 +30,6 @@ struct HalfTurns { double f[128]; };                            // theta^(-2 d /
 
 constexpr int kStoreWarps = 8;
 constexpr int kStoreThreads = kStoreWarps * 32;
-constexpr int kStorePasses = 3;
 
 __device__ __forceinline__ unsigned long long abs_bits(double x) { return (unsigned long long)__double_as_longlong(x) & 0x7FFFFFFFFFFFFFFFull; }
 
@@ -99,6 +98,9 @@ paged_store_kernel(const __grid_constant__ StoreParams P, const __grid_constant_
 // The same for rows on 16-byte boundaries and head_dim a multiple of 8.  Bound: HBM, 4 bytes an element in, 4 or 1 out.
 // A group of lanes has a head, a lane four neighbouring elements of each half, so that a pair lies in one lane; a warp takes
 // kPasses times as many heads as it has groups, all of their loads in flight while the angles are computed, once a CTA.
+// 7 k tokens of 32/8 heads of 128: 61 us (4.7 TB/s), a warp a head 181, one / two / four / six passes 83 / 84 / 73 / 81; bound by a
+// CTA's chain of length, page and angles.  Slower: CTAs that walk neighbouring rows with the next one's loads in flight and
+// the angles turned on from position to position (67), four CTAs an SM in 64 registers (61), fewer 64-bit instructions (65).
 template <int kPasses>
 __global__ void __launch_bounds__(kStoreThreads)
 paged_store_rows_kernel(const __grid_constant__ StoreParams P, const __grid_constant__ HalfTurns F)
@@ -386,10 +388,10 @@ int s12_rope_store_kv_paged_async(const float* q, int q_stride, const float* k, 
     if (rows16) {
         while ((1 << P.group_shift) < hd / 8) P.group_shift++;
         const int all = n_head + 2 * kv->n_head_kv, per_pass = kStoreWarps * (32 >> P.group_shift);
-        const bool many = batch->num_tokens >= sm_count();
-        const int passes = many ? kStorePasses : 1;
-        return launch(many ? paged_store_rows_kernel<kStorePasses> : paged_store_rows_kernel<1>,
-                      dim3(batch->num_tokens, (all + passes * per_pass - 1) / (passes * per_pass)), dim3(kStoreThreads), 0, stream, who, P, F);
+        // Up to three passes a warp, so that the angles are computed once for 48 heads of 128; one where the tokens are few.
+        const int needed = (all + per_pass - 1) / per_pass, parts = batch->num_tokens >= sm_count() ? (needed + 2) / 3 : needed, passes = (needed + parts - 1) / parts;
+        return launch(passes == 1 ? paged_store_rows_kernel<1> : passes == 2 ? paged_store_rows_kernel<2> : paged_store_rows_kernel<3>,
+                      dim3(batch->num_tokens, parts), dim3(kStoreThreads), 0, stream, who, P, F);
     }
     P.heads_per_warp = 1;
     const int heads = n_head + 2 * kv->n_head_kv, per = kStoreWarps * P.heads_per_warp;
