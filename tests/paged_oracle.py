@@ -117,7 +117,7 @@ def store(c, theta):
         for j in (0, 1):
             x = new[j][row:row + n]
             top = x.abs().amax(-1)
-            codes[j][page, :, slot] = torch.where(top[..., None] > 0, x * 127 / torch.where(top > 0, top, 1)[..., None], 0).round().to(torch.int8)
+            codes[j][page, :, slot] = (x * (torch.where(top > 0, top, 1).reciprocal() * 127)[..., None]).round().to(torch.int8)
             scales[j][page, :, slot] = (top / 127).float()
         row += n
     return rotate(c.q).view(c.tokens, -1), codes, scales

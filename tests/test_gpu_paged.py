@@ -377,3 +377,22 @@ def test_dependent_launches_wait_for_one_another():
         check(out, *PO.attention(c, 0.1))
         c.q = q
         assert torch.equal(c.codes[0][dst.long()], c.codes[0][src.long()]) and e.device_status() == 0
+
+
+def test_codes_of_values_on_a_border():
+    """Values of few bits, many of which lie halfway between two codes: both store kernels (rows on 16-byte boundaries, and others)
+    put them where the rounded product with 127 / absmax, to the nearest even code, puts them.  At position 0 k is not turned."""
+    from turbo_lossless_b200 import Split12Engine
+    e = Split12Engine()
+    for n_kv, hd, page in ((4, 128, 64), (2, 20, 16)):
+        c = PO.Case([(0, 1)] * 300, n_kv, n_kv, hd, page, seed=61)
+        g = torch.Generator().manual_seed(62)
+        for name in ("k", "v"):
+            x = torch.randint(-127, 128, (c.tokens, n_kv, hd), generator=g).float() / 2
+            x[..., 0] = torch.randint(100, 128, (c.tokens, n_kv), generator=g)
+            setattr(c, name, (x * torch.randint(1, 50, (c.tokens, n_kv, 1), generator=g)).view(c.tokens, -1).cuda())
+        _, codes, scales = PO.store(c, 10000.0)
+        e.rope_store_kv_paged(c.q, c.k, c.v, *c.cache(), c.table, c.kv_len, None, n_kv, 10000.0)
+        for j in (0, 1):
+            assert torch.equal(c.codes[j], codes[j])
+            assert torch.equal(c.scales[j].nan_to_num(-1), scales[j].nan_to_num(-1))

@@ -15,7 +15,8 @@ namespace s12 {
 
 // ---------------------------------------------------------------------------
 // Store.  angle = position * theta^(-2 d / head_dim); (x0, x1) = elements d, d + head_dim / 2 of a head become
-// (x0 cos - x1 sin, x0 sin + x1 cos); scale = absmax / 127, code = rint(x * 127 / absmax) of the rotated k and of v.
+// (x0 cos - x1 sin, x0 sin + x1 cos); scale = absmax / 127, code = rint(x * (127 * (1 / absmax))) of the rotated k and of v,
+// each operation rounded to 64 bits: so are values on a border between two codes put to one side by all.
 // The angles, k's rotation and the codes are computed in 64 bits (an angle of position 100 000 rounded to 32 bits is off
 // by 4e-3): the cache's bytes are those of the exact values but for ties; q is rotated in 32 bits.
 // ---------------------------------------------------------------------------
@@ -82,10 +83,10 @@ paged_store_kernel(const __grid_constant__ StoreParams P, const __grid_constant_
         }
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-        const double amax = __longlong_as_double((long long)top), inv = 127.0 / amax;   // a NaN counts as the largest
+        const double amax = __longlong_as_double((long long)top), inv = __dmul_rn(1.0 / amax, 127.0);   // a NaN counts as the largest
         const size_t at = ((size_t)page * hkv + kvh) << P.c.page_shift | (size_t)(pos & ((1 << P.c.page_shift) - 1));
         int8_t* dst = (is_v ? P.c.v : P.c.k) + at * hd;
-        auto code = [&](double v) { const double r = rint(v * inv); return (int8_t)(r == r ? (int)fmin(fmax(r, -127.0), 127.0) : 0); };
+        auto code = [&](double v) { const double r = rint(__dmul_rn(v, inv)); return (int8_t)(r == r ? (int)fmin(fmax(r, -127.0), 127.0) : 0); };
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int d = i * 32 + lane;
@@ -162,12 +163,13 @@ paged_store_rows_kernel(const __grid_constant__ StoreParams P, const __grid_cons
         }
         for (int off = 1 << P.group_shift >> 1; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
         if (!keep) continue;
-        const double amax = __longlong_as_double((long long)top), inv = 127.0 / amax;   // a NaN counts as the largest
+        const double amax = __longlong_as_double((long long)top), inv = __dmul_rn(1.0 / amax, 127.0);   // a NaN counts as the largest
         const bool fine = top < 0x7FF0000000000000ull && top > 0;
         uint32_t w[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; e++) {                             // rounded to nearest by 1.5 * 2^52: the low word holds the code
-            const uint32_t r = fine ? (uint32_t)__double2loint(x[e] * inv + 6755399441055744.0) : 0u;
+        for (int e = 0; e < 8; e++) {
+            // rounded to nearest by 1.5 * 2^52: the low word holds the code; the product is rounded first, not fused
+            const uint32_t r = fine ? (uint32_t)__double2loint(__dadd_rn(__dmul_rn(x[e], inv), 6755399441055744.0)) : 0u;
             w[e >> 2] |= (r & 0xFFu) << (8 * (e & 3));
         }
         const int kvh = h - P.n_head - (is_v ? hkv : 0);
