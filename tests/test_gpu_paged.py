@@ -396,3 +396,41 @@ def test_codes_of_values_on_a_border():
         for j in (0, 1):
             assert torch.equal(c.codes[j], codes[j])
             assert torch.equal(c.scales[j].nan_to_num(-1), scales[j].nan_to_num(-1))
+
+
+@pytest.mark.parametrize("lens", [[(300, 1), (0, 1)], [(100, 200), (20, 30)]])
+@pytest.mark.parametrize("hd", [128, 64, 80])
+def test_elements_near_the_largest_float(kernel, lens, hd):
+    """q up to 2e38 under a scale that makes ordinary scores of it; values up to 3e38 / 350, whose sums stay finite."""
+    c = PO.Case(lens, 8, 2, hd, 64, seed=71)
+    c.q *= 2e38 / c.q.abs().max()
+    c.scales[0] *= 0.2
+    c.scales[1] *= 3e38 / 350 / 127 / c.scales[1].nan_to_num(0).max()
+    scale = torch.tensor(1.2e-38).item()
+    out, status = run_attention(c, scale)
+    assert status == 0
+    check(out, *PO.attention(c, scale))
+
+
+def test_one_value_near_the_largest_float(kernel):
+    c = PO.Case([(0, 1), (0, 1)], 8, 2, 128, 64, seed=72)
+    c.codes[1].copy_(c.codes[1] % 2)
+    c.scales[1] /= c.scales[1].nan_to_num(0).max()
+    c.scales[1] *= 3e38
+    out, _ = run_attention(c, 0.1)
+    check(out, *PO.attention(c, 0.1))
+
+
+@pytest.mark.parametrize("lens", [[(300, 1), (40, 1)], [(100, 200), (20, 30)]])
+@pytest.mark.parametrize("hd", [128, 80])
+@pytest.mark.parametrize("size", [1e3, 3e5, -7e6, 1e15, -1e16])
+def test_scores_of_any_size(kernel, lens, hd, size):
+    """All keys alike: equal scores, however large, are equal weights, as those of q = 0."""
+    c = PO.Case(lens, 8, 2, hd, 64, seed=73)
+    c.codes[0][:] = c.codes[0][0, :, :1].clone()
+    c.scales[0].copy_(torch.where(c.scales[0].isnan(), c.scales[0], abs(size)))
+    q = c.q * size
+    c.q.zero_()
+    want = PO.attention(c, 0.1)
+    out, _ = run_attention(c, 0.1, q=q)
+    check(out, *want)

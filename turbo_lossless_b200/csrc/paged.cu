@@ -8,6 +8,7 @@
 //
 // Pages are head-major, [page][kv head][position][head_dim]: what a CTA reads of a page is contiguous.
 #include "paged.cuh"
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 
@@ -24,7 +25,6 @@ struct StoreParams {
     PagedArgs c;
     const float* q; const float* k; const float* v; float* q_out;
     int q_stride, kv_stride, q_out_stride, n_head;
-    int heads_per_warp;         // paged_store_kernel
     int group_shift;            // paged_store_rows_kernel: 2^this lanes have a head
 };
 struct HalfTurns { double f[128]; };                            // theta^(-2 d / head_dim) / pi
@@ -53,47 +53,46 @@ paged_store_kernel(const __grid_constant__ StoreParams P, const __grid_constant_
     if (page < 0 && pos >= 0 && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(P.c.status, kStatusPage);
     __syncthreads();
     const int hkv = P.c.n_head_kv, heads = P.n_head + 2 * hkv;
-    const int first = (blockIdx.y * kStoreWarps + warp) * P.heads_per_warp;
-    for (int h = first; h < first + P.heads_per_warp && h < heads; h++) {
-        if (h < P.n_head) {
-            const float* x = P.q + (size_t)row * P.q_stride + (size_t)h * hd;
-            float* y = P.q_out + (size_t)row * P.q_out_stride + (size_t)h * hd;
-            for (int d = lane; d < half; d += 32) {
-                const float c = (float)cos_s[d], s = (float)sin_s[d], x0 = x[d], x1 = x[d + half];
-                y[d] = x0 * c - x1 * s; y[d + half] = x0 * s + x1 * c;
-            }
-            continue;
+    const int h = blockIdx.y * kStoreWarps + warp;
+    if (h >= heads) return;
+    if (h < P.n_head) {
+        const float* x = P.q + (size_t)row * P.q_stride + (size_t)h * hd;
+        float* y = P.q_out + (size_t)row * P.q_out_stride + (size_t)h * hd;
+        for (int d = lane; d < half; d += 32) {
+            const float c = (float)cos_s[d], s = (float)sin_s[d], x0 = x[d], x1 = x[d + half];
+            y[d] = x0 * c - x1 * s; y[d + half] = x0 * s + x1 * c;
         }
-        if (page < 0) continue;
-        const bool is_v = h >= P.n_head + hkv;
-        const int kvh = h - P.n_head - (is_v ? hkv : 0);
-        const float* x = (is_v ? P.v : P.k) + (size_t)row * P.kv_stride + (size_t)kvh * hd;
-        double lo[4], hi[4];
-        unsigned long long top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int d = i * 32 + lane;
-            if (d >= half) continue;
-            lo[i] = x[d]; hi[i] = x[d + half];
-            if (!is_v) {
-                const double c = cos_s[d], s = sin_s[d], x0 = lo[i], x1 = hi[i];
-                lo[i] = x0 * c - x1 * s; hi[i] = x0 * s + x1 * c;
-            }
-            top = max(top, max(abs_bits(lo[i]), abs_bits(hi[i])));
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-        const double amax = __longlong_as_double((long long)top), inv = __dmul_rn(1.0 / amax, 127.0);   // a NaN counts as the largest
-        const size_t at = ((size_t)page * hkv + kvh) << P.c.page_shift | (size_t)(pos & ((1 << P.c.page_shift) - 1));
-        int8_t* dst = (is_v ? P.c.v : P.c.k) + at * hd;
-        auto code = [&](double v) { const double r = rint(__dmul_rn(v, inv)); return (int8_t)(r == r ? (int)fmin(fmax(r, -127.0), 127.0) : 0); };
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int d = i * 32 + lane;
-            if (d < half) { dst[d] = code(lo[i]); dst[d + half] = code(hi[i]); }
-        }
-        if (lane == 0) (is_v ? P.c.sv : P.c.sk)[at] = (float)(amax / 127.0);
+        return;
     }
+    if (page < 0) return;
+    const bool is_v = h >= P.n_head + hkv;
+    const int kvh = h - P.n_head - (is_v ? hkv : 0);
+    const float* x = (is_v ? P.v : P.k) + (size_t)row * P.kv_stride + (size_t)kvh * hd;
+    double lo[4], hi[4];
+    unsigned long long top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int d = i * 32 + lane;
+        if (d >= half) continue;
+        lo[i] = x[d]; hi[i] = x[d + half];
+        if (!is_v) {
+            const double c = cos_s[d], s = sin_s[d], x0 = lo[i], x1 = hi[i];
+            lo[i] = x0 * c - x1 * s; hi[i] = x0 * s + x1 * c;
+        }
+        top = max(top, max(abs_bits(lo[i]), abs_bits(hi[i])));
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+    const double amax = __longlong_as_double((long long)top), inv = __dmul_rn(1.0 / amax, 127.0);   // a NaN counts as the largest
+    const size_t at = ((size_t)page * hkv + kvh) << P.c.page_shift | (size_t)(pos & ((1 << P.c.page_shift) - 1));
+    int8_t* dst = (is_v ? P.c.v : P.c.k) + at * hd;
+    auto code = [&](double v) { const double r = rint(__dmul_rn(v, inv)); return (int8_t)(r == r ? (int)fmin(fmax(r, -127.0), 127.0) : 0); };
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int d = i * 32 + lane;
+        if (d < half) { dst[d] = code(lo[i]); dst[d + half] = code(hi[i]); }
+    }
+    if (lane == 0) (is_v ? P.c.sv : P.c.sk)[at] = (float)(amax / 127.0);
 }
 
 // The same for rows on 16-byte boundaries and head_dim a multiple of 8.  Bound: HBM, 4 bytes an element in, 4 or 1 out.
@@ -254,7 +253,7 @@ paged_attention_general_kernel(const __grid_constant__ PagedAttn P)
     for (int c = 0; c < 2; c++) {
         live[c] = c * 128 + lane * 4 < hd;
 #pragma unroll
-        for (int e = 0; e < 4; e++) { qv[c][e] = live[c] ? q[c * 128 + lane * 4 + e] : 0.f; acc[c][e] = 0.f; }
+        for (int e = 0; e < 4; e++) { qv[c][e] = live[c] ? q[c * 128 + lane * 4 + e] * P.scale : 0.f; acc[c][e] = 0.f; }
     }
     float m = -INFINITY, l = 0.f;
     bool bad = false;
@@ -273,7 +272,7 @@ paged_attention_general_kernel(const __grid_constant__ PagedAttn P)
         }
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, off);
-        const float s = dot * C.sk[at] * P.scale;
+        const float s = dot * C.sk[at];
         if (s > m) {
             const float f = expf(m - s);
             m = s; l *= f;
@@ -395,9 +394,7 @@ int s12_rope_store_kv_paged_async(const float* q, int q_stride, const float* k, 
         return launch(passes == 1 ? paged_store_rows_kernel<1> : passes == 2 ? paged_store_rows_kernel<2> : paged_store_rows_kernel<3>,
                       dim3(batch->num_tokens, parts), dim3(kStoreThreads), 0, stream, who, P, F);
     }
-    P.heads_per_warp = 1;
-    const int heads = n_head + 2 * kv->n_head_kv, per = kStoreWarps * P.heads_per_warp;
-    return launch(paged_store_kernel, dim3(batch->num_tokens, (heads + per - 1) / per), dim3(kStoreThreads), 0, stream, who, P, F);
+    return launch(paged_store_kernel, dim3(batch->num_tokens, (n_head + 2 * kv->n_head_kv + kStoreWarps - 1) / kStoreWarps), dim3(kStoreThreads), 0, stream, who, P, F);
 }
 
 int s12_copy_pages_async(const S12PagedKv* kv, int layers, const int32_t* src, const int32_t* dst, int count, void* stream)
@@ -441,7 +438,7 @@ int s12_attention_paged_async(const float* q, int q_stride, const S12PagedKv* kv
         return fail(S12_ERR_BAD_ARG, "%s: a row stride shorter than the row, max_new or max_len below 1, or a scale that is not finite", who);
     if ((rc = paged_status(P.c, who)) != S12_OK) return rc;
     P.q = q; P.out = (int16_t*)out_bf16; P.q_stride = q_stride; P.out_stride = out_stride; P.n_head = n_head; P.scale = scale;
-    P.max_new = batch->max_new; P.c.max_len = batch->max_len; P.workspace = workspace; P.workspace_bytes = workspace_bytes;
+    P.max_new = batch->max_new; P.c.max_len = std::min(batch->max_len, kPagedMostPositions); P.workspace = workspace; P.workspace_bytes = workspace_bytes;
     if ((rc = paged_decode_launch(P, stream, who)) <= 0 || (rc = paged_prompt_launch(P, stream, who)) <= 0) return rc;
     return launch(paged_attention_general_kernel, dim3(batch->num_tokens, n_head), dim3(kGenWarps * 32), 0, stream, who, P);
 }

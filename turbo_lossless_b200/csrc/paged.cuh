@@ -4,6 +4,7 @@
 
 namespace s12 {
 
+constexpr int kPagedMostPositions = 0x7FFFFFFF - 4096;     // of a sequence: positions of a step further stay below 2^31
 constexpr unsigned int kStatusPage = 0x100000u;     // a block table entry outside the pool, or a position past the table
 
 // A position t of sequence s lies in page table[s * table_stride + (t >> page_shift)], row t & (page_size - 1):

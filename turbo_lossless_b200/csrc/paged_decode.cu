@@ -33,6 +33,7 @@ constexpr int kDecMostRows = 1024;                  // of a sequence and kv head
 constexpr int kDecWhole = 16;                       // chunks up to which a warp's item is never cut
 constexpr int kDecGroup = 16;                       // parts that are added up together
 constexpr float kDigits = 32512.f;                  // 127 * 256: the high digit stays below 128
+constexpr float kDecLowest = -3e38f;                // a maximum of no scores
 // a partial result: [rows][head_dim], then [rows][max, sum], then the same of a group that begins with this part
 __host__ __device__ constexpr int64_t dec_slot_floats(int rows) { return (int64_t)rows * (kDecMaxDim + 4); }
 
@@ -62,6 +63,9 @@ __device__ __forceinline__ float dec_exp2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// kDigits / top; both quartered, since __fdividef gives 0 for divisors above 2^126
+__device__ __forceinline__ float dec_digits_over(float top) { return __fdividef(kDigits / 4, top * 0.25f); }
 
 // kHD codes of a K row that a lane needs: kHD / 4 consecutive bytes of every 64 (or 32) go to its quad's lanes
 template <int kHD> struct KRow { uint32_t w[kHD / 16]; };
@@ -302,7 +306,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                 bits = __reduce_max_sync(0xFFFFFFFFu, bits);
                 const float top = __uint_as_float(bits);
                 const bool fine = top >= 1e-30f && bits < 0x7F800000u;   // rows of smaller ones count as zero
-                const float inv = fine ? __fdividef(kDigits, top) : 0.f;
+                const float inv = fine ? dec_digits_over(top) : 0.f;
                 uint32_t y[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) y[j] = __float_as_uint(fmaf(fine ? e[j] : 0.f, inv, 12582912.f + 128.f));   // 256 hi + lo + 128
@@ -329,7 +333,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
             float acc[kTiles][kCols][2], m[kTiles], l[kTiles];
 #pragma unroll
             for (int i = 0; i < kTiles; i++) {
-                m[i] = -1e30f; l[i] = 0.f;
+                m[i] = kDecLowest; l[i] = 0.f;
 #pragma unroll
                 for (int j = 0; j < kCols; j++) acc[i][j][0] = acc[i][j][1] = 0.f;
             }
@@ -384,7 +388,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
 #pragma unroll
                         for (int p = 0; p < 8; p++) if (pv < 0 || t0 + 8 * t4 + p >= limit[i]) s[i][p] = -INFINITY;
                     }
-                    float mx = -1e30f;
+                    float mx = kDecLowest;
 #pragma unroll
                     for (int p = 0; p < 8; p++) mx = fmaxf(mx, s[i][p]);
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
@@ -411,7 +415,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                     }
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                    const float inv = top >= 1e-30f ? __fdividef(kDigits, top) : 0.f;
+                    const float inv = top >= 1e-30f ? dec_digits_over(top) : 0.f;
                     uint32_t y[8];                                  // 256 hi + lo + 128 in the low half
 #pragma unroll
                     for (int p = 0; p < 8; p++) y[p] = __float_as_uint(fmaf(z[p], inv, 12582912.f + 128.f));
@@ -504,7 +508,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                 __syncthreads();
                 for (int i = tt; i < rows * (kHD / 4); i += kTeamThreads) {
                     const int r = i / (kHD / 4), d = (i - r * (kHD / 4)) * 4;
-                    float mm = -1e30f, den = 0.f;
+                    float mm = kDecLowest, den = 0.f;
                     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int w = 0; w < kTeam; w++) mm = fmaxf(mm, m_s[w][r]);
@@ -541,7 +545,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                 auto add_up = [&](int first, int step, int n, int stats, bool finish) {
                     for (int i = tt; i < rows * (kHD / 4); i += kTeamThreads) {
                         const int r = i / (kHD / 4), d = (i - r * (kHD / 4)) * 4;
-                        float mm = -1e30f, den = 0.f;
+                        float mm = kDecLowest, den = 0.f;
                         float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
                         for (int j = 0; j < n; j++) {
@@ -589,7 +593,7 @@ static int decode_launch(DecodeParams P, void* stream, const char* who)
     const long long items = (long long)P.a.c.num_seqs * P.a.c.n_head_kv * P.row_groups;
     const long long parts = (P.a.c.max_len + (long long)kTeam * kDecChunk * P.min_units - 1) / ((long long)kTeam * kDecChunk * P.min_units);
     const long long grid = ((P.whole ? items : std::min(items * parts, items + P.teams)) * kTeam + kDecWarps - 1) / kDecWarps;
-    if (grid > 0x7FFFFFFF) return fail(S12_ERR_TOO_LARGE, "%s: %lld sequences' heads", who, items);
+    if (grid > 0x7FFFFFFF || items > 1 << 30) return fail(S12_ERR_TOO_LARGE, "%s: %lld sequences' heads", who, items);
     return launch(paged_decode_kernel<kHD, kTiles, kTeam>, dim3((unsigned)grid), dim3(kDecThreads), 0, stream, who, P);
 }
 template <int kHD>

@@ -34,7 +34,9 @@ constexpr int kPrHalf = 64;                         // positions of an MMA and s
 constexpr int kPrThreads = 512;
 constexpr int kPrScaleStages = 4;                    // tiles whose powers of two are kept
 constexpr unsigned int kPrSite = 0x200000u;         // a wait of this kernel gave up
+constexpr float kPrLowest = -3e38f;                  // a maximum of no scores
 constexpr float kPrLift = 7.f;                       // weights are multiplied by 2^7: 2^15 at most
+constexpr int kPrCtaRows = 2 * kPrRows;             // rows of a CTA
 constexpr float kPrSlack = 8.f;                     // a maximum may be exceeded by 2^8 before the sums are scaled
 
 __host__ __device__ constexpr int pr_tile_bytes(int hd) { return (hd + 63) / 64 * kPrRows * 128; }   // blocks of 64 dims: [128 rows][128 bytes]
@@ -145,7 +147,6 @@ __device__ __forceinline__ uint64_t pr_desc(uint32_t at, uint32_t lead)
 
 struct PromptParams {
     PagedAttn a;
-    int tile_rows;              // rows of a CTA: 128 or 256
     uint32_t gqa_mul;           // ceil(2^32 / query heads of a kv head), 0 for one: divides what is below 2^32 / that number
 };
 
@@ -160,7 +161,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     __shared__ uint2 top_s[2][4];                                  // the converters' largest scales of a tile
     __shared__ float unit_s;                                       // 2^E at the end
     __shared__ __align__(4) uint8_t absent_s[kPrScaleStages][4];   // byte i, bit h: the 16 positions from 32 i + 16 h on have no page
-    __shared__ float factor_s[2 * kPrRows];
+    __shared__ float factor_s[kPrCtaRows];
     __shared__ uint32_t tmem_s;
     __shared__ int s_abort;
     uint8_t* smem = pr_smem + ((1024u - (smem_addr(pr_smem) & 1023u)) & 1023u);
@@ -178,7 +179,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     for (int s1 = C.num_seqs; s1 > 0 && seq < 0; s1 -= 32) {       // sequence s1 - 1 - lane
         const int s = s1 - 1 - lane;
         int a = 0, b = 0, n = 0;
-        if (s >= 0) { paged_rows(C, s, a, b); n = b > a ? (int)(((long long)(b - a) * gqa + P.tile_rows - 1) / P.tile_rows) : 0; }
+        if (s >= 0) { paged_rows(C, s, a, b); n = b > a ? (int)(((long long)(b - a) * gqa + kPrCtaRows - 1) / kPrCtaRows) : 0; }
         int upto = n;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xFFFFFFFFu, upto, off); if (lane >= off) upto += o; }
@@ -192,7 +193,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
         }
     }
     if (seq < 0) return;                                           // more CTAs than tiles
-    const int row0 = tile * P.tile_rows, rows = min(P.tile_rows, (hi - lo) * gqa - row0);
+    const int row0 = tile * kPrCtaRows, rows = min(kPrCtaRows, (hi - lo) * gqa - row0);
     const int n_q = rows > kPrRows ? 2 : 1;                        // row tiles
     const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // token t sees min(before + t, room) positions
     const int seen = max(0, min(before + token_of(row0 + rows - 1), room)), halves = max(1, (seen + kPrHalf - 1) / kPrHalf), n = (halves + 1) / 2;
@@ -277,7 +278,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             const int limit = r < rows ? min(before + tok, room) : 0;       // positions that this row sees
             const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
             const float factor = factor_s[r];
-            float m = -1e30f;
+            float m = kPrLowest;
             Pair l = {0.f, 0.f};
 #pragma unroll 1
             for (int h = 0; h < halves; h++) {
@@ -306,7 +307,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                     t2 = pr_max3(t2, at(c + 4), at(c + 5)); t3 = pr_max3(t3, at(c + 6), at(c + 7));
                 }
                 const float top = pr_max3(fmaxf(t0, t1), pr_max3(t2, at(kPrHalf - 4), at(kPrHalf - 3)), pr_max3(t3, at(kPrHalf - 2), at(kPrHalf - 1))) * fac;
-                const bool rise = top > m + kPrSlack;
+                const bool rise = top - m > kPrSlack;
                 const float shift = b == 0 ? unit.y : 1.f;
                 if (__any_sync(0xFFFFFFFFu, rise) || shift != 1.f) {
                     const float mn = rise ? top : m, f = pr_exp2(m - mn);
@@ -327,7 +328,13 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                         }
                     }
                 }
-                const Pair fac2 = {fac, fac}, neg = {kPrLift - m, kPrLift - m};
+                Pair fac2 = {fac, fac}, neg = {kPrLift - m, kPrLift - m};
+                // Scores this large are their own roundings apart from x * fac, which is not rounded below: a weight could leave f16
+                if (__any_sync(0xFFFFFFFFu, fabsf(m) > 1048576.f && m != kPrLowest)) {
+#pragma unroll
+                    for (int c = 0; c < kPrHalf; c++) x[c / 32][c % 32] = __fsub_rn(__fmul_rn(x[c / 32][c % 32], fac), m);
+                    fac2 = {1.f, 1.f}; neg = {kPrLift, kPrLift};
+                }
                 uint32_t p[32];
 #pragma unroll
                 for (int c = 0; c < 32; c++) {
@@ -595,10 +602,10 @@ int paged_prompt_launch(const PagedAttn& A, void* stream, const char* who)
     const int hd = A.c.head_dim, gqa = A.n_head / A.c.n_head_kv;
     if (hd != 64 && hd != 96 && hd != 128) return 1;
     // rows as far as the division by multiplication holds
-    if ((long long)A.c.num_tokens * gqa + 2 * kPrRows >= (1ll << 32) / gqa) return 1;
-    PromptParams P = {A, 2 * kPrRows, gqa == 1 ? 0u : (uint32_t)(((1ull << 32) + gqa - 1) / gqa)};
+    if ((long long)A.c.num_tokens * gqa + kPrCtaRows >= (1ll << 32) / gqa) return 1;
+    PromptParams P = {A, gqa == 1 ? 0u : (uint32_t)(((1ull << 32) + gqa - 1) / gqa)};
     // every sequence's last tile may be a part of one
-    const long long tiles = (long long)A.c.num_tokens * gqa / P.tile_rows + std::min(A.c.num_seqs, A.c.num_tokens), grid = tiles * A.c.n_head_kv;
+    const long long tiles = (long long)A.c.num_tokens * gqa / kPrCtaRows + std::min(A.c.num_seqs, A.c.num_tokens), grid = tiles * A.c.n_head_kv;
     if (grid > 0x7FFFFFFF) return fail(S12_ERR_TOO_LARGE, "%s: %d tokens", who, A.c.num_tokens);
     return hd == 64 ? prompt_launch<64>(P, grid, stream, who) : hd == 96 ? prompt_launch<96>(P, grid, stream, who) : prompt_launch<128>(P, grid, stream, who);
 }

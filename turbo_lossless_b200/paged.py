@@ -208,8 +208,8 @@ class PagedDecoder:
         c, e = self.cfg, self.eng
         new = [len(t) for t in tokens]
         rows, S = sum(new), len(seqs)
-        if len(set(seqs)) != S or S == 0 or min(new) < 1 or rows > self.max_tokens:
-            raise ValueError(f"needs distinct sequences with a token each, {self.max_tokens} tokens at most")
+        if len(new) != S or len(set(seqs)) != S or S == 0 or min(new) < 1 or rows > self.max_tokens:
+            raise ValueError(f"needs distinct sequences with at least a token each, {self.max_tokens} tokens at most")
         self.cache.extend(dict(zip(seqs, new)))
         dev, hd, scale = self.token_embd.device, c.head_dim, 1.0 / float(c.head_dim) ** 0.5
         starts = [0]
