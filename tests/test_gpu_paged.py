@@ -22,10 +22,12 @@ KINDS = {
 SHAPES = [(32, 8, 128), (8, 8, 128), (8, 1, 128), (6, 2, 128), (10, 2, 64), (16, 1, 96), (4, 2, 64), (40, 2, 128), (2, 2, 20), (4, 2, 80), (2, 1, 256)]
 
 
-@pytest.fixture(params=["rule", "digits", "tiles"])
+@pytest.fixture(params=["rule", "digits", "warps", "tiles"])
 def kernel(request, monkeypatch):
-    """The kernel that the rule chooses, and each of the two for heads of 64, 96 and 128 whatever the rule says."""
-    monkeypatch.setenv("S12_PAGED_FORCE", {"rule": "0", "digits": "1", "tiles": "2"}[request.param])
+    """The kernel that the rule chooses, and each of the two for heads of 64, 96 and 128 whatever the rule says, the first with
+    four warps to a part and with one to an item."""
+    monkeypatch.setenv("S12_PAGED_FORCE", {"rule": "0", "digits": "1", "warps": "1", "tiles": "2"}[request.param])
+    monkeypatch.setenv("S12_PAGED_TEAM", {"rule": "0", "digits": "4", "warps": "1", "tiles": "0"}[request.param])
     return request.param
 
 
@@ -434,3 +436,22 @@ def test_scores_of_any_size(kernel, lens, hd, size):
     want = PO.attention(c, 0.1)
     out, _ = run_attention(c, 0.1, q=q)
     check(out, *want)
+
+
+@pytest.mark.parametrize("many", [90, 700])
+def test_many_sequences_one_of_them_long(kernel, many):
+    """Every team looks at all lengths: several to a lane, more than 32 lanes' worth, and a length array off its boundary."""
+    if kernel == "tiles" and many > 100:
+        pytest.skip("one launch of the other kernel is like any other")
+    lens = [(i * 7 % 60, 1) for i in range(many)]
+    lens[many * 2 // 3] = (5000, 1)
+    c = PO.Case(lens, 4, 1, 64, 32, seed=81)
+    for off in (0, 1):
+        room = torch.zeros(many + 4, dtype=torch.int32, device="cuda")
+        room[off:off + many] = c.kv_len
+        c.kv_len = room[off:off + many]
+        out, status = run_attention(c, 0.125)
+        assert status == 0
+        if off == 0:
+            want = PO.attention(c, 0.125)
+        check(out, *want)

@@ -181,7 +181,8 @@ paged_store_rows_kernel(const __grid_constant__ StoreParams P, const __grid_cons
 }
 
 // ---------------------------------------------------------------------------
-// Copy.  A CTA copies 16 KB of a page in one layer.
+// Copy.  A CTA copies 16 KB of a page in one layer, four 16-byte loads a thread in flight.  Bound: HBM; 300 pages of 8 x 64 x 128
+// in 16 layers 197.5 us (6.57 TB/s, a plain copy's rate), one page in 32 layers 2.8 us.
 // ---------------------------------------------------------------------------
 struct CopyParams {
     uint4* part[4];             // k, v, their scales
@@ -226,7 +227,7 @@ paged_copy_kernel(const __grid_constant__ CopyParams P)
 }
 
 // ---------------------------------------------------------------------------
-// Attention, any head_dim that is a multiple of 4 up to 256: a CTA per (token, query head), a warp per position, running
+// Attention, any other head_dim that is a multiple of 4 up to 256, for completeness: a CTA per (token, query head), a warp per position, running
 // maximum and sum per warp, the warps' partial results merged in shared memory.  Sums in 32 bits.
 // out[t] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q . k_j - m) over the positions j <= position of t; 0 where there
 // is none.

@@ -13,6 +13,8 @@
 //             are the A operand of the second product as they lie, against V's rows in order
 //   dims      column n of PV tile j is dim n * head_dim / 8 + j: a lane reads consecutive bytes of each of eight rows
 //             and turns them by byte permutes
+// 24 sequences of 2-4 k positions (32/8 heads of 128) take 38.4 us (4.2 TB/s), 256 of 70-320 34 us (3.2 TB/s), two of 65 521
+// with one kv head 20.4 us, one of 256 5.2 us.
 // Work is cut by the device, which alone knows the lengths: the positions of a (sequence, kv head, rows) item go in equal
 // parts to teams of warps, as many as are resident together (dec_part_units).  The parts of an item leave their results in
 // the workspace; of 16 neighbouring parts the team that comes last adds them in order, and of these sums the last again, so
@@ -30,7 +32,6 @@ constexpr int kDecCtasPerSm = 3;                    // resident with 8 rows; 2 w
 __host__ __device__ constexpr int dec_ctas_per_sm(int tiles) { return tiles == 1 ? kDecCtasPerSm : 2; }
 constexpr int kDecMaxRows = 16, kDecMaxDim = 128;
 constexpr int kDecMostRows = 1024;                  // of a sequence and kv head: in groups of 16
-constexpr int kDecWhole = 16;                       // chunks up to which a warp's item is never cut
 constexpr int kDecGroup = 16;                       // parts that are added up together
 constexpr float kDigits = 32512.f;                  // 127 * 256: the high digit stays below 128
 constexpr float kDecLowest = -3e38f;                // a maximum of no scores
@@ -107,26 +108,30 @@ __device__ __forceinline__ void load_v(VRow<kHD>& r, const int8_t* row, int g)
 
 // floor(n / d): 64-bit divisions take long
 __device__ __forceinline__ unsigned long long div_small(unsigned long long n, uint32_t d) { return n >> 32 ? n / d : (uint32_t)n / d; }
-// units of sequence s, in steps of `unit` positions; a sequence without positions has one
-__device__ __forceinline__ uint32_t dec_units(const PagedArgs& C, int s, int unit)
+// f(the units of sequence s: its steps of `unit` positions, at least one) for s from first to end - 1, the lengths of many four at a time: each CTA looks at them all (1000
+// sequences of 320 positions, 2 kv heads of 64, teams of four: 103 -> 52 us)
+template <class F> __device__ __forceinline__ void dec_each(const PagedArgs& C, int first, int end, int unit, F f)
 {
-    const int n = paged_len(C, s);
-    return n <= 0 ? 1u : (uint32_t)(n + unit - 1) / (uint32_t)unit;
+    const int room = (int)min((long long)C.table_pages << C.page_shift, (long long)C.max_len);
+    auto one = [&](int n) { n = min(n, room); f(n <= 0 ? 1u : (uint32_t)(n + unit - 1) / (uint32_t)unit); };
+    if (C.num_seqs <= 32) { if (first < end) one(C.kv_len[first]); return; }      // one to a lane
+    const bool wide = ((reinterpret_cast<uintptr_t>(C.kv_len) | first * 4u) & 15) == 0;
+    int s = first;
+    if (wide)
+#pragma unroll 2
+        for (; s + 4 <= end; s += 4) { const int4 n = *reinterpret_cast<const int4*>(C.kv_len + s); one(n.x); one(n.y); one(n.z); one(n.w); }
+    for (; s < end; s++) one(C.kv_len[s]);
 }
 // The most units of a part: the least that gives all items' parts to resident teams.  With so many items that this would
 // cut nothing or nearly nothing, twice a team's share: only what is far longer than the others is cut (cutting all of 2400
-// items so that they fill two rounds of 1776 teams measured the same).  At least min_units, and a 128th of the longest item:
+// items so that they fill two rounds of teams measured the same).  At least min_units, and a 128th of the longest item:
 // adding up more parts takes longer than they save.  For a whole warp; a lane looks at `per_lane` neighbouring sequences.
 __device__ __forceinline__ uint32_t dec_part_units(const DecodeParams& P, int unit, int per_seq, int per_lane)
 {
     const PagedArgs& C = P.a.c;
     const int first = (threadIdx.x & 31) * per_lane, end = min(first + per_lane, C.num_seqs);
     uint32_t n = 0, top = 0;
-#pragma unroll 4
-    for (int s = first; s < end; s++) {
-        const uint32_t u = dec_units(C, s, unit);
-        n += u; top = max(top, u);
-    }
+    dec_each(C, first, end, unit, [&](uint32_t u) { n += u; top = max(top, u); });
     top = __reduce_max_sync(0xFFFFFFFFu, top);
     const unsigned long long total = (unsigned long long)__reduce_add_sync(0xFFFFFFFFu, n) * (unsigned long long)per_seq;
     const unsigned long long items = (unsigned long long)C.num_seqs * per_seq, share = div_small(total, P.teams) + 1;
@@ -136,8 +141,7 @@ __device__ __forceinline__ uint32_t dec_part_units(const DecodeParams& P, int un
     while (lo < hi) {
         const uint32_t mid = (lo + hi) / 2;
         uint32_t parts = 0;
-#pragma unroll 4
-        for (int s = first; s < end; s++) parts += (dec_units(C, s, unit) + mid - 1) / mid;
+        dec_each(C, first, end, unit, [&](uint32_t u) { parts += (u + mid - 1) / mid; });
         if ((unsigned long long)__reduce_add_sync(0xFFFFFFFFu, parts) * (unsigned long long)per_seq <= (unsigned long long)P.teams) hi = mid; else lo = mid + 1;
     }
     return lo;
@@ -159,7 +163,7 @@ __device__ __forceinline__ void dec_store4(int16_t* o, const float4& n, float rd
     else { o[0] = (int16_t)y.x; o[1] = (int16_t)(y.x >> 16); o[2] = (int16_t)y.y; o[3] = (int16_t)(y.y >> 16); }
 }
 
-// A team is one warp (many items: nothing waits for another warp) or the CTA (few, long items).
+// A team is one warp (many short items: nothing waits for another warp; an item is one team's) or the CTA (long ones, cut).
 template <int kHD, int kTiles, int kTeam>
 __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm(kTiles))
 paged_decode_kernel(const __grid_constant__ DecodeParams P)
@@ -178,26 +182,24 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     const int team = blockIdx.x * (kDecWarps / kTeam) + warp / kTeam, tw = warp % kTeam, tt = threadIdx.x % kTeamThreads;
     const int gqa = P.a.n_head / C.n_head_kv, per_seq = C.n_head_kv * P.row_groups;
-    auto team_sync = [] { if (kTeam > 1) __syncthreads(); else __syncwarp(); };
 
     // ---- this team's part: part `part` of `parts` of item `item` of sequence seq; slot0: the item's first slot
     int seq = -1, parts = 0, slot0 = 0;
     uint32_t units = 0, left = team;
-    if (P.whole) {
+    if (kTeam == 1 || P.whole) {
         if (team < C.num_seqs * per_seq) { seq = team / per_seq; left = team - seq * per_seq; parts = 1; }
     } else {
-        const int per_lane = (C.num_seqs + 31) >> 5;
+        const int per_lane = C.num_seqs > 32 ? (C.num_seqs + 127) >> 7 << 2 : 1;   // fours of lengths
         const uint32_t most = dec_part_units(P, kUnit, per_seq, per_lane);
         // left: teams of the sequences from here on that come before this one
         // the lane whose sequences hold the team, then the sequence: two scans, each of (teams, slots) of a lane's sequences
         for (int s0 = 0, per = per_lane, n_seqs = C.num_seqs; ; ) {
             uint32_t n = 0, cut = 0, u = 0, parts_of = 0;
-#pragma unroll 4
-            for (int s = s0 + lane * per; s < min(s0 + (lane + 1) * per, n_seqs); s++) {
-                u = dec_units(C, s, kUnit);
+            dec_each(C, s0 + lane * per, min(s0 + (lane + 1) * per, n_seqs), kUnit, [&](uint32_t units_of) {
+                u = units_of;
                 parts_of = (u + most - 1) / most;
                 n += parts_of; cut += parts_of > 1 ? parts_of : 0;
-            }
+            });
             unsigned long long mine = (unsigned long long)(n * per_seq) | (unsigned long long)(cut * per_seq) << 32, upto = mine;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
@@ -234,7 +236,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
         paged_rows(C, seq, lo, hi);
         const int rows = min(kRows, (hi - lo) * gqa - row_base);   // rows of this item; 0 or less: none
         if (rows > 0) {
-            const int t_lo = P.whole ? 0 : (int)((unsigned long long)units * part / parts) * kUnit;
+            const int t_lo = kTeam == 1 || P.whole ? 0 : (int)((unsigned long long)units * part / parts) * kUnit;
             // the first chunks' pages are asked for before the lengths are there
             const int kt = (g >> 2) * 16, vt = (t4 >> 1) * 16;
             const int* table = C.table + (size_t)seq * C.table_stride;
@@ -243,7 +245,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
             const int entry[4] = {entry_at(t0 + kt), entry_at(t0 + vt), entry_at(t0 + kUnit + kt), entry_at(t0 + kUnit + vt)};
             const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // row r sees min(before + token, room) positions
             const int least = min(before + token_of(row_base), room), most_seen = min(before + token_of(row_base + rows - 1), room);
-            const int t_hi = P.whole ? most_seen : (int)min((long long)((unsigned long long)units * (part + 1) / parts) * kUnit, (long long)most_seen);
+            const int t_hi = kTeam == 1 || P.whole ? most_seen : (int)min((long long)((unsigned long long)units * (part + 1) / parts) * kUnit, (long long)most_seen);
             bool missing = false;
             // the page of position t, whose table entry was read; -1: none, or t not below t_hi
             auto page_of = [&](int entry, int t) {
@@ -468,7 +470,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                 l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
                 l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
             }
-            const bool alone = parts == 1;
+            const bool alone = kTeam == 1 || parts == 1;
             auto out_at = [&](int r, int d) {
                 const int tok = token_of(row_base + r), head = row_base + r - tok * gqa;
                 return P.a.out + (size_t)(lo + tok) * P.a.out_stride + (size_t)(kvh * gqa + head) * kHD + d;
@@ -481,15 +483,13 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                     if (r >= rows) continue;
                     const float rd = dec_over(l[i]);
                     int16_t* o = out_at(r, 0);
-                    if (!alone && t4 == 0) { mine[kRows * kHD + 2 * r] = m[i]; mine[kRows * kHD + 2 * r + 1] = l[i]; }
 #pragma unroll
                     for (int e = 0; e < 2; e++)
 #pragma unroll
                         for (int j = 0; j < kCols; j += 4) {
                             const float4 n = make_float4(acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]);
                             const int d = (2 * t4 + e) * kCols + j;
-                            if (alone) dec_store4(o + d, n, rd, out_aligned);
-                            else *reinterpret_cast<float4*>(mine + r * kHD + d) = n;
+                            dec_store4(o + d, n, rd, out_aligned);
                         }
                 }
             } else {
@@ -524,22 +524,19 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
                     if (d == 0) { mine[kRows * kHD + 2 * r] = mm; mine[kRows * kHD + 2 * r + 1] = den; }
                 }
             }
-            if (!alone) {
+            if (kTeam > 1 && !alone) {
                 const int ngroups = (parts + kDecGroup - 1) / kDecGroup;
                 // true in the team that is the last of `n` to come
                 auto last_of = [&](unsigned int* counter, int n) {
-                    team_sync();
-                    int last = 0;
+                    __syncthreads();
                     if (tt == 0) {
                         __threadfence();                            // with the barrier before it: all the team's writes
-                        last = atomicAdd(counter, 1u) == (unsigned)n - 1;
-                        if (last) *counter = 0;
-                        if (kTeam > 1) last_s = last;
+                        last_s = atomicAdd(counter, 1u) == (unsigned)n - 1;
+                        if (last_s) *counter = 0;
                     }
-                    team_sync();
-                    last = kTeam > 1 ? last_s : __shfl_sync(0xFFFFFFFFu, last, 0);
+                    __syncthreads();
                     __threadfence();
-                    return last != 0;
+                    return last_s != 0;
                 };
                 // adds n parts, or sums of groups (stats: where their statistics lie): to the output, or over the first one
                 auto add_up = [&](int first, int step, int n, int stats, bool finish) {
@@ -575,9 +572,9 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
 
 // The workspace: partial results, then the counters; the same places for every call on a device.  The parts of cut items
 // are at most 2 * teams: an item of u units has at most 2 u / (units of a part).
-static int64_t dec_teams(int team) { return (int64_t)sm_count() * kDecCtasPerSm * (kDecWarps / team); }
-static int64_t dec_slot_bytes() { return std::max(2 * dec_teams(kDecWarps) * dec_slot_floats(kDecMaxRows), 2 * dec_teams(1) * dec_slot_floats(8)) * 4; }
-static int64_t dec_group_bytes() { return 2 * dec_teams(1) * 4; }
+static int64_t dec_teams() { return (int64_t)sm_count() * kDecCtasPerSm; }   // of four warps, resident together
+static int64_t dec_slot_bytes() { return 2 * dec_teams() * dec_slot_floats(kDecMaxRows) * 4; }
+static int64_t dec_group_bytes() { return 2 * dec_teams() * 4; }
 int64_t paged_decode_workspace_bytes(int n_head, int n_head_kv, int num_seqs, int max_new)
 {
     const long long rows = std::min((long long)(n_head / n_head_kv) * max_new, (long long)kDecMostRows);   // enough for fewer, too
@@ -587,9 +584,9 @@ int64_t paged_decode_workspace_bytes(int n_head, int n_head_kv, int num_seqs, in
 template <int kHD, int kTiles, int kTeam>
 static int decode_launch(DecodeParams P, void* stream, const char* who)
 {
-    P.whole = P.a.c.max_len <= kTeam * kDecChunk * (kTeam == 1 ? kDecWhole : P.min_units);
+    P.whole = kTeam == 1 || P.a.c.max_len <= kTeam * kDecChunk * P.min_units;
     // at most, by the caller's bounds: every item whole, and what cutting adds; a grid for less than all resident teams
-    P.teams = (int)dec_teams(kTeam) * dec_ctas_per_sm(kTiles) / kDecCtasPerSm;
+    P.teams = (int)dec_teams() * dec_ctas_per_sm(kTiles) / kDecCtasPerSm;
     const long long items = (long long)P.a.c.num_seqs * P.a.c.n_head_kv * P.row_groups;
     const long long parts = (P.a.c.max_len + (long long)kTeam * kDecChunk * P.min_units - 1) / ((long long)kTeam * kDecChunk * P.min_units);
     const long long grid = ((P.whole ? items : std::min(items * parts, items + P.teams)) * kTeam + kDecWarps - 1) / kDecWarps;
@@ -603,7 +600,11 @@ static int decode_launch_hd(DecodeParams P, int tiles, void* stream, const char*
     const long long items = (long long)A.c.num_seqs * A.c.n_head_kv * P.row_groups;
     P.min_units = env_knob("S12_PAGED_MIN_UNITS", 2);
     if (tiles == 2) return decode_launch<kHD, 2, kDecWarps>(P, stream, who);
-    if (items >= env_knob("S12_PAGED_ITEMS", 1000)) return decode_launch<kHD, 1, 1>(P, stream, who);
+    // us with one / four warps, sequences of half of these lengths to all: 8 kv heads of 128, 64 sequences of 128 positions
+    // 8.0 / 9.4, 320 15.8 / 15.6, 500 27.6 / 21.8; 256 of 500 57 / 60, 700 81 / 73; 800 of 900 237 / 255; 2 kv heads of 64, 100
+    // sequences of 128 6.2 / 5.4, 256 of 500 13.6 / 17.1, 1000 of 900 59 / 76, 1500 95 / 102
+    const int team = env_knob("S12_PAGED_TEAM", 0);                // 1, 4: whatever the rule says
+    if (team == 1 || (team == 0 && (long long)kHD * A.c.max_len <= std::min(40 * items, 131072ll))) return decode_launch<kHD, 1, 1>(P, stream, who);
     return decode_launch<kHD, 1, kDecWarps>(P, stream, who);
 }
 
