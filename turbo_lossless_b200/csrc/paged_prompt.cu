@@ -43,7 +43,7 @@ constexpr float kPrSlack = 8.f;                     // a maximum may be exceeded
 __host__ __device__ constexpr int pr_tile_bytes(int hd) { return (hd + 63) / 64 * kPrRows * 128; }   // blocks of 64 dims: [128 rows][128 bytes]
 __host__ __device__ constexpr int pr_smem_bytes(int hd) { return 6 * pr_tile_bytes(hd) + 1024; }
 
-struct PrBars { uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], sums_done[2]; };
+struct PrBars { uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], sums_done[2], all_done[2]; };
 
 __device__ __forceinline__ uint32_t pr_elect()
 {
@@ -206,7 +206,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             mbar_init(smem_addr(&bars.k_full[i]), 4); mbar_init(smem_addr(&bars.v_full[i]), 4);
             mbar_init(smem_addr(&bars.k_empty[i]), n_q); mbar_init(smem_addr(&bars.v_empty[i]), n_q);
             for (int b = 0; b < 2; b++) { mbar_init(smem_addr(&bars.s_full[i][b]), 1); mbar_init(smem_addr(&bars.p_full[i][b]), 4); }
-            mbar_init(smem_addr(&bars.sums_done[i]), 1);
+            mbar_init(smem_addr(&bars.sums_done[i]), 1); mbar_init(smem_addr(&bars.all_done[i]), 1);
         }
         mbar_fence_init();
     }
@@ -351,8 +351,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 if (lane == 0) mbar_arrive(bar(bars.p_full[i][b]));
             }
             // ---- the output
-            if (halves > 1) wait(bars.sums_done[i], halves - 2);    // one after the other: a wait tells odd from even only
-            wait(bars.sums_done[i], halves - 1);
+            wait(bars.all_done[i], 0);                               // a wait tells odd from even only: of sums_done's phases two may be ahead
             pr_fence_after();
             const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : unit_s / sum;   // no position at all: zeros
             // A row as one piece: by way of shared memory, where this row tile's q has been read.  Row of 256 bytes, its
@@ -561,6 +560,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                         pr_mma_ts(o_at, p + 8 * s, v + (uint32_t)(s * 16 * 128 >> 4), idesc_o, h > 0 || s > 0);
                     if (b == 1 || h + 1 == halves) pr_commit(bar(bars.v_empty[st]));
                     pr_commit(bar(bars.sums_done[i]));
+                    if (h + 1 == halves) pr_commit(bar(bars.all_done[i]));
                 }
                 __syncwarp();
                 if (more) {                                         // in the weights' place, when they have been read
