@@ -455,3 +455,19 @@ def test_many_sequences_one_of_them_long(kernel, many):
         if off == 0:
             want = PO.attention(c, 0.125)
         check(out, *want)
+
+
+@pytest.mark.parametrize("n_head,n_kv,hd", [(8, 4, 128), (24, 2, 64), (8, 4, 96)])
+def test_many_prompts_of_all_lengths(monkeypatch, n_head, n_kv, hd):
+    """More tiles of rows than the GPU holds at once, so that a CTA takes one after the other: one or two tiles of rows, an odd or
+    an even number of steps, sequences without tokens between them; the same bits every time."""
+    monkeypatch.setenv("S12_PAGED_FORCE", "2")
+    lens = [(i * 37 % 211, (i * i + 3 * i) % 97) for i in range(330)] + [(0, 400), (900, 3), (0, 1)]
+    lens = [(0 if n == 0 else b, n) for b, n in lens]
+    c = PO.Case(lens, n_head, n_kv, hd, 32, seed=91)
+    first, status = run_attention(c, 0.09)
+    assert status == 0
+    check(first, *PO.attention(c, 0.09))
+    for _ in range(20):
+        out, status = run_attention(c, 0.09)
+        assert status == 0 and torch.equal(out, first)

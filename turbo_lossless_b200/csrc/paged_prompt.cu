@@ -2,15 +2,19 @@
 // (tcgen05.mma, scores, weights and sums in tensor memory), head_dim 64 / 96 / 128.
 //
 // Bound: the two products, 4 * head_dim FLOP per (row, position), and as much time of the exponentials: 16 a clock of an SM
-// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1180 us
-// (1000 TFLOP/s; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 245 us.
+// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1172 us
+// (1007 TFLOP/s; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 225 us.
 //
-// A CTA has 256 rows of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
-// products and softmax take turns.  It walks the positions in tiles of 128.
+// An item is 256 rows of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
+// products and softmax take turns, and the positions in tiles of 128.  The grid has a CTA for each; one that runs takes over, one
+// after the other, items of CTAs that have not begun (cluster launch control), so that the next item's keys are converted and
+// its rows of q on their way while this one ends (11 packed prompts 245 -> 226 us, 12 000 tokens 1184 -> 1173).  What is done
+// once an item is rolled up: the 32 rows of q of a warp in one piece of code cost 237 us for the former, in a loop of eights 226.
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row: scores from tensor memory, running maximum and sum,
 //                    weights back to tensor memory as f16 in the place of the scores; the output at the end
 //   warps 8-11       int8 codes from global memory to f16 in swizzled shared memory; the next tile's loads are in flight
 //                    meanwhile
+//   warp 14          looks for the next item
 //   warps 12, 13     issue the MMAs of row tile 0 / 1, one thread each: S = Q K^T (both from shared memory), O += P V (P from
 //                    tensor memory, V with the dims contiguous), 64 positions at a time: the next 64 scores are there
 //                    when the softmax has done with these
@@ -43,7 +47,9 @@ constexpr float kPrSlack = 8.f;                     // a maximum may be exceeded
 __host__ __device__ constexpr int pr_tile_bytes(int hd) { return (hd + 63) / 64 * kPrRows * 128; }   // blocks of 64 dims: [128 rows][128 bytes]
 __host__ __device__ constexpr int pr_smem_bytes(int hd) { return 6 * pr_tile_bytes(hd) + 1024; }
 
-struct PrBars { uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], sums_done[2], all_done[2]; };
+constexpr int kPrItems = 4;                         // places for items
+struct PrItem { int seq, lo, row0, rows, kvh, before, room, seen; };   // seq -1: no more
+struct PrBars { uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], sums_done[2], all_done[2], item_full[kPrItems], item_empty[kPrItems], more, next; };
 
 __device__ __forceinline__ uint32_t pr_elect()
 {
@@ -131,6 +137,20 @@ __device__ __forceinline__ void pr_codes_f16(uint32_t w, uint32_t& lo, uint32_t&
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
 }
+// asks for the work of a CTA that has not begun; the answer's 16 bytes arrive at `at`, counted on `bar`
+__device__ __forceinline__ void pr_take_cta(uint32_t at, uint32_t bar)
+{
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(at), "r"(bar) : "memory");
+}
+// that CTA's number, or -1: none is left, and no further question is allowed
+__device__ __forceinline__ int pr_taken_cta(uint32_t at)
+{
+    int cta;
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b128 x;\n\tld.shared.b128 x, [%1];\n\tmov.b32 %0, -1;\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, x;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, x;\n\t}" : "=r"(cta) : "r"(at) : "memory");
+    return cta;
+}
 // two at a time
 typedef float2 Pair;
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) { return __fmul2_rn(a, b); }
@@ -160,7 +180,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     __shared__ PrBars bars;
     __shared__ __align__(8) float2 unit_s2[kPrScaleStages];        // of a tile: the power of two of its keys, 2^(E before - E) of its values
     __shared__ uint2 top_s[2][4];                                  // the converters' largest scales of a tile
-    __shared__ float unit_s;                                       // 2^E at the end
+    __shared__ float unit_s[2 * kPrItems];                         // of an item: 2^E at the end; four items may be read ahead of one
+    __shared__ __align__(16) PrItem item_s[kPrItems];
+    __shared__ __align__(16) uint4 taken_s;
     __shared__ __align__(4) uint8_t absent_s[kPrScaleStages][4];   // byte i, bit h: the 16 positions from 32 i + 16 h on have no page
     __shared__ float factor_s[kPrCtaRows];
     __shared__ uint32_t tmem_s;
@@ -174,37 +196,14 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     grid_launch_dependents();
     grid_dependency_wait();
 
-    // ---- this CTA's rows: tiles of all sequences counted from the last, a kv head after the other
-    const int kvh = blockIdx.x % C.n_head_kv;
-    int seq = -1, lo = 0, hi = 0, tile = (int)(blockIdx.x / C.n_head_kv);
-    for (int s1 = C.num_seqs; s1 > 0 && seq < 0; s1 -= 32) {       // sequence s1 - 1 - lane
-        const int s = s1 - 1 - lane;
-        int a = 0, b = 0, n = 0;
-        if (s >= 0) { paged_rows(C, s, a, b); n = b > a ? (int)(((long long)(b - a) * gqa + kPrCtaRows - 1) / kPrCtaRows) : 0; }
-        int upto = n;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xFFFFFFFFu, upto, off); if (lane >= off) upto += o; }
-        const unsigned over = __ballot_sync(0xFFFFFFFFu, upto > tile);
-        if (over) {
-            const int l = __ffs(over) - 1;
-            seq = s1 - 1 - l; lo = __shfl_sync(0xFFFFFFFFu, a, l); hi = __shfl_sync(0xFFFFFFFFu, b, l);
-            tile = __shfl_sync(0xFFFFFFFFu, upto, l) - 1 - tile;   // the sequence's last tile, which sees most, comes first
-        } else {
-            tile -= __shfl_sync(0xFFFFFFFFu, upto, 31);
-        }
-    }
-    if (seq < 0) return;                                           // more CTAs than tiles
-    const int row0 = tile * kPrCtaRows, rows = min(kPrCtaRows, (hi - lo) * gqa - row0);
-    const int n_q = rows > kPrRows ? 2 : 1;                        // row tiles
-    const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // token t sees min(before + t, room) positions
-    const int seen = max(0, min(before + token_of(row0 + rows - 1), room)), halves = max(1, (seen + kPrHalf - 1) / kPrHalf), n = (halves + 1) / 2;
-
     if (threadIdx.x == 0) {
         s_abort = 0;
-        mbar_init(smem_addr(&bars.q_full), 8);
+        for (int i = 0; i < kPrItems; i++) { mbar_init(smem_addr(&bars.item_full[i]), 1); mbar_init(smem_addr(&bars.item_empty[i]), 14); }
+        mbar_init(smem_addr(&bars.more), 1); mbar_init(smem_addr(&bars.next), 1);
         for (int i = 0; i < 2; i++) {
+            mbar_init(smem_addr(&bars.q_full[i]), 4);
             mbar_init(smem_addr(&bars.k_full[i]), 4); mbar_init(smem_addr(&bars.v_full[i]), 4);
-            mbar_init(smem_addr(&bars.k_empty[i]), n_q); mbar_init(smem_addr(&bars.v_empty[i]), n_q);
+            mbar_init(smem_addr(&bars.k_empty[i]), 2); mbar_init(smem_addr(&bars.v_empty[i]), 2);
             for (int b = 0; b < 2; b++) { mbar_init(smem_addr(&bars.s_full[i][b]), 1); mbar_init(smem_addr(&bars.p_full[i][b]), 4); }
             mbar_init(smem_addr(&bars.sums_done[i]), 1); mbar_init(smem_addr(&bars.all_done[i]), 1);
         }
@@ -221,71 +220,98 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     auto bar = [](const uint64_t& b) { return smem_addr(&b); };
     auto wait = [&](const uint64_t& b, int phase) { mbar_wait(smem_addr(&b), (uint32_t)phase & 1, C.status, kPrSite, &s_abort); };
 
+    // the k-th item of this CTA, for a whole warp
+    auto item_at = [&](int k) {
+        wait(bars.item_full[k % kPrItems], k / kPrItems);
+        const PrItem w = item_s[k % kPrItems];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(bars.item_empty[k % kPrItems]));
+        if (*(volatile int*)&s_abort) return PrItem{-1};
+        return w;
+    };
+    auto halves_of = [](const PrItem& w) { return max(1, (w.seen + kPrHalf - 1) / kPrHalf); };
+
     if (warp < 8) {
         // ------------------------------ softmax -------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-        // ---- q as f16: warp w takes rows w, w + 8, ..., all of them in flight together, a lane four dims of each; the
-        // converters have begun meanwhile
-        {
-            const float to_log2 = fabsf(P.a.scale) * 1.4426950408889634f;
-            const float* q0 = P.a.q + (size_t)lo * P.a.q_stride + (size_t)kvh * gqa * kHD + 4 * lane;
-            const bool in_row = 4 * lane < kHD;
-            uint8_t* to = q_s + pr_chunk(warp, lane >> 1) + (lane & 1) * 8;
-            auto row_of = [&](int r) {
-                const int t = token_of(row0 + r);
-                return q0 + (size_t)t * P.a.q_stride + (row0 + r - t * gqa) * kHD;
-            };
-            auto put = [&](int i, const float4& v) {                // row warp + 8 i
-                const uint32_t a = __float_as_uint(v.x) & 0x7FFFFFFFu, b = __float_as_uint(v.y) & 0x7FFFFFFFu;
-                const uint32_t c = __float_as_uint(v.z) & 0x7FFFFFFFu, d = __float_as_uint(v.w) & 0x7FFFFFFFu;
-                // 2^e of the largest, e >= -100, or nothing: rows of smaller ones count as zero, and a NaN or an infinity, the
-                // largest of all, becomes a NaN
-                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d))) & 0x7F800000u;
-                const bool fine = top - (27u << 23) < (228u << 23);
-                const float up = fine ? __uint_as_float((268u << 23) - top ^ (P.a.scale < 0.f ? 0x80000000u : 0u)) : 0.f;   // 2^(14 - e)
-                if (in_row) *reinterpret_cast<uint2*>(to + i / 16 * kTileBytes + i % 16 * 1024) = make_uint2(pr_f16x2(v.x * up, v.y * up), pr_f16x2(v.z * up, v.w * up));
-                if (lane == 0) factor_s[warp + 8 * i] = fine ? to_log2 * __uint_as_float(top - (14u << 23)) : 0.f;
-            };
-            if (((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0) {
-                float4 v[32];
+        const int i = warp >> 2, r = warp * 32 + lane;               // row tile, row of the CTA
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t s_at = mine + i * 2 * kPrHalf, o_at = mine + 4 * kPrHalf + i * 128;
+        uint8_t* const tile_q = q_s + i * kTileBytes;                // the warp's 32 rows in it are its own: q, then the output
+        int g = 0, c0 = 0, c1 = 0, cs = 0, done = 0;                 // tiles; halves of this row tile in either buffer, all, and items, so far
+        for (int item = 0; ; item++) {
+            const PrItem w = item_at(item);
+            if (w.seq < 0) break;
+            const int halves = halves_of(w), rows = w.rows, row0 = w.row0, g0 = g;
+            g += (halves + 1) / 2;
+            if (i > 0 && rows <= kPrRows) continue;
+            // ---- the warp's rows of q as f16, all of them in flight together, a lane four dims of each
+            {
+                const float to_log2 = fabsf(P.a.scale) * 1.4426950408889634f;
+                const float* q0 = P.a.q + (size_t)w.lo * P.a.q_stride + (size_t)w.kvh * gqa * kHD + 4 * lane;
+                const bool in_row = 4 * lane < kHD;
+                auto row_of = [&](int r) {
+                    const int t = token_of(row0 + r);
+                    return q0 + (size_t)t * P.a.q_stride + (row0 + r - t * gqa) * kHD;
+                };
+                auto top_of = [&](const float4& v) {
+                    const uint32_t a = __float_as_uint(v.x) & 0x7FFFFFFFu, b = __float_as_uint(v.y) & 0x7FFFFFFFu;
+                    const uint32_t c = __float_as_uint(v.z) & 0x7FFFFFFFu, d = __float_as_uint(v.w) & 0x7FFFFFFFu;
+                    return __reduce_max_sync(0xFFFFFFFFu, max(max(a, b), max(c, d))) & 0x7F800000u;
+                };
+                auto put = [&](int n, const float4& v, uint32_t top) {   // row 32 warp + n
+                    // 2^e of the largest, e >= -100, or nothing: rows of smaller ones count as zero, and a NaN or an infinity, the
+                    // largest of all, becomes a NaN
+                    const bool fine = top - (27u << 23) < (228u << 23);
+                    const float up = fine ? __uint_as_float((268u << 23) - top ^ (P.a.scale < 0.f ? 0x80000000u : 0u)) : 0.f;   // 2^(14 - e)
+                    if (in_row) *reinterpret_cast<uint2*>(tile_q + pr_chunk((warp & 3) * 32 + n, lane >> 1) + (lane & 1) * 8) = make_uint2(pr_f16x2(v.x * up, v.y * up), pr_f16x2(v.z * up, v.w * up));
+                    if (lane == 0) factor_s[warp * 32 + n] = fine ? to_log2 * __uint_as_float(top - (14u << 23)) : 0.f;
+                };
+                if (((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0) {
+                    float4 v[8], next[8];
+                    auto fetch = [&](float4 (&to)[8], int n) {
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (warp + 8 * i < rows && in_row) v[i] = *reinterpret_cast<const float4*>(row_of(warp + 8 * i));
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i++) put(i, v[i]);
-                if (n_q > 1)
-#pragma unroll
-                    for (int i = 16; i < 32; i++) put(i, v[i]);
-            } else {
+                        for (int e = 0; e < 8; e++) {
+                            to[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (warp * 32 + n + e < rows && in_row) to[e] = *reinterpret_cast<const float4*>(row_of(warp * 32 + n + e));
+                        }
+                    };
+                    fetch(v, 0);
+                    fetch(next, 8);
 #pragma unroll 1
-                for (int i = 0; i < 16 * n_q; i++) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (warp + 8 * i < rows && in_row) { const float* q = row_of(warp + 8 * i); v = make_float4(q[0], q[1], q[2], q[3]); }
-                    put(i, v);
+                    for (int n = 0; n < 32; n += 8) {                // no store is moved before a reduction: eight of them together
+                        uint32_t top[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) top[e] = top_of(v[e]);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) put(n + e, v[e], top[e]);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[e] = next[e];
+                        if (n < 16) fetch(next, n + 16);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int n = 0; n < 32; n++) {
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (warp * 32 + n < rows && in_row) { const float* q = row_of(warp * 32 + n); v = make_float4(q[0], q[1], q[2], q[3]); }
+                        put(n, v, top_of(v));
+                    }
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what ordinary stores wrote
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(bars.q_full[i]));
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMAs read what ordinary stores wrote
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(bars.q_full));
-            wait(bars.q_full, 0);                                   // the rows' factors come from all warps
-        }
-        const int i = warp >> 2, r = i * kPrRows + (warp & 3) * 32 + lane;   // row tile, row of the CTA
-        if (i < n_q) {
-            const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            const uint32_t s_at = mine + i * 2 * kPrHalf, o_at = mine + 4 * kPrHalf + i * 128;
             const int tok = token_of(row0 + r);
-            const int limit = r < rows ? min(before + tok, room) : 0;       // positions that this row sees
+            const int limit = r < rows ? min(w.before + tok, w.room) : 0;   // positions that this row sees
             const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
             const float factor = factor_s[r];
             float m = kPrLowest;
             Pair l = {0.f, 0.f};
 #pragma unroll 1
             for (int h = 0; h < halves; h++) {
-                const int j = (h >> 1) % kPrScaleStages, b = h & 1;
+                const int j = (g0 + (h >> 1)) % kPrScaleStages, b = h & 1;
                 float x[2][32];
-                wait(bars.s_full[i][b], h >> 1);                    // then half h - 2 is in the sums
+                wait(bars.s_full[i][b], (b ? c1 : c0) + (h >> 1));                    // then half h - 2 is in the sums
                 pr_fence_after();
                 pr_ld32(s_at + b * kPrHalf, x[0]);
                 pr_ld32(s_at + b * kPrHalf + 32, x[1]);
@@ -315,7 +341,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                     m = mn;
                     l = mul2(l, {f, f});
                     if (h > 0) {
-                        wait(bars.sums_done[i], h - 1);                 // the half before it, too
+                        wait(bars.sums_done[i], cs + h - 1);                 // the half before it, too
                         pr_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < kHD; c += 32) {
@@ -351,14 +377,12 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 if (lane == 0) mbar_arrive(bar(bars.p_full[i][b]));
             }
             // ---- the output
-            wait(bars.all_done[i], 0);                               // a wait tells odd from even only: of sums_done's phases two may be ahead
+            wait(bars.all_done[i], done++);                          // a wait tells odd from even only: of sums_done's phases two may be ahead
             pr_fence_after();
-            const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : unit_s / sum;   // no position at all: zeros
-            // A row as one piece: by way of shared memory, where this row tile's q has been read.  Row of 256 bytes, its
-            // 16-byte chunks permuted so that the lanes of a store and of a load meet different banks.
-            uint8_t* stage = q_s + i * kTileBytes + (warp & 3) * (kTileBytes / 4);
-            constexpr int kRowBytes = kHD == 64 ? 128 : 256, kChunks = kHD / 8;
-            auto chunk_at = [&](int row, int c) { return stage + row * kRowBytes + ((c ^ (row & 7)) << 4); };
+            const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : unit_s[item % (2 * kPrItems)] / sum;   // no position at all: zeros
+            // A row as one piece: by way of shared memory, in the place of the warp's rows of q, which have been read
+            constexpr int kChunks = kHD / 8;
+            auto chunk_at = [&](int row, int c) { return tile_q + pr_chunk((warp & 3) * 32 + row, c); };
 #pragma unroll 1
             for (int c = 0; c < kHD; c += 32) {
                 float o[32];
@@ -373,14 +397,14 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             }
             __syncwarp();
             const bool aligned = ((reinterpret_cast<uintptr_t>(P.a.out) & 15) | (P.a.out_stride & 7)) == 0;
-            const int first = i * kPrRows + (warp & 3) * 32;       // this warp's rows
-            int16_t* out0 = P.a.out + (size_t)lo * P.a.out_stride + (size_t)kvh * gqa * kHD;
-#pragma unroll 4
-            for (int x = lane; x < 32 * kChunks; x += 32) {
-                const int row = x / kChunks, c = x - row * kChunks, t = token_of(row0 + first + row), hd = row0 + first + row - t * gqa;
-                if (first + row >= rows) break;
+            const int first = warp * 32;                            // this warp's rows
+            int16_t* out0 = P.a.out + (size_t)w.lo * P.a.out_stride + (size_t)w.kvh * gqa * kHD;
+#pragma unroll 2
+            for (int it = 0; it < kChunks; it++) {
+                const int x = it * 32 + lane, row = x / kChunks, c = x - row * kChunks, t = token_of(row0 + first + row), hd = row0 + first + row - t * gqa;
                 const uint4 y = *reinterpret_cast<const uint4*>(chunk_at(row, c));
                 int16_t* out = out0 + (size_t)t * P.a.out_stride + hd * kHD + c * 8;
+                if (first + row >= rows) continue;
                 if (aligned) {
                     *reinterpret_cast<uint4*>(out) = y;
                 } else {
@@ -389,6 +413,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                     for (int e = 0; e < 8; e++) out[e] = (int16_t)(w[e >> 1] >> (16 * (e & 1)));
                 }
             }
+            __syncwarp();                                           // the next item's q goes where the rows were
+            c0 += (halves + 1) / 2; c1 += halves / 2; cs += halves;
         }
     } else if (warp < 12) {
         // ------------------------------ codes to operands ---------------------
@@ -399,177 +425,265 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
         constexpr int kRowsAt = kHD == 64 ? 8 : 4, kIts = 32 / kRowsAt;
         const int row_of = kHD == 64 ? lane >> 2 : (lane >> 4) << 1 | (lane >> 2 & 1), piece = kHD == 64 ? lane & 3 : (lane >> 3 & 1) * 4 + (lane & 3);
         const bool live = piece < kPieces;
-        const int* table = C.table + (size_t)seq * C.table_stride;
         const int ps = 1 << C.page_shift, mine = cw * 32 + lane;
         bool missing = false;
-        // the pools' row of position p, and whether there is one; -1 where the table has no page or no row sees p
-        auto row_at = [&](int p) {
-            if (p >= seen) return -1ll;
-            const int page = table[p >> C.page_shift];
-            if ((unsigned)page >= (unsigned)C.num_pages) { missing = true; return -1ll; }
-            return (long long)((((uint32_t)page * C.n_head_kv + kvh) << C.page_shift) + (p & (ps - 1)));
-        };
-        const int8_t* k_at = C.k + row_of * kHD + 16 * piece, *v_at = C.v + row_of * kHD + 16 * piece;
-        uint4 k[kIts], v[kIts];
-        float sk = 0.f, sv = 0.f;
-        // 16 rows lie together; absent ones read row 0 and are masked later
-        auto fetch = [&](uint4 (&to)[kIts], const int8_t* at, long long row) {
-            const uint32_t r = (uint32_t)max(row, 0ll);
-            const int8_t* half[2] = {at + (size_t)__shfl_sync(0xFFFFFFFFu, r, 0) * kHD, at + (size_t)__shfl_sync(0xFFFFFFFFu, r, 16) * kHD};
+        int g = 0;                                                  // tiles so far
+        for (int item = 0; ; item++) {
+            const PrItem w = item_at(item);
+            if (w.seq < 0) break;
+            const int halves = halves_of(w), n = (halves + 1) / 2, seen = w.seen, kvh = w.kvh;
+            const int* table = C.table + (size_t)w.seq * C.table_stride;
+            // the pools' row of position p, and whether there is one; -1 where the table has no page or no row sees p
+            auto row_at = [&](int p) {
+                if (p >= seen) return -1ll;
+                const int page = table[p >> C.page_shift];
+                if ((unsigned)page >= (unsigned)C.num_pages) { missing = true; return -1ll; }
+                return (long long)((((uint32_t)page * C.n_head_kv + kvh) << C.page_shift) + (p & (ps - 1)));
+            };
+            const int8_t* k_at = C.k + row_of * kHD + 16 * piece, *v_at = C.v + row_of * kHD + 16 * piece;
+            uint4 k[kIts], v[kIts];
+            float sk = 0.f, sv = 0.f;
+            // 16 rows lie together; absent ones read row 0 and are masked later
+            auto fetch = [&](uint4 (&to)[kIts], const int8_t* at, long long row) {
+                const uint32_t r = (uint32_t)max(row, 0ll);
+                const int8_t* half[2] = {at + (size_t)__shfl_sync(0xFFFFFFFFu, r, 0) * kHD, at + (size_t)__shfl_sync(0xFFFFFFFFu, r, 16) * kHD};
 #pragma unroll
-            for (int it = 0; it < kIts; it++)
-                if (live) to[it] = *reinterpret_cast<const uint4*>(half[it / (kIts / 2)] + it % (kIts / 2) * kRowsAt * kHD);
-        };
-        auto fetch_scales = [&](long long row) { sk = row >= 0 ? C.sk[row] : 0.f; sv = row >= 0 ? C.sv[row] : 0.f; };
-        // Where a lane's chunks go: row + 4 changes bit 2 of the chunk
-        const uint32_t to0 = pr_chunk(cw * 32 + row_of, 2 * piece);
-        auto store = [&](uint8_t* tile, int it, const uint32_t (&y)[8]) {
-            const uint32_t to = (kRowsAt == 4 && (it & 1) ? to0 ^ 64u : to0) + it * kRowsAt * 128;
-            *reinterpret_cast<uint4*>(tile + to) = make_uint4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint4*>(tile + (to ^ 16u)) = make_uint4(y[4], y[5], y[6], y[7]);
-        };
-        long long row = row_at(mine), row_next = n > 1 ? row_at(kPrTile + mine) : -1;
-        fetch_scales(row);
-        fetch(k, k_at, row);
-        fetch(v, v_at, row);
-        int E = 0;
-        for (int j = 0; j < n; j++) {
-            const int st = j & 1;
-            const bool absent = row < 0;
-            // the values' unit 2^E
-            const uint32_t bits_k = __float_as_uint(sk) & 0x7FFFFFFFu, bits = __float_as_uint(sv) & 0x7FFFFFFFu;
-            const bool fine = bits < 0x7F800000u;
-            const uint32_t top_k = __reduce_max_sync(0xFFFFFFFFu, bits_k < 0x7F800000u ? bits_k : 0u), top_v = __reduce_max_sync(0xFFFFFFFFu, fine ? bits : 0u);
-            if (lane == 0) top_s[st][cw] = make_uint2(top_k, top_v);
-            named_bar_sync(1, 128);
-            const uint2 w0 = top_s[st][0], w1 = top_s[st][1], w2 = top_s[st][2], w3 = top_s[st][3];
-            const int e_top = (int)(max(max(w0.y, w1.y), max(w2.y, w3.y)) >> 23) - 126;   // scales are below 2^e_top
-            const int e_key = min(max((int)(max(max(w0.x, w1.x), max(w2.x, w3.x)) >> 23) - 126 - 8, -100), 100);   // keys below 2^15
-            float shift = 1.f;
-            if (j == 0 || e_top > E + 8) {
-                const int old = E;
-                E = max(e_top - 2, -120);
-                if (j > 0) shift = old - E < -126 ? 0.f : __uint_as_float((uint32_t)(127 + old - E) << 23);
-            }
-            const float unit = __uint_as_float((uint32_t)(127 - E) << 23);   // 2^-E
-            const float key_scale = (fine ? sk : __uint_as_float(0x7FC00000u)) * __uint_as_float((uint32_t)(127 - e_key) << 23);
-            const uint32_t key_hi = pr_f16x2(key_scale, 0.f) & 0xFFFFu;       // the scale as a sum of two f16
-            float key_hi_f;
-            asm("{\n\t.reg .b16 h, z;\n\tmov.b32 {h, z}, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(key_hi_f) : "r"(key_hi));
-            const uint32_t key_parts = key_hi | pr_f16x2(0.f, key_scale - key_hi_f);
-            // ---- K
-            if (j >= 2) wait(bars.k_empty[st], (j >> 1) - 1);
-            const uint32_t gone = __ballot_sync(0xFFFFFFFFu, absent);   // a whole half, or rows that nobody sees
-            if (lane == 0) absent_s[j % kPrScaleStages][cw] = (uint8_t)((gone & 1u) | (gone >> 16 & 1u) << 1);
-            if (mine == 0) {
-                unit_s2[j % kPrScaleStages] = make_float2(__uint_as_float((uint32_t)(127 + e_key) << 23), shift);
-                if (j == n - 1) unit_s = __uint_as_float((uint32_t)(127 + E) << 23);
-            }
+                for (int it = 0; it < kIts; it++)
+                    if (live) to[it] = *reinterpret_cast<const uint4*>(half[it / (kIts / 2)] + it % (kIts / 2) * kRowsAt * kHD);
+            };
+            auto fetch_scales = [&](long long row) { sk = row >= 0 ? C.sk[row] : 0.f; sv = row >= 0 ? C.sv[row] : 0.f; };
+            // Where a lane's chunks go: row + 4 changes bit 2 of the chunk
+            const uint32_t to0 = pr_chunk(cw * 32 + row_of, 2 * piece);
+            auto store = [&](uint8_t* tile, int it, const uint32_t (&y)[8]) {
+                const uint32_t to = (kRowsAt == 4 && (it & 1) ? to0 ^ 64u : to0) + it * kRowsAt * 128;
+                *reinterpret_cast<uint4*>(tile + to) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(tile + (to ^ 16u)) = make_uint4(y[4], y[5], y[6], y[7]);
+            };
+            long long row = row_at(mine), row_next = n > 1 ? row_at(kPrTile + mine) : -1;
+            fetch_scales(row);
+            fetch(k, k_at, row);
+            fetch(v, v_at, row);
+            int E = 0;
+            for (int j = 0; j < n; j++, g++) {
+                const int st = g & 1;
+                if (j == max(n - 2, 0) && mine == 0) mbar_arrive(bar(bars.more));   // the item after this one may be looked for
+                const bool absent = row < 0;
+                // the values' unit 2^E
+                const uint32_t bits_k = __float_as_uint(sk) & 0x7FFFFFFFu, bits = __float_as_uint(sv) & 0x7FFFFFFFu;
+                const bool fine = bits < 0x7F800000u;
+                const uint32_t top_k = __reduce_max_sync(0xFFFFFFFFu, bits_k < 0x7F800000u ? bits_k : 0u), top_v = __reduce_max_sync(0xFFFFFFFFu, fine ? bits : 0u);
+                if (lane == 0) top_s[st][cw] = make_uint2(top_k, top_v);
+                named_bar_sync(1, 128);
+                const uint2 w0 = top_s[st][0], w1 = top_s[st][1], w2 = top_s[st][2], w3 = top_s[st][3];
+                const int e_top = (int)(max(max(w0.y, w1.y), max(w2.y, w3.y)) >> 23) - 126;   // scales are below 2^e_top
+                const int e_key = min(max((int)(max(max(w0.x, w1.x), max(w2.x, w3.x)) >> 23) - 126 - 8, -100), 100);   // keys below 2^15
+                float shift = 1.f;
+                if (j == 0 || e_top > E + 8) {
+                    const int old = E;
+                    E = max(e_top - 2, -120);
+                    if (j > 0) shift = old - E < -126 ? 0.f : __uint_as_float((uint32_t)(127 + old - E) << 23);
+                }
+                const float unit = __uint_as_float((uint32_t)(127 - E) << 23);   // 2^-E
+                const float key_scale = (fine ? sk : __uint_as_float(0x7FC00000u)) * __uint_as_float((uint32_t)(127 - e_key) << 23);
+                const uint32_t key_hi = pr_f16x2(key_scale, 0.f) & 0xFFFFu;       // the scale as a sum of two f16
+                float key_hi_f;
+                asm("{\n\t.reg .b16 h, z;\n\tmov.b32 {h, z}, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(key_hi_f) : "r"(key_hi));
+                const uint32_t key_parts = key_hi | pr_f16x2(0.f, key_scale - key_hi_f);
+                // ---- K
+                if (g >= 2) wait(bars.k_empty[st], (g >> 1) - 1);
+                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, absent);   // a whole half, or rows that nobody sees
+                if (lane == 0) absent_s[g % kPrScaleStages][cw] = (uint8_t)((gone & 1u) | (gone >> 16 & 1u) << 1);
+                if (mine == 0) {
+                    unit_s2[g % kPrScaleStages] = make_float2(__uint_as_float((uint32_t)(127 + e_key) << 23), shift);
+                    if (j == n - 1) unit_s[item % (2 * kPrItems)] = __uint_as_float((uint32_t)(127 + E) << 23);
+                }
 #pragma unroll
-            for (int it = 0; it < kIts; it++) {
-                const uint32_t parts = __shfl_sync(0xFFFFFFFFu, key_parts, it * kRowsAt + row_of), f_hi = prmt(parts, parts, 0x1010u), f_lo = prmt(parts, parts, 0x3232u);
-                if (!live) continue;
-                const uint32_t w[4] = {k[it].x, k[it].y, k[it].z, k[it].w};
-                uint32_t y[8];
+                for (int it = 0; it < kIts; it++) {
+                    const uint32_t parts = __shfl_sync(0xFFFFFFFFu, key_parts, it * kRowsAt + row_of), f_hi = prmt(parts, parts, 0x1010u), f_lo = prmt(parts, parts, 0x3232u);
+                    if (!live) continue;
+                    const uint32_t w[4] = {k[it].x, k[it].y, k[it].z, k[it].w};
+                    uint32_t y[8];
 #pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    pr_codes_f16(w[d], y[2 * d], y[2 * d + 1]);
+                    for (int d = 0; d < 4; d++) {
+                        pr_codes_f16(w[d], y[2 * d], y[2 * d + 1]);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t low;
-                        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(low) : "r"(y[2 * d + h]), "r"(f_lo));
-                        asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(y[2 * d + h]) : "r"(f_hi), "r"(low));
+                        for (int h = 0; h < 2; h++) {
+                            uint32_t low;
+                            asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(low) : "r"(y[2 * d + h]), "r"(f_lo));
+                            asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(y[2 * d + h]) : "r"(f_hi), "r"(low));
+                        }
                     }
+                    store(k_s + st * kTileBytes, it, y);
                 }
-                store(k_s + st * kTileBytes, it, y);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(bars.k_full[st]));
-            const float scale = fine ? sv * unit : 0.f;
-            const uint32_t scale2 = pr_f16x2(scale, scale);
-            const long long row_next2 = j + 2 < n ? row_at((j + 2) * kPrTile + mine) : -1;
-            if (j + 1 < n) { fetch_scales(row_next); fetch(k, k_at, row_next); }
-            // ---- V
-            if (j >= 2) wait(bars.v_empty[st], (j >> 1) - 1);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(bars.k_full[st]));
+                const float scale = fine ? sv * unit : 0.f;
+                const uint32_t scale2 = pr_f16x2(scale, scale);
+                const long long row_next2 = j + 2 < n ? row_at((j + 2) * kPrTile + mine) : -1;
+                if (j + 1 < n) { fetch_scales(row_next); fetch(k, k_at, row_next); }
+                // ---- V
+                if (g >= 2) wait(bars.v_empty[st], (g >> 1) - 1);
 #pragma unroll
-            for (int it = 0; it < kIts; it++) {
-                const uint32_t f2 = __shfl_sync(0xFFFFFFFFu, scale2, it * kRowsAt + row_of);
-                if (!live) continue;
-                const uint32_t w[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
-                uint32_t y[8];
+                for (int it = 0; it < kIts; it++) {
+                    const uint32_t f2 = __shfl_sync(0xFFFFFFFFu, scale2, it * kRowsAt + row_of);
+                    if (!live) continue;
+                    const uint32_t w[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
+                    uint32_t y[8];
 #pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    pr_codes_f16(w[d], y[2 * d], y[2 * d + 1]);
-                    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(y[2 * d]) : "r"(f2));
-                    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(y[2 * d + 1]) : "r"(f2));
+                    for (int d = 0; d < 4; d++) {
+                        pr_codes_f16(w[d], y[2 * d], y[2 * d + 1]);
+                        asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(y[2 * d]) : "r"(f2));
+                        asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(y[2 * d + 1]) : "r"(f2));
+                    }
+                    store(v_s + st * kTileBytes, it, y);
                 }
-                store(v_s + st * kTileBytes, it, y);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(bars.v_full[st]));
+                if (j + 1 < n) fetch(v, v_at, row_next);
+                row = row_next; row_next = row_next2;
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(bars.v_full[st]));
-            if (j + 1 < n) fetch(v, v_at, row_next);
-            row = row_next; row_next = row_next2;
         }
         if (missing) atomicOr(C.status, kStatusPage);
     } else {
         // ------------------------------ MMAs ----------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp - 12 < n_q) {                                     // a warp per row tile
+        // the rows of CTA number cta: tiles of all sequences counted from the last, a kv head after the other
+        auto find = [&](int cta) {
+            const int kvh = cta % C.n_head_kv;
+            int seq = -1, lo = 0, hi = 0, tile = cta / C.n_head_kv;
+            for (int s1 = C.num_seqs; s1 > 0 && seq < 0; s1 -= 32) {   // sequence s1 - 1 - lane
+                const int s = s1 - 1 - lane;
+                int a = 0, b = 0, n = 0;
+                if (s >= 0) { paged_rows(C, s, a, b); n = b > a ? (int)(((long long)(b - a) * gqa + kPrCtaRows - 1) / kPrCtaRows) : 0; }
+                int upto = n;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xFFFFFFFFu, upto, off); if (lane >= off) upto += o; }
+                const unsigned over = __ballot_sync(0xFFFFFFFFu, upto > tile);
+                if (over) {
+                    const int l = __ffs(over) - 1;
+                    seq = s1 - 1 - l; lo = __shfl_sync(0xFFFFFFFFu, a, l); hi = __shfl_sync(0xFFFFFFFFu, b, l);
+                    tile = __shfl_sync(0xFFFFFFFFu, upto, l) - 1 - tile;   // the sequence's last tile, which sees most, comes first
+                } else {
+                    tile -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+                }
+            }
+            PrItem w = {-1};
+            if (seq >= 0) {
+                const int row0 = tile * kPrCtaRows, rows = min(kPrCtaRows, (hi - lo) * gqa - row0);
+                const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // token t sees min(before + t, room) positions
+                w = {seq, lo, row0, rows, kvh, before, room, max(0, min(before + token_of(row0 + rows - 1), room))};
+            }
+            return w;
+        };
+        // the number of a CTA that has not begun, which then never does; -1: none
+        int asked = 0;
+        auto take = [&] {
+            if (lane == 0) { mbar_arrive_expect_tx(bar(bars.next), 16); pr_take_cta(smem_addr(&taken_s), bar(bars.next)); }
+            __syncwarp();
+            wait(bars.next, asked++);
+            const int cta = *(volatile int*)&s_abort ? -1 : pr_taken_cta(smem_addr(&taken_s));
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // read before the next answer comes
+            __syncwarp();
+            return cta;
+        };
+        // an item's rows of q on their way to L2 while the one before it is worked on
+        auto ask = [&](const PrItem& w) {
+            if (((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) != 0) return;
+            const int first = token_of(w.row0), last = token_of(w.row0 + w.rows - 1);
+            for (int t = first + lane; t <= last; t += 32)
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(P.a.q + (size_t)(w.lo + t) * P.a.q_stride + (size_t)w.kvh * gqa * kHD), "r"(gqa * kHD * 4) : "memory");
+        };
+        if (warp < 14) {                                           // a warp per row tile
             const int i = warp - 12;
             const uint32_t idesc_s = 1u << 4 | (uint32_t)(kPrHalf >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;                        // f16 x f16
             const uint32_t idesc_o = 1u << 4 | 1u << 16 | (uint32_t)(kHD >> 3) << 17 | (uint32_t)(kPrRows >> 4) << 24;   // the same, B with N contiguous
             const uint64_t qd = pr_desc(smem_addr(q_s) + i * kTileBytes, 16), kd = pr_desc(smem_addr(k_s), 16), vd = pr_desc(smem_addr(v_s), kPrRows * 128);
             const uint32_t s_at = tmem + i * 2 * kPrHalf, o_at = tmem + 4 * kPrHalf + i * 128;
-            // scores of half h; the tile's keys have been used with its last half
-            auto scores = [&](int h) {
-                const uint64_t k = kd + (uint32_t)((h >> 1 & 1) * (kTileBytes >> 4) + (h & 1) * (kPrHalf * 128 >> 4));
-                const uint32_t d = s_at + (h & 1) * kPrHalf;
-#pragma unroll
-                for (int s = 0; s < kHD / 16; s++) {
-                    const uint32_t off = (uint32_t)((s >> 2) * (kPrRows * 128) + (s & 3) * 32) >> 4;
-                    pr_mma_ss(d, qd + off, k + off, idesc_s, s > 0);
+            int g = 0, c0 = 0, c1 = 0, cs = 0, nq = 0;              // tiles, halves in either buffer, halves, items of two row tiles so far
+            for (int item = 0; ; item++) {
+                const PrItem w = item_at(item);
+                if (w.seq < 0) break;
+                const int halves = halves_of(w), n = (halves + 1) / 2, g0 = g;
+                g += n;
+                if (i > 0 && w.rows <= kPrRows) {                       // nothing to do with the item's keys and values
+                    for (int j = g0; j < g; j++) {
+                        wait(bars.k_full[j & 1], j >> 1);
+                        if (lane == 0) mbar_arrive(bar(bars.k_empty[j & 1]));
+                        wait(bars.v_full[j & 1], j >> 1);
+                        if (lane == 0) mbar_arrive(bar(bars.v_empty[j & 1]));
+                    }
+                    continue;
                 }
-                pr_commit(bar(bars.s_full[i][h & 1]));
-                if ((h & 1) || h + 1 == halves) pr_commit(bar(bars.k_empty[h >> 1 & 1]));
-            };
-            wait(bars.q_full, 0);
-            wait(bars.k_full[0], 0);
-            pr_fence_after();
-            __syncwarp();
-            if (pr_elect()) {
-                scores(0);
-                if (halves > 1) scores(1);
-            }
-            __syncwarp();
-#pragma unroll 1
-            for (int h = 0; h < halves; h++) {
-                const int b = h & 1, st = h >> 1 & 1;
-                if (b == 0) wait(bars.v_full[st], h >> 2);
-                wait(bars.p_full[i][b], h >> 1);
-                const bool more = h + 2 < halves;
-                if (more && b == 0) wait(bars.k_full[st ^ 1], (h + 2) >> 2);
+                // scores of half h; the tile's keys have been used with its last half
+                auto scores = [&](int h) {
+                    const uint64_t k = kd + (uint32_t)((g0 + (h >> 1) & 1) * (kTileBytes >> 4) + (h & 1) * (kPrHalf * 128 >> 4));
+                    const uint32_t d = s_at + (h & 1) * kPrHalf;
+#pragma unroll
+                    for (int s = 0; s < kHD / 16; s++) {
+                        const uint32_t off = (uint32_t)((s >> 2) * (kPrRows * 128) + (s & 3) * 32) >> 4;
+                        pr_mma_ss(d, qd + off, k + off, idesc_s, s > 0);
+                    }
+                    pr_commit(bar(bars.s_full[i][h & 1]));
+                    if ((h & 1) || h + 1 == halves) pr_commit(bar(bars.k_empty[g0 + (h >> 1) & 1]));
+                };
+                wait(bars.q_full[i], nq++);
+                wait(bars.k_full[g0 & 1], g0 >> 1);
                 pr_fence_after();
                 __syncwarp();
                 if (pr_elect()) {
-                    const uint64_t v = vd + (uint32_t)((st * kTileBytes + b * kPrHalf * 128) >> 4);
-                    const uint32_t p = s_at + b * kPrHalf;
-#pragma unroll
-                    for (int s = 0; s < kPrHalf / 16; s++)          // 16 positions: 8 columns of weights, 16 rows of values
-                        pr_mma_ts(o_at, p + 8 * s, v + (uint32_t)(s * 16 * 128 >> 4), idesc_o, h > 0 || s > 0);
-                    if (b == 1 || h + 1 == halves) pr_commit(bar(bars.v_empty[st]));
-                    pr_commit(bar(bars.sums_done[i]));
-                    if (h + 1 == halves) pr_commit(bar(bars.all_done[i]));
+                    scores(0);
+                    if (halves > 1) scores(1);
                 }
                 __syncwarp();
-                if (more) {                                         // in the weights' place, when they have been read
-                    wait(bars.sums_done[i], h);
+#pragma unroll 1
+                for (int h = 0; h < halves; h++) {
+                    const int b = h & 1, at = g0 + (h >> 1), st = at & 1;      // tile of all
+                    if (b == 0) wait(bars.v_full[st], at >> 1);
+                    wait(bars.p_full[i][b], (b ? c1 : c0) + (h >> 1));
+                    const bool more = h + 2 < halves;
+                    if (more && b == 0) wait(bars.k_full[st ^ 1], (at + 1) >> 1);
                     pr_fence_after();
                     __syncwarp();
-                    if (pr_elect()) scores(h + 2);
+                    if (pr_elect()) {
+                        const uint64_t v = vd + (uint32_t)((st * kTileBytes + b * kPrHalf * 128) >> 4);
+                        const uint32_t p = s_at + b * kPrHalf;
+#pragma unroll
+                        for (int s = 0; s < kPrHalf / 16; s++)          // 16 positions: 8 columns of weights, 16 rows of values
+                            pr_mma_ts(o_at, p + 8 * s, v + (uint32_t)(s * 16 * 128 >> 4), idesc_o, h > 0 || s > 0);
+                        if (b == 1 || h + 1 == halves) pr_commit(bar(bars.v_empty[st]));
+                        pr_commit(bar(bars.sums_done[i]));
+                        if (h + 1 == halves) pr_commit(bar(bars.all_done[i]));
+                    }
                     __syncwarp();
+                    if (more) {                                         // in the weights' place, when they have been read
+                        wait(bars.sums_done[i], cs + h);
+                        pr_fence_after();
+                        __syncwarp();
+                        if (pr_elect()) scores(h + 2);
+                        __syncwarp();
+                    }
                 }
+                c0 += (halves + 1) / 2; c1 += halves / 2; cs += halves;
+            }
+        } else if (warp == 14) {
+            // ---- the items: this CTA's, then those of CTAs that have not begun
+            int cta = (int)blockIdx.x;
+            for (int k = 0; ; k++) {
+                PrItem w = {-1};
+                while (cta >= 0 && w.seq < 0) {
+                    w = find(cta);
+                    if (w.seq >= 0) break;
+                    cta = take();                                   // more CTAs than tiles
+                }
+                if (k >= kPrItems) wait(bars.item_empty[k % kPrItems], k / kPrItems - 1);
+                if (lane == 0) { item_s[k % kPrItems] = w; mbar_arrive(bar(bars.item_full[k % kPrItems])); }
+                __syncwarp();
+                if (w.seq < 0 || *(volatile int*)&s_abort) break;
+                if (k > 0) ask(w);
+                wait(bars.more, k);
+                cta = take();
             }
         }
     }
