@@ -5,7 +5,7 @@
 // against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1172 us
 // (1007 TFLOP/s; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 225 us.
 //
-// An item is 256 rows of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
+// An item is 256 rows (128 where there are few) of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
 // products and softmax take turns, and the positions in tiles of 128.  The grid has a CTA for each; one that runs takes over, one
 // after the other, items of CTAs that have not begun (cluster launch control), so that the next item's keys are converted and
 // its rows of q on their way while this one ends (11 packed prompts 245 -> 226 us, 12 000 tokens 1184 -> 1173).  What is done
@@ -168,6 +168,7 @@ __device__ __forceinline__ uint64_t pr_desc(uint32_t at, uint32_t lead)
 
 struct PromptParams {
     PagedAttn a;
+    int item_rows;              // of an item: 256, or 128
     uint32_t gqa_mul;           // ceil(2^32 / query heads of a kv head), 0 for one: divides what is below 2^32 / that number
 };
 
@@ -556,7 +557,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             for (int s1 = C.num_seqs; s1 > 0 && seq < 0; s1 -= 32) {   // sequence s1 - 1 - lane
                 const int s = s1 - 1 - lane;
                 int a = 0, b = 0, n = 0;
-                if (s >= 0) { paged_rows(C, s, a, b); n = b > a ? (int)(((long long)(b - a) * gqa + kPrCtaRows - 1) / kPrCtaRows) : 0; }
+                if (s >= 0) { paged_rows(C, s, a, b); n = b > a ? (int)(((long long)(b - a) * gqa + P.item_rows - 1) / P.item_rows) : 0; }
                 int upto = n;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xFFFFFFFFu, upto, off); if (lane >= off) upto += o; }
@@ -571,7 +572,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             }
             PrItem w = {-1};
             if (seq >= 0) {
-                const int row0 = tile * kPrCtaRows, rows = min(kPrCtaRows, (hi - lo) * gqa - row0);
+                const int row0 = tile * P.item_rows, rows = min(P.item_rows, (hi - lo) * gqa - row0);
                 const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // token t sees min(before + t, room) positions
                 w = {seq, lo, row0, rows, kvh, before, room, max(0, min(before + token_of(row0 + rows - 1), room))};
             }
@@ -718,9 +719,16 @@ int paged_prompt_launch(const PagedAttn& A, void* stream, const char* who)
     if (hd != 64 && hd != 96 && hd != 128) return 1;
     // rows as far as the division by multiplication holds
     if ((long long)A.c.num_tokens * gqa + kPrCtaRows >= (1ll << 32) / gqa) return 1;
-    PromptParams P = {A, gqa == 1 ? 0u : (uint32_t)(((1ull << 32) + gqa - 1) / gqa)};
-    // every sequence's last tile may be a part of one
-    const long long tiles = (long long)A.c.num_tokens * gqa / kPrCtaRows + std::min(A.c.num_seqs, A.c.num_tokens), grid = tiles * A.c.n_head_kv;
+    PromptParams P = {A, kPrCtaRows, gqa == 1 ? 0u : (uint32_t)(((1ull << 32) + gqa - 1) / gqa)};
+    // items at most: every sequence's last one may be a part of one
+    auto items = [&](int rows) {
+        return std::min((long long)A.c.num_tokens * gqa / rows + std::min(A.c.num_seqs, A.c.num_tokens), A.c.num_seqs * (((long long)A.max_new * gqa + rows - 1) / rows)) * A.c.n_head_kv;
+    };
+    // So few that halves of them are all resident together: halves.  One prompt of 300 tokens (32/8 heads) 17.2 -> 15.3 us, of 512 20.8 ->
+    // 18.9, two of 256 behind 8000 149 -> 140; halves in the last round alone: three chunks of 2.3 rounds 250 -> 244, but one prompt
+    // of 4000 tokens 161 -> 170
+    if (2 * items(kPrCtaRows) <= sm_count()) P.item_rows = kPrRows;
+    const long long grid = items(P.item_rows);
     if (grid > 0x7FFFFFFF) return fail(S12_ERR_TOO_LARGE, "%s: %d tokens", who, A.c.num_tokens);
     return hd == 64 ? prompt_launch<64>(P, grid, stream, who) : hd == 96 ? prompt_launch<96>(P, grid, stream, who) : prompt_launch<128>(P, grid, stream, who);
 }
