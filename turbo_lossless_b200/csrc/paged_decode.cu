@@ -614,12 +614,13 @@ int paged_decode_launch(const PagedAttn& A, void* stream, const char* who)
     const int hd = A.c.head_dim, gqa = A.n_head / A.c.n_head_kv;
     const long long rows = (long long)gqa * A.max_new;
     if ((hd != 64 && hd != 96 && hd != 128) || rows > kDecMostRows) return 1;
-    // Groups of 16 rows read the cache anew, 256 rows of the other kernel share it, but without cutting the positions.  us here
-    // / there, 8 kv heads of 128: 64 sequences of 8000 positions with 16 rows 288 / 595, 32 rows 552 / 589, 64 rows 957 / 583; one
-    // sequence of 8000 with 128 rows 46 / 120, four 128 / 128, sixteen 529 / 149; one of 128 positions with 128 rows 8.1 / 9.8.
+    // Groups of 16 rows read the cache anew, 256 rows of the other kernel share it, but without cutting the positions: this one
+    // while all groups are resident together.  us here / there, 32/8 heads of 128: 128 tokens (256 groups) 9.1 / 11.5, 200 (400)
+    // 17.7 / 13.0, 128 behind 8000 77.5 / 82.6, 256 (512) behind 8000 211 / 117, 4 x 32 (256) behind 6000 100 / 106, 16 x 16 (512)
+    // behind 6000 189 / 123; and always with two groups to a sequence or one: 64 sequences of 8000, 32 rows, 552 / 589.
     const long long groups16 = (rows + 15) / 16 * A.c.num_seqs * A.c.n_head_kv;
     const int force = env_knob("S12_PAGED_FORCE", 0);              // 1: here, 2: there
-    if (force == 2 || (force == 0 && rows > 32 && groups16 > 192)) return 1;
+    if (force == 2 || (force == 0 && rows > 32 && groups16 > (long long)dec_ctas_per_sm(2) * sm_count())) return 1;
     const int64_t need = paged_decode_workspace_bytes(A.n_head, A.c.n_head_kv, A.c.num_seqs, A.max_new);
     if (!A.workspace || A.workspace_bytes < need || (reinterpret_cast<uintptr_t>(A.workspace) & 15))
         return fail(S12_ERR_BAD_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
