@@ -471,3 +471,35 @@ def test_many_prompts_of_all_lengths(monkeypatch, n_head, n_kv, hd):
     for _ in range(20):
         out, status = run_attention(c, 0.09)
         assert status == 0 and torch.equal(out, first)
+
+
+def test_many_prompts_in_dependent_launches(monkeypatch):
+    """CTAs that take over others' work, and launches that begin while they run."""
+    from turbo_lossless_b200 import Split12Engine
+    monkeypatch.setenv("S12_PAGED_FORCE", "2")
+    e = Split12Engine()
+    c = PO.Case([(i * 5 % 90, 1 + i * 29 % 150) for i in range(120)], 8, 4, 128, 32, seed=95)
+    ws = e.attention_paged_workspace(8, 4, 128, 120, c.max_new)
+    q_out, out = torch.zeros_like(c.q), torch.zeros(c.tokens, 8 * 128, dtype=torch.int16, device="cuda")
+
+    def step():
+        e.rope_store_kv_paged(c.q, c.k, c.v, *c.cache(), c.table, c.kv_len, c.q_start, 8, 10000.0, q_out=q_out)
+        e.attention_paged(q_out, *c.cache(), out, c.table, c.kv_len, c.q_start, 8, 0.1, c.max_new, c.max_len, ws)
+    step()
+    torch.cuda.synchronize()
+    old = e.set_dependent_launch(True)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(6):
+                step()
+    finally:
+        e.set_dependent_launch(old)
+    q_out.zero_()
+    out.zero_()
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert e.device_status() == 0
+    c.q = q_out
+    check(out, *PO.attention(c, 0.1))

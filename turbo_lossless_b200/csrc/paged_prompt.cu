@@ -137,6 +137,13 @@ __device__ __forceinline__ void pr_codes_f16(uint32_t w, uint32_t& lo, uint32_t&
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
 }
+// whether x is true in any of the four converter warps
+__device__ __forceinline__ bool pr_any(bool x)
+{
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)x) : "memory");
+    return any != 0;
+}
 // asks for the work of a CTA that has not begun; the answer's 16 bytes arrive at `at`, counted on `bar`
 __device__ __forceinline__ void pr_take_cta(uint32_t at, uint32_t bar)
 {
@@ -431,7 +438,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
         int g = 0;                                                  // tiles so far
         for (int item = 0; ; item++) {
             const PrItem w = item_at(item);
-            if (w.seq < 0) break;
+            if (pr_any(w.seq < 0)) break;                           // all four together, also where a wait gave up: they share a barrier
             const int halves = halves_of(w), n = (halves + 1) / 2, seen = w.seen, kvh = w.kvh;
             const int* table = C.table + (size_t)w.seq * C.table_stride;
             // the pools' row of position p, and whether there is one; -1 where the table has no page or no row sees p
@@ -676,7 +683,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 while (cta >= 0 && w.seq < 0) {
                     w = find(cta);
                     if (w.seq >= 0) break;
-                    cta = take();                                   // more CTAs than tiles
+                    cta = take();                                   // more CTAs than items
                 }
                 if (k >= kPrItems) wait(bars.item_empty[k % kPrItems], k / kPrItems - 1);
                 if (lane == 0) { item_s[k % kPrItems] = w; mbar_arrive(bar(bars.item_full[k % kPrItems])); }
@@ -724,8 +731,8 @@ int paged_prompt_launch(const PagedAttn& A, void* stream, const char* who)
     auto items = [&](int rows) {
         return std::min((long long)A.c.num_tokens * gqa / rows + std::min(A.c.num_seqs, A.c.num_tokens), A.c.num_seqs * (((long long)A.max_new * gqa + rows - 1) / rows)) * A.c.n_head_kv;
     };
-    // So few that halves of them are all resident together: halves.  One prompt of 300 tokens (32/8 heads) 17.2 -> 15.3 us, of 512 20.8 ->
-    // 18.9, two of 256 behind 8000 149 -> 140; halves in the last round alone: three chunks of 2.3 rounds 250 -> 244, but one prompt
+    // So few that halves of them are all resident together: halves.  One prompt of 300 tokens (32/8 heads) 17.2 -> 15.0 us, of 512 20.7 ->
+    // 18.2, two of 256 behind 8000 149 -> 138; halves in the last round alone: three chunks of 2.3 rounds 250 -> 244, but one prompt
     // of 4000 tokens 161 -> 170
     if (2 * items(kPrCtaRows) <= sm_count()) P.item_rows = kPrRows;
     const long long grid = items(P.item_rows);
