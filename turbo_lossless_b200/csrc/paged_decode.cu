@@ -13,7 +13,7 @@
 //             are the A operand of the second product as they lie, against V's rows in order
 //   dims      column n of PV tile j is dim n * head_dim / 8 + j: a lane reads consecutive bytes of each of eight rows
 //             and turns them by byte permutes
-// 24 sequences of 2-4 k positions (32/8 heads of 128) take 38.2 us (4.2 TB/s), 256 of 70-320 34 us (3.2 TB/s), two of 65 521
+// 24 sequences of 2-4 k positions (32/8 heads of 128) take 38.2 us (4.2 TB/s), 256 of 70-320 30.6 us (3.6 TB/s), two of 65 521
 // with one kv head 20.4 us, one of 256 5.2 us.
 // Work is cut by the device, which alone knows the lengths: the positions of a (sequence, kv head, rows) item go in equal
 // parts to teams of warps, as many as are resident together (dec_part_units).  The parts of an item leave their results in
@@ -179,7 +179,8 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
     grid_launch_dependents();
     grid_dependency_wait();
     const PagedArgs& C = P.a.c;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    // warp: the same in all lanes, for the compiler to see (256 sequences of 70-320 positions 33.9 -> 30.6 us)
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), g = lane >> 2, t4 = lane & 3;
     const int team = blockIdx.x * (kDecWarps / kTeam) + warp / kTeam, tw = warp % kTeam, tt = threadIdx.x % kTeamThreads;
     const int gqa = P.a.n_head / C.n_head_kv, per_seq = C.n_head_kv * P.row_groups;
 

@@ -2,14 +2,15 @@
 // (tcgen05.mma, scores, weights and sums in tensor memory), head_dim 64 / 96 / 128.
 //
 // Bound: the two products, 4 * head_dim FLOP per (row, position), and as much time of the exponentials: 16 a clock of an SM
-// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1172 us
-// (1007 TFLOP/s; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 225 us.
+// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1153 us
+// (1023 TFLOP/s; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 208 us.
 //
 // An item is 256 rows (128 where there are few) of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
 // products and softmax take turns, and the positions in tiles of 128.  The grid has a CTA for each; one that runs takes over, one
 // after the other, items of CTAs that have not begun (cluster launch control), so that the next item's keys are converted and
 // its rows of q on their way while this one ends (11 packed prompts 245 -> 226 us, 12 000 tokens 1184 -> 1173).  What is done
-// once an item is rolled up: the 32 rows of q of a warp in one piece of code cost 237 us for the former, in a loop of eights 226.
+// once an item is rolled up: the 32 rows of q of a warp in one piece of code cost 237 us for the former, in a loop of eights 226;
+// rows that are not there read the last one instead of zeros: 216 -> 208.
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row: scores from tensor memory, running maximum and sum,
 //                    weights back to tensor memory as f16 in the place of the scores; the output at the end
 //   warps 8-11       int8 codes from global memory to f16 in swizzled shared memory; the next tile's loads are in flight
@@ -198,7 +199,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     uint8_t* smem = pr_smem + ((1024u - (smem_addr(pr_smem) & 1023u)) & 1023u);
     uint8_t* q_s = smem, *k_s = smem + 2 * kTileBytes, *v_s = smem + 4 * kTileBytes;
     const PagedArgs& C = P.a.c;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the same in all lanes, for the compiler to see: a warp's addresses are computed once (226 -> 215 us, 1180 -> 1157)
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int gqa = P.a.n_head / C.n_head_kv;
     auto token_of = [&](int row) { return P.gqa_mul ? (int)__umulhi((uint32_t)row, P.gqa_mul) : row; };
     grid_launch_dependents();
@@ -256,7 +258,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             // ---- the warp's rows of q as f16, all of them in flight together, a lane four dims of each
             {
                 const float to_log2 = fabsf(P.a.scale) * 1.4426950408889634f;
-                const float* q0 = P.a.q + (size_t)w.lo * P.a.q_stride + (size_t)w.kvh * gqa * kHD + 4 * lane;
+                const float* q0 = P.a.q + (size_t)w.lo * P.a.q_stride + (size_t)w.kvh * gqa * kHD + 4 * (lane % (kHD / 4));
                 const bool in_row = 4 * lane < kHD;
                 auto row_of = [&](int r) {
                     const int t = token_of(row0 + r);
@@ -272,7 +274,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                     // largest of all, becomes a NaN
                     const bool fine = top - (27u << 23) < (228u << 23);
                     const float up = fine ? __uint_as_float((268u << 23) - top ^ (P.a.scale < 0.f ? 0x80000000u : 0u)) : 0.f;   // 2^(14 - e)
-                    if (in_row) *reinterpret_cast<uint2*>(tile_q + pr_chunk((warp & 3) * 32 + n, lane >> 1) + (lane & 1) * 8) = make_uint2(pr_f16x2(v.x * up, v.y * up), pr_f16x2(v.z * up, v.w * up));
+                    const Pair xy = mul2({v.x, v.y}, {up, up}), zw = mul2({v.z, v.w}, {up, up});
+                    if (in_row) *reinterpret_cast<uint2*>(tile_q + pr_chunk((warp & 3) * 32 + n, lane >> 1) + (lane & 1) * 8) = make_uint2(pr_f16x2(xy.x, xy.y), pr_f16x2(zw.x, zw.y));
                     if (lane == 0) factor_s[warp * 32 + n] = fine ? to_log2 * __uint_as_float(top - (14u << 23)) : 0.f;
                 };
                 if (((reinterpret_cast<uintptr_t>(P.a.q) & 15) | (P.a.q_stride & 3)) == 0) {
@@ -280,8 +283,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                     auto fetch = [&](float4 (&to)[8], int n) {
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
-                            to[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (warp * 32 + n + e < rows && in_row) to[e] = *reinterpret_cast<const float4*>(row_of(warp * 32 + n + e));
+                            to[e] = *reinterpret_cast<const float4*>(row_of(min(warp * 32 + n + e, rows - 1)));
                         }
                     };
                     fetch(v, 0);
@@ -300,8 +302,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 } else {
 #pragma unroll 1
                     for (int n = 0; n < 32; n++) {
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (warp * 32 + n < rows && in_row) { const float* q = row_of(warp * 32 + n); v = make_float4(q[0], q[1], q[2], q[3]); }
+                        const float* q = row_of(min(warp * 32 + n, rows - 1));
+                        const float4 v = make_float4(q[0], q[1], q[2], q[3]);
                         put(n, v, top_of(v));
                     }
                 }
