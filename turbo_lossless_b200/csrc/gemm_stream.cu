@@ -271,8 +271,10 @@ gemm_stream_kernel(const __grid_constant__ SMaps maps, const __grid_constant__ C
                 s[j] = *reinterpret_cast<const uint4*>(rs + sm_off + ro);
                 gq[j] = *reinterpret_cast<const uint2*>(rs + gr_off + ro);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(b_rawempty + 8 * sr);     // the stage's bytes are in registers
+            if (NB < 4) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_rawempty + 8 * sr);     // the stage's bytes are in registers
+            }
             if (!mbar_wait(b_xfull + 8 * sx, wx & 1, P.status, 0x40000u, &s_abort)) break;
             const uint8_t* xb = xs + (size_t)sx * kXStage;
 #pragma unroll
@@ -301,6 +303,10 @@ gemm_stream_kernel(const __grid_constant__ SMaps maps, const __grid_constant__ C
                         mma_bf16_16816(acc[mt][i], pa[0], pb[0], pa[1], pb[1], bq[i][0], bq[i][1]);
                         mma_bf16_16816(acc[mt][i], pa[2], pb[2], pa[3], pb[3], bq[i][2], bq[i][3]);
                     }
+                }
+                if (NB == 4 && h == 0) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b_rawempty + 8 * sr);     // the first half's products have used every load
                 }
             }
             __syncwarp();
