@@ -221,7 +221,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for this warp's loads; r is what they brought.  The compiler takes a load's registers for ready before the wait, so the wait
+// names them: no use of r can come before it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
 
 // ----------------------------------------------------------------------------
 // schedule shared by all roles: CTA c of G works on the contiguous range
@@ -434,7 +443,7 @@ __device__ __forceinline__ void drain_chunks(const GemmParams& P, const GemmTens
     for (int c0 = first * 32; c0 < BN; c0 += step * 32) {
         uint32_t v[32];
         tmem_ld32(tmem_acc + (uint32_t)c0, v);
-        tmem_ld_wait();
+        tmem_ld_wait(v);
         if (kind == kDrainContributor) {
             float* o = P.ws + blockIdx.x * slot + (size_t)c0 * kTileRows + mrow;
 #pragma unroll
@@ -504,7 +513,7 @@ __device__ __noinline__ void cluster_reduce(const GemmParams& P, uint8_t* smem, 
         for (int c = team; c < nch; c += kDrainTeams) {
             uint32_t v[32];
             tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(c * 32), v);
-            tmem_ld_wait();
+            tmem_ld_wait(v);
             float* dst = xbuf + (size_t)c * 32 * kTileRows + mrow;
 #pragma unroll
             for (int j = 0; j < 32; j++) dst[j * kTileRows] = __uint_as_float(v[j]);

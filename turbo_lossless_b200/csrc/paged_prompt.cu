@@ -85,15 +85,15 @@ __device__ __forceinline__ void pr_ld32(uint32_t at, float (&r)[32])
                    "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
                  : "r"(at) : "memory");
 }
-__device__ __forceinline__ void pr_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// After a wait: r is what the loads brought.  Between a load and this no branch may define r: the compiler takes the load's
-// registers for ready and might copy them.
-__device__ __forceinline__ void pr_ready(float (&r)[32])
+// Waits for this warp's loads; r is what one of them brought.  The compiler takes a load's registers for ready before the wait, so
+// the wait names them: no use of r can come before it.  Between the load and this no branch may define r either.
+__device__ __forceinline__ void pr_ld_wait(float (&r)[32])
 {
-    asm volatile("" : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
-                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
-                 "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
-                 "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                   "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                   "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+                   "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]) :: "memory");
 }
 __device__ __forceinline__ void pr_st32(uint32_t at, const uint32_t (&u)[32])
 {
@@ -325,9 +325,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 pr_fence_after();
                 pr_ld32(s_at + b * kPrHalf, x[0]);
                 pr_ld32(s_at + b * kPrHalf + 32, x[1]);
-                pr_ld_wait();
-                pr_ready(x[0]);
-                pr_ready(x[1]);
+                pr_ld_wait(x[0]);
+                pr_ld_wait(x[1]);                                   // nothing is left to wait for: names the registers
                 const float2 unit = unit_s2[j];
                 const float fac = fmaxf(factor * unit.x, 1e-37f);   // above 0: a masked score stays -infinity
                 const int left = limit - h * kPrHalf;               // positions of the half that the row sees
@@ -357,7 +356,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                         for (int c = 0; c < kHD; c += 32) {
                             float o[32];
                             pr_ld32(o_at + c, o);
-                            pr_ld_wait();
+                            pr_ld_wait(o);
                             uint32_t u[32];
 #pragma unroll
                             for (int d = 0; d < 32; d++) u[d] = __float_as_uint(o[d] * (f * shift));
@@ -397,8 +396,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             for (int c = 0; c < kHD; c += 32) {
                 float o[32];
                 pr_ld32(o_at + c, o);
-                pr_ld_wait();
-                pr_ready(o);
+                pr_ld_wait(o);
 #pragma unroll
                 for (int d = 0; d < 32; d += 8)
                     *reinterpret_cast<uint4*>(chunk_at(lane, (c + d) / 8)) =
