@@ -1,0 +1,55 @@
+"""Stages of a ring that bulk copies fill: a warp that has read one gives it back with the fence between the proxies, since an arrive
+alone does not order its reads before the copy that overwrites them (found with 17 to 32 sequences: 21 of 3000 calls differed)."""
+import os
+import re
+
+import pytest
+import torch
+
+CSRC = os.path.join(os.path.dirname(__file__), "..", "turbo_lossless_b200", "csrc")
+
+
+def source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return f.read()
+
+
+def test_giving_back_fences_the_reads():
+    body = re.search(r"void mbar_give_back\(uint32_t bar\)\s*\{(.*?)\n\}", source("common.cuh"), re.S).group(1)
+    assert re.search(r"fence\.proxy\.async\.shared::cta.*__syncwarp\(\).*mbar_arrive\(bar\)", body, re.S)
+
+
+@pytest.mark.parametrize("name,rings", [("gemm_stream.cu", ["b_rawempty", "b_xempty"])])
+def test_stages_are_given_back_with_the_fence(name, rings):
+    text = source(name)
+    for ring in rings:
+        assert f"mbar_wait({ring}" in text and f"mbar_give_back({ring}" in text
+        assert f"mbar_arrive({ring}" not in text
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,B,stages,calls", [(4096, 4096, 32, 2, 4000), (4096, 4096, 17, 2, 2000), (4096, 4096, 16, 2, 4000),
+                                                (4096, 4096, 8, 2, 4000), (14336, 4096, 16, 3, 2000), (14336, 4096, 8, 3, 2000)])
+def test_small_batches_repeat_their_bits(monkeypatch, O, M, K, B, stages, calls):
+    """With two stages the copies follow the reads most closely."""
+    from gpu_util import assert_close, dev
+    from turbo_lossless_b200 import CompressedWeight, Split12Engine
+    monkeypatch.setenv("S12_GSTREAM", "2")
+    monkeypatch.setenv("S12_GSTREAM_MAXB", "32")
+    monkeypatch.setenv("S12_GSTREAM_STAGES", str(stages))
+    eng = Split12Engine()
+    w, x = O.synth_weights(M, K, M + B, outlier_frac=2e-3), O.synth_acts(B, K, B)
+    cw, xd = CompressedWeight.from_packed(O.pack(w)), dev(x)
+    call = eng.gemv_batched if B <= 16 else eng.gemm
+    first = torch.zeros(B, M, device="cuda")
+    call(cw, xd, first, K, M, B)
+    torch.cuda.synchronize()
+    assert_close(first, O.gemm_exact(w, x), what=f"B={B}")
+    out, differ = torch.zeros_like(first), torch.zeros((), dtype=torch.int64, device="cuda")
+    flush = torch.empty(48 << 20, device="cuda")
+    for i in range(calls):
+        if i % 4 == 0:
+            flush.fill_(i)                                            # the weights come from memory, then from L2
+        call(cw, xd, out, K, M, B)
+        differ += (out != first).any()
+    assert int(differ) == 0 and eng.device_status() == 0

@@ -168,6 +168,15 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// A warp gives a ring's stage back to the producer whose next bulk copy overwrites it.  The lanes' reads are ordinary accesses, the
+// copy is made by the async proxy: an arrive alone orders only what ordinary accesses do, so that the copy may overwrite what a
+// read that was issued long before has not fetched yet.  The fence between the two proxies puts the reads in front of it.
+__device__ __forceinline__ void mbar_give_back(uint32_t bar)
+{
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");

@@ -21,8 +21,9 @@
 //     16-byte and one 8-byte shared load per row, decode8 in registers, and the
 //     result IS the A fragment of mma.sync.m16n8k16 (the pairing (e0,e4),(e1,e5)...
 //     of decode8 is matched by permuting the B fragment, which is cheaper: one
-//     permute serves four rows).  The raw stage is released as soon as its bytes
-//     are in registers, so the ring's whole capacity is in flight.
+//     permute serves four rows).  The raw stage is given back as soon as its bytes
+//     are in registers (mbar_give_back: the next copy waits for the reads
+//     themselves), so the ring's whole capacity is in flight.
 //     MMA row g of a tile stands for tile row bitrev3(g): the two rows of an 8-lane
 //     load phase then differ in bit 2 of the swizzle and the four rows of a 16-lane
 //     phase in bits 1-2, which makes both loads free of bank conflicts.
@@ -271,10 +272,7 @@ gemm_stream_kernel(const __grid_constant__ SMaps maps, const __grid_constant__ C
                 s[j] = *reinterpret_cast<const uint4*>(rs + sm_off + ro);
                 gq[j] = *reinterpret_cast<const uint2*>(rs + gr_off + ro);
             }
-            if (NB < 4) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b_rawempty + 8 * sr);     // the stage's bytes are in registers
-            }
+            mbar_give_back(b_rawempty + 8 * sr);                     // the stage's bytes are in registers
             if (!mbar_wait(b_xfull + 8 * sx, wx & 1, P.status, 0x40000u, &s_abort)) break;
             const uint8_t* xb = xs + (size_t)sx * kXStage;
 #pragma unroll
@@ -304,13 +302,8 @@ gemm_stream_kernel(const __grid_constant__ SMaps maps, const __grid_constant__ C
                         mma_bf16_16816(acc[mt][i], pa[2], pb[2], pa[3], pb[3], bq[i][2], bq[i][3]);
                     }
                 }
-                if (NB == 4 && h == 0) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(b_rawempty + 8 * sr);     // the first half's products have used every load
-                }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(b_xempty + 8 * sx);
+            mbar_give_back(b_xempty + 8 * sx);
             if (++sr == P.raw_stages) { sr = 0; wr++; }
             if (++sx == kSXStages) { sx = 0; wx++; }
             const bool seg_end = kb + 1 == KB || it + 1 == hi;
