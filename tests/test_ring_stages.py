@@ -19,7 +19,7 @@ def test_giving_back_fences_the_reads():
     assert re.search(r"fence\.proxy\.async\.shared::cta.*__syncwarp\(\).*mbar_arrive\(bar\)", body, re.S)
 
 
-@pytest.mark.parametrize("name,rings", [("gemm_stream.cu", ["b_rawempty", "b_xempty"])])
+@pytest.mark.parametrize("name,rings", [("gemm_stream.cu", ["b_rawempty", "b_xempty"]), ("gemv_stream.cu", ["bar_empty"]), ("gemm_tc.cu", ["b_rawempty"])])
 def test_stages_are_given_back_with_the_fence(name, rings):
     text = source(name)
     for ring in rings:
@@ -51,5 +51,28 @@ def test_small_batches_repeat_their_bits(monkeypatch, O, M, K, B, stages, calls)
         if i % 4 == 0:
             flush.fill_(i)                                            # the weights come from memory, then from L2
         call(cw, xd, out, K, M, B)
+        differ += (out != first).any()
+    assert int(differ) == 0 and eng.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,B,calls", [(4096, 4096, 1, 4000), (14336, 4096, 1, 2000), (14336, 4096, 48, 1000), (4096, 4096, 256, 1000)])
+def test_single_sequences_and_large_batches_repeat_their_bits(O, M, K, B, calls):
+    from turbo_lossless_b200 import CompressedWeight, Split12Engine
+    from gpu_util import assert_close, dev
+    eng = Split12Engine()
+    w, x = O.synth_weights(M, K, M + B, outlier_frac=2e-3), O.synth_acts(B, K, B)
+    cw, xd = CompressedWeight.from_packed(O.pack(w)), dev(x)
+    first, out = torch.zeros(B, M, device="cuda"), torch.zeros(B, M, device="cuda")
+    call = (lambda o: eng.gemv([cw], xd, [o])) if B == 1 else (lambda o: eng.gemm(cw, xd, o, K, M, B))
+    call(first)
+    torch.cuda.synchronize()
+    few = min(B, 16)
+    assert_close(first[:few], O.gemm_exact(w, x[:few]), what=f"B={B}")
+    differ, flush = torch.zeros((), dtype=torch.int64, device="cuda"), torch.empty(48 << 20, device="cuda")
+    for i in range(calls):
+        if i % 4 == 0:
+            flush.fill_(i)
+        call(out)
         differ += (out != first).any()
     assert int(differ) == 0 and eng.device_status() == 0

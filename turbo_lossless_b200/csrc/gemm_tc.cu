@@ -717,8 +717,7 @@ gemm_tc_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ CU
             if (P.neg_base == 0) decode_row<0>(raw + sr * kRawBytes, t, gi, T.base2, P.mul, v);
             else if (P.neg_base == 1) decode_row<1>(raw + sr * kRawBytes, t, gi, T.base2, P.mul, v);
             else decode_row<3>(raw + sr * kRawBytes, t, gi, T.base2, P.mul, v);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(b_rawempty + 8 * sr);      // this warp has read its share of the stage
+            mbar_give_back(b_rawempty + 8 * sr);                  // this warp has read its share of the stage
             esc_apply(esc, T, kb * kBigK + gi * kTK, v);
             if (wo > 0) mbar_wait(b_free + 8 * gi, (wo - 1) & 1, P.status, 0x400u, &s_abort);
             __syncwarp();                                         // lanes with escapes took another way

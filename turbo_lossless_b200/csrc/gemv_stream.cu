@@ -291,8 +291,7 @@ gemv_stream_kernel(const __grid_constant__ StreamParams P)
             uint4 xq[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) xq[j] = xp[j * 4];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_empty + 8 * s);   // stage data is in registers
+            mbar_give_back(bar_empty + 8 * s);               // stage data is in registers
 
             // first / second run as loaded: for an odd chunk that is high / low, and its activations are staged likewise
             const uint4 a0 = af, a1 = as, b0v = bf, b1v = bs;
