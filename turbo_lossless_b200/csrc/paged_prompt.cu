@@ -2,8 +2,8 @@
 // (tcgen05.mma, scores, weights and sums in tensor memory), head_dim 64 / 96 / 128.
 //
 // Bound: the two products, 4 * head_dim FLOP per (row, position), and as much time of the exponentials: 16 a clock of an SM
-// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1153 us
-// (1023 TFLOP/s; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 208 us.
+// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1152 us
+// (1024 TFLOP/s; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 217 us.
 //
 // An item is 256 rows (128 where there are few) of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
 // products and softmax take turns, and the positions in tiles of 128.  The grid has a CTA for each; one that runs takes over, one
@@ -24,8 +24,13 @@
 // tile, rounded once (the scale goes in as two f16 numbers); multiplying the scores by the scales instead took a tenth of the
 // softmax's time.  A weight is at most 2^15: 2^7 times its distance from the row's maximum, which follows the scores
 // only when they exceed it by 2^8, since the sums have to be multiplied then.  A V operand is code * scale / 2^E with one E
-// for all: what the largest scale so far asks for, and six binary orders of room; when that is not enough the sums are
-// multiplied, too.  Sums are 32-bit.
+// for all, after the largest scale so far; when that grows the sums are multiplied, too.  Sums are 32-bit.
+// That holds while the scales of an item's values, and those of a tile's keys, lie in two neighbouring ranges of eight binary orders:
+// a row must not lose what it sees to the scale of a position that it does not see, or whose weight is nothing.  From the first
+// tile on that breaks it ("wide") an item's operands are the codes themselves, exact; the softmax multiplies the scores by the
+// keys' scales and the weights by the values', and a row has a power of two of its own, after the largest such product that it
+// sees (pr_wide_halves; an item takes about twice as long).  As a function: as a second loop in its place it cost the first
+// one 3 % (three chunks 244 -> 253 us).
 // A position that a row may not see gets weight 0, and its value must be finite for that: values behind the sequence's end
 // are zeros, and one whose scale is not finite is zero with its K scale made NaN, which marks the rows that see it.
 #include "paged.cuh"
@@ -145,6 +150,26 @@ __device__ __forceinline__ bool pr_any(bool x)
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)x) : "memory");
     return any != 0;
 }
+// Binary orders of scales, eight to a bit: bit i stands for [2^(8 i - 127), 2^(8 i - 119)).  A unit that takes them below 2^8:
+__device__ __forceinline__ int pr_unit(uint32_t orders) { return max(8 * (31 - __clz(orders)) - 127, -110); }
+// whether there are more than the largest order's bit and the next, or any too small for that unit
+__device__ __forceinline__ bool pr_wide(uint32_t orders)
+{
+    return (orders & (((0x40000000u >> __clz(orders | 1u)) - 1u) | 3u)) != 0;
+}
+__device__ __forceinline__ float pr_over_1(float power) { return __uint_as_float(0x7F000000u - __float_as_uint(power)); }   // of a power of two
+struct PrUnits { float key, value, shift; bool wide; };
+// What the scales of a tile's keys and of an item's values are multiplied by, from their orders; `before` and `old` are the values' orders and
+// multiplier before this tile.  shift: 2^(E before - E), or, where the item becomes wide here, -zu for the unit that the sums are in
+__device__ __forceinline__ PrUnits pr_units(uint32_t before, float old, uint32_t orders_k, uint32_t orders_v)
+{
+    PrUnits u = {1.f, 1.f, 1.f, (before & 1u) || pr_wide(orders_k) || pr_wide(orders_v)};
+    if (u.wide) { if (!(before & 1u)) u.shift = before ? -65536.f * old : -1.f; return u; }
+    u.key = __uint_as_float((uint32_t)(127 - pr_unit(orders_k)) << 23);
+    u.value = __uint_as_float((uint32_t)(127 - pr_unit(orders_v)) << 23);
+    u.shift = u.value / old;
+    return u;
+}
 // asks for the work of a CTA that has not begun; the answer's 16 bytes arrive at `at`, counted on `bar`
 __device__ __forceinline__ void pr_take_cta(uint32_t at, uint32_t bar)
 {
@@ -174,6 +199,97 @@ __device__ __forceinline__ uint64_t pr_desc(uint32_t at, uint32_t lead)
     return (uint64_t)((at >> 4) & 0x3FFF) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+// The halves of a wide item from h on, for a row of the softmax: the operands are codes, their scales come in here.  Seldom, so that they
+// are read from the cache again, a lane those of two positions.  m, sum: the row's maximum and sum so far.  Returns the sum and zu:
+// the row's unit is 2^16 / zu.
+template <int kHD>
+__device__ __noinline__ float2 pr_wide_halves(const PagedArgs& C, PrBars& bars, int* s_abort, const uint8_t (&absent_s)[kPrScaleStages][4], const float2 (&unit_s2)[kPrScaleStages], const PrItem w,
+                                              int i, int h, int halves, int g0, int c0, int c1, int cs, uint32_t s_at, uint32_t o_at, int limit, float factor, float m, float sum)
+{
+    const int lane = threadIdx.x & 31;
+    auto bar = [](const uint64_t& b) { return smem_addr(&b); };
+    auto wait = [&](const uint64_t& b, int phase) { mbar_wait(smem_addr(&b), (uint32_t)phase & 1, C.status, kPrSite, s_abort); };
+    float zu = 0.f, zt = 0.f;                                   // the row's unit is 2^16 / zu; its largest weighted value so far over 2^16
+#pragma unroll 1
+    for (; h < halves; h++) {
+        const int j = (g0 + (h >> 1)) % kPrScaleStages, b = h & 1;
+        float sk[2], sv[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int t = h * kPrHalf + c * 32 + lane, page = t < w.seen ? paged_page(C, w.seq, t) : -1;
+            const size_t at = ((size_t)max(page, 0) * C.n_head_kv + w.kvh) << C.page_shift | (size_t)(t & ((1 << C.page_shift) - 1));
+            sk[c] = page < 0 ? 0.f : C.sk[at];
+            sv[c] = page < 0 ? 0.f : C.sv[at] * (1.f / 65536.f);
+            if (!(fabsf(sv[c]) < INFINITY)) { sk[c] = __uint_as_float(0x7FC00000u); sv[c] = 0.f; }
+            if (!(fabsf(sk[c]) < INFINITY)) sk[c] = __uint_as_float(0x7FC00000u);   // an infinity, too
+        }
+        float x[2][32];
+        wait(bars.s_full[i][b], (b ? c1 : c0) + (h >> 1));
+        pr_fence_after();
+        pr_ld32(s_at + b * kPrHalf, x[0]);
+        pr_ld32(s_at + b * kPrHalf + 32, x[1]);
+        pr_ld_wait(x[0]);
+        pr_ld_wait(x[1]);
+        const int left = limit - h * kPrHalf;
+        const uint32_t absent = *reinterpret_cast<const uint16_t*>(&absent_s[j][2 * b]);
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kPrHalf; c++) {
+            float& y = x[c / 32][c % 32];
+            y *= factor * __shfl_sync(0xFFFFFFFFu, sk[c / 32], c % 32);
+            if (c >= left || (absent >> (c / 32 * 8 + c / 16 % 2) & 1)) y = -INFINITY;
+            top = fmaxf(top, y);
+        }
+        const float mn = top - m > kPrSlack ? top : m, f = pr_exp2(m - mn);
+        m = mn;
+        sum *= f;
+        if (zu == 0.f) {                                    // the sums so far are in this unit
+            zu = -unit_s2[j].y;
+            zt = sum > 0.f ? 8.f / zu : 0.f;                    // about: 2^-1 to 2^23 over zu
+        }
+        float z = 0.f;
+#pragma unroll
+        for (int c = 0; c < kPrHalf; c++) {
+            float& y = x[c / 32][c % 32];
+            y = pr_exp2(__fsub_rn(y, m) + kPrLift);
+            sum += y;
+            y *= __shfl_sync(0xFFFFFFFFu, sv[c / 32], c % 32);
+            z = fmaxf(z, fabsf(y));
+        }
+        zt = fmaxf(zt * f, z);
+        const bool turn = zt > 0.f && !(zt * zu >= 64.f && zt * zu <= 32768.f);
+        const int e_old = (int)(__float_as_uint(zu) >> 23), e_new = turn ? min(max(264 - (int)(__float_as_uint(zt) >> 23), 1), 254) : e_old;
+        if (__any_sync(0xFFFFFFFFu, f != 1.f || turn)) {
+            if (h > 0) {
+                const int by = e_new - e_old;               // in two steps: each is a float
+                const float f0 = f * __uint_as_float((uint32_t)(127 + by / 2) << 23), f1 = __uint_as_float((uint32_t)(127 + by - by / 2) << 23);
+                wait(bars.sums_done[i], cs + h - 1);
+                pr_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < kHD; c += 32) {
+                    float o[32];
+                    pr_ld32(o_at + c, o);
+                    pr_ld_wait(o);
+                    uint32_t u[32];
+#pragma unroll
+                    for (int d = 0; d < 32; d++) u[d] = __float_as_uint(o[d] * f0 * f1);
+                    pr_st32(o_at + c, u);
+                }
+            }
+            zu = __uint_as_float((uint32_t)e_new << 23);
+        }
+        uint32_t p[32];
+#pragma unroll
+        for (int c = 0; c < 32; c++) p[c] = pr_f16x2(x[c / 16][2 * c % 32] * zu, x[c / 16][2 * c % 32 + 1] * zu);
+        pr_st32(s_at + b * kPrHalf, p);
+        pr_st_wait();
+        pr_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(bars.p_full[i][b]));
+    }
+    return make_float2(sum, zu);
+}
+
 struct PromptParams {
     PagedAttn a;
     int item_rows;              // of an item: 256, or 128
@@ -187,8 +303,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
     constexpr int kTileBytes = pr_tile_bytes(kHD), kPieces = kHD / 16;
     extern __shared__ __align__(16) uint8_t pr_smem[];
     __shared__ PrBars bars;
-    __shared__ __align__(8) float2 unit_s2[kPrScaleStages];        // of a tile: the power of two of its keys, 2^(E before - E) of its values
-    __shared__ uint2 top_s[2][4];                                  // the converters' largest scales of a tile
+    // of a tile: the power of two of its keys; 2^(E before - E) of its values, or, where the item becomes wide, less the first zu (pr_wide_halves)
+    __shared__ __align__(8) float2 unit_s2[kPrScaleStages];
+    __shared__ uint2 orders_s[2][4];                               // the converters' binary orders of a tile's scales: keys, values
     __shared__ float unit_s[2 * kPrItems];                         // of an item: 2^E at the end; four items may be read ahead of one
     __shared__ __align__(16) PrItem item_s[kPrItems];
     __shared__ __align__(16) uint4 taken_s;
@@ -317,8 +434,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             const float factor = factor_s[r];
             float m = kPrLowest;
             Pair l = {0.f, 0.f};
+            int h = 0;
 #pragma unroll 1
-            for (int h = 0; h < halves; h++) {
+            for (; h < halves; h++) {
                 const int j = (g0 + (h >> 1)) % kPrScaleStages, b = h & 1;
                 float x[2][32];
                 wait(bars.s_full[i][b], (b ? c1 : c0) + (h >> 1));                    // then half h - 2 is in the sums
@@ -346,6 +464,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 const bool rise = top - m > kPrSlack;
                 const float shift = b == 0 ? unit.y : 1.f;
                 if (__any_sync(0xFFFFFFFFu, rise) || shift != 1.f) {
+                    if (shift < 0.f) break;                         // from here on the item is wide
                     const float mn = rise ? top : m, f = pr_exp2(m - mn);
                     m = mn;
                     l = mul2(l, {f, f});
@@ -385,10 +504,16 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(bars.p_full[i][b]));
             }
+            float zu = 0.f;                                         // wide: the row's unit is 2^16 / zu
+            if (h < halves) {
+                const float2 rest = pr_wide_halves<kHD>(C, bars, &s_abort, absent_s, unit_s2, w, i, h, halves, g0, c0, c1, cs, s_at, o_at, limit, factor, m, l.x + l.y);
+                l = {rest.x, 0.f};
+                zu = rest.y;
+            }
             // ---- the output
             wait(bars.all_done[i], done++);                          // a wait tells odd from even only: of sums_done's phases two may be ahead
             pr_fence_after();
-            const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : unit_s[item % (2 * kPrItems)] / sum;   // no position at all: zeros
+            const float sum = l.x + l.y, rd = sum == 0.f ? 0.f : zu != 0.f ? 65536.f / sum / zu : unit_s[item % (2 * kPrItems)] / sum;   // no position at all: zeros
             // A row as one piece: by way of shared memory, in the place of the warp's rows of q, which have been read
             constexpr int kChunks = kHD / 8;
             auto chunk_at = [&](int row, int c) { return tile_q + pr_chunk((warp & 3) * 32 + row, c); };
@@ -471,28 +596,32 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             fetch_scales(row);
             fetch(k, k_at, row);
             fetch(v, v_at, row);
-            int E = 0;
+            uint32_t orders_k = 0, orders_v = 0;                    // of the last tile's keys, and of the item's values so far
+            float unit_k = 0.f, unit_v = 0.f;                       // what these scales are multiplied by
+            // Binary orders of the tile's scales, eight to a bit: bit i for [2^(8 i - 127), 2^(8 i - 119)); zeros and what is not finite have none
+            auto note_orders = [&](int st) {
+                const uint32_t bits_k = __float_as_uint(sk) & 0x7FFFFFFFu, bits_v = __float_as_uint(sv) & 0x7FFFFFFFu;
+                const uint32_t mine_k = __reduce_or_sync(0xFFFFFFFFu, bits_k - 1 < 0x7F7FFFFFu ? 1u << (bits_k >> 26) : 0u);
+                const uint32_t mine_v = __reduce_or_sync(0xFFFFFFFFu, bits_v - 1 < 0x7F7FFFFFu ? 1u << (bits_v >> 26) : 0u);
+                if (lane == 0) orders_s[st][cw] = make_uint2(mine_k, mine_v);
+            };
+            note_orders(g & 1);
             for (int j = 0; j < n; j++, g++) {
                 const int st = g & 1;
                 if (j == max(n - 2, 0) && mine == 0) mbar_arrive(bar(bars.more));   // the item after this one may be looked for
                 const bool absent = row < 0;
-                // the values' unit 2^E
-                const uint32_t bits_k = __float_as_uint(sk) & 0x7FFFFFFFu, bits = __float_as_uint(sv) & 0x7FFFFFFFu;
-                const bool fine = bits < 0x7F800000u;
-                const uint32_t top_k = __reduce_max_sync(0xFFFFFFFFu, bits_k < 0x7F800000u ? bits_k : 0u), top_v = __reduce_max_sync(0xFFFFFFFFu, fine ? bits : 0u);
-                if (lane == 0) top_s[st][cw] = make_uint2(top_k, top_v);
                 named_bar_sync(1, 128);
-                const uint2 w0 = top_s[st][0], w1 = top_s[st][1], w2 = top_s[st][2], w3 = top_s[st][3];
-                const int e_top = (int)(max(max(w0.y, w1.y), max(w2.y, w3.y)) >> 23) - 126;   // scales are below 2^e_top
-                const int e_key = min(max((int)(max(max(w0.x, w1.x), max(w2.x, w3.x)) >> 23) - 126 - 8, -100), 100);   // keys below 2^15
+                const uint2 w0 = orders_s[st][0], w1 = orders_s[st][1], w2 = orders_s[st][2], w3 = orders_s[st][3];
+                const uint32_t now_k = w0.x | w1.x | w2.x | w3.x, now_v = orders_v | w0.y | w1.y | w2.y | w3.y;
                 float shift = 1.f;
-                if (j == 0 || e_top > E + 8) {
-                    const int old = E;
-                    E = max(e_top - 2, -120);
-                    if (j > 0) shift = old - E < -126 ? 0.f : __uint_as_float((uint32_t)(127 + old - E) << 23);
+                if (j == 0 || now_k != orders_k || now_v != orders_v) {   // seldom
+                    const PrUnits u = pr_units(j == 0 ? 0u : orders_v, unit_v, now_k, now_v);
+                    unit_k = u.key; unit_v = u.value; shift = j == 0 && u.shift > 0.f ? 1.f : u.shift;
+                    orders_k = now_k; orders_v = u.wide ? now_v | 1u : now_v;
                 }
-                const float unit = __uint_as_float((uint32_t)(127 - E) << 23);   // 2^-E
-                const float key_scale = (fine ? sk : __uint_as_float(0x7FC00000u)) * __uint_as_float((uint32_t)(127 - e_key) << 23);
+                const bool fine = (__float_as_uint(sv) & 0x7FFFFFFFu) < 0x7F800000u;
+                if (orders_v & 1u) sk = sv = 1.f;                   // wide: the codes themselves
+                const float key_scale = (fine ? sk : __uint_as_float(0x7FC00000u)) * unit_k;
                 const uint32_t key_hi = pr_f16x2(key_scale, 0.f) & 0xFFFFu;       // the scale as a sum of two f16
                 float key_hi_f;
                 asm("{\n\t.reg .b16 h, z;\n\tmov.b32 {h, z}, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(key_hi_f) : "r"(key_hi));
@@ -502,8 +631,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 const uint32_t gone = __ballot_sync(0xFFFFFFFFu, absent);   // a whole half, or rows that nobody sees
                 if (lane == 0) absent_s[g % kPrScaleStages][cw] = (uint8_t)((gone & 1u) | (gone >> 16 & 1u) << 1);
                 if (mine == 0) {
-                    unit_s2[g % kPrScaleStages] = make_float2(__uint_as_float((uint32_t)(127 + e_key) << 23), shift);
-                    if (j == n - 1) unit_s[item % (2 * kPrItems)] = __uint_as_float((uint32_t)(127 + E) << 23);
+                    unit_s2[g % kPrScaleStages] = make_float2(pr_over_1(unit_k), shift);
+                    if (j == n - 1) unit_s[item % (2 * kPrItems)] = pr_over_1(unit_v);
                 }
 #pragma unroll
                 for (int it = 0; it < kIts; it++) {
@@ -526,7 +655,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(bars.k_full[st]));
-                const float scale = fine ? sv * unit : 0.f;
+                const float scale = fine ? sv * unit_v : 0.f;
                 const uint32_t scale2 = pr_f16x2(scale, scale);
                 const long long row_next2 = j + 2 < n ? row_at((j + 2) * kPrTile + mine) : -1;
                 if (j + 1 < n) { fetch_scales(row_next); fetch(k, k_at, row_next); }
@@ -549,7 +678,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(bars.v_full[st]));
-                if (j + 1 < n) fetch(v, v_at, row_next);
+                if (j + 1 < n) { fetch(v, v_at, row_next); note_orders(st ^ 1); }
                 row = row_next; row_next = row_next2;
             }
         }
