@@ -7,6 +7,7 @@ decodes all sequences side by side.  Device work is launches of the CUDA library
 """
 from __future__ import annotations
 
+import contextlib
 import heapq
 from typing import Dict, List, Optional, Sequence
 
@@ -26,7 +27,8 @@ class PagedKVCache:
 
     ``kv_k`` / ``kv_v`` int8 [layer][page][kv head][position][head_dim], ``scale_k`` / ``scale_v`` fp32 without the last;
     ``block_table`` int32 [max_seqs][max_pages] and ``kv_len`` int32 [max_seqs] on the device follow the host's lists after
-    every call, in place, so that a captured graph may read them.  Calls are ordered on the current stream.
+    every call, in place, so that a captured graph may read them.  Calls are ordered on the current stream.  A call that raises
+    leaves everything as it was.
     """
 
     def __init__(self, n_layer: int, num_pages: int, n_head_kv: int, head_dim: int, page_size: int = 64, max_seqs: int = 8,
@@ -83,6 +85,36 @@ class PagedKVCache:
         self.block_table.copy_(self._table)                           # from pageable memory: read before the call returns
         self.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
 
+    def _follow(self) -> None:
+        """After a failure: the device's arrays follow the lists, or do so with the next call that gets through."""
+        with contextlib.suppress(Exception):
+            self._upload()
+
+    @contextlib.contextmanager
+    def _or_as_before(self):
+        """The lists go back to what they were when the block raises."""
+        before = list(self._free), list(self._users), {seq: list(pages) for seq, pages in self._pages.items()}, dict(self._len)
+        try:
+            yield
+        except BaseException:
+            self._free, self._users, self._pages, self._len = before
+            self._follow()
+            raise
+
+    def _shorten(self, lens: Dict[int, int]) -> None:
+        """Sequences back to the lengths they had: the pages behind are free again.  As ``_or_as_before``, of these sequences alone."""
+        for seq, n in lens.items():
+            pages = self._pages[seq]
+            while len(pages) > -(-n // self.page_size):
+                self._drop(pages.pop())
+            self._len[seq] = n
+        self._follow()
+
+    def _drop(self, page: int) -> None:
+        self._users[page] -= 1
+        if self._users[page] == 0:
+            heapq.heappush(self._free, page)
+
     def _copy(self, src: Sequence[int], dst: Sequence[int]) -> None:
         if not src:
             return
@@ -101,8 +133,9 @@ class PagedKVCache:
     def add(self) -> int:
         """A new, empty sequence: its row in ``block_table`` and ``kv_len``."""
         seq = self._slot()
-        self._pages[seq], self._len[seq] = [], 0
-        self._upload()
+        with self._or_as_before():
+            self._pages[seq], self._len[seq] = [], 0
+            self._upload()
         return seq
 
     def extend(self, new: Dict[int, int]) -> None:
@@ -117,10 +150,16 @@ class PagedKVCache:
             need[seq] = pages - len(self._pages[seq])
         if sum(need.values()) > len(self._free):
             raise PagedCacheFull(f"{sum(need.values())} pages needed, {len(self._free)} free")
-        for seq, n in new.items():
-            self._pages[seq] += [self._take() for _ in range(need[seq])]
-            self._len[seq] += n
-        self._upload()
+        before = {seq: self._len[seq] for seq in new}
+        try:
+            for seq, n in new.items():
+                for _ in range(need[seq]):
+                    self._pages[seq].append(self._take())
+                self._len[seq] += n
+            self._upload()
+        except BaseException:
+            self._shorten(before)
+            raise
 
     def fork(self, seq: int) -> int:
         """A new sequence with the same positions: full pages are shared (nobody writes them again), a last page with room
@@ -130,24 +169,24 @@ class PagedKVCache:
         full = n // self.page_size
         if len(pages) > full and not self._free:
             raise PagedCacheFull("a fork needs one free page")
-        mine = pages[:full]
-        for page in mine:
-            self._users[page] += 1
-        if len(pages) > full:
-            mine.append(self._take())
-            self._copy([pages[full]], [mine[full]])
-        self._pages[child], self._len[child] = mine, n
-        self._upload()
+        with self._or_as_before():
+            mine = pages[:full]
+            for page in mine:
+                self._users[page] += 1
+            if len(pages) > full:
+                mine.append(self._take())
+                self._copy([pages[full]], [mine[full]])
+            self._pages[child], self._len[child] = mine, n
+            self._upload()
         return child
 
     def release(self, seq: int) -> None:
         """Ends a sequence; pages that no other sequence holds are free again."""
-        for page in self._pages.pop(seq):
-            self._users[page] -= 1
-            if self._users[page] == 0:
-                heapq.heappush(self._free, page)
-        del self._len[seq]
-        self._upload()
+        with self._or_as_before():
+            for page in self._pages.pop(seq):
+                self._drop(page)
+            del self._len[seq]
+            self._upload()
 
     def compact(self) -> int:
         """Moves pages so that those in use are the pool's first ones; returns how many were moved."""
@@ -156,20 +195,22 @@ class PagedKVCache:
         moved = [p for p in range(used, self.num_pages) if self._users[p]]
         if not moved:
             return 0
-        self._copy(moved, holes)
-        to = dict(zip(moved, holes))
-        for a, b in to.items():
-            self._users[b], self._users[a] = self._users[a], 0
-        for pages in self._pages.values():
-            pages[:] = [to.get(p, p) for p in pages]
-        self._free = list(range(used, self.num_pages))
-        self._upload()
+        with self._or_as_before():
+            self._copy(moved, holes)
+            to = dict(zip(moved, holes))
+            for a, b in to.items():
+                self._users[b], self._users[a] = self._users[a], 0
+            for pages in self._pages.values():
+                pages[:] = [to.get(p, p) for p in pages]
+            self._free = list(range(used, self.num_pages))
+            self._upload()
         return len(moved)
 
 
 class PagedDecoder:
     """A decoder (weights as for ``Decoder``) over a ``PagedKVCache``: ``prefill`` runs packed prompts or chunks in one
-    pass, ``step`` one token of every given sequence.  ``max_tokens`` bounds the tokens of a call."""
+    pass, ``step`` one token of every given sequence.  ``max_tokens`` bounds the tokens of a call.  A call that raises leaves
+    the sequences as they were."""
 
     def __init__(self, cfg: DecoderConfig, layers: List[Dict[str, CompressedWeight]], lm_head: CompressedWeight, token_embd: torch.Tensor,
                  norms: Dict[str, torch.Tensor], max_tokens: int, max_seqs: int = 8, num_pages: Optional[int] = None, page_size: int = 64,
@@ -205,19 +246,27 @@ class PagedDecoder:
 
     def _forward(self, seqs: List[int], tokens: List[List[int]]) -> torch.Tensor:
         """Logits [len(seqs)][vocabulary] after the last of each sequence's new tokens (the decoder's own buffer)."""
-        c, e = self.cfg, self.eng
         new = [len(t) for t in tokens]
         rows, S = sum(new), len(seqs)
         if len(new) != S or len(set(seqs)) != S or S == 0 or min(new) < 1 or rows > self.max_tokens:
             raise ValueError(f"needs distinct sequences with at least a token each, {self.max_tokens} tokens at most")
-        self.cache.extend(dict(zip(seqs, new)))
-        dev, hd, scale = self.token_embd.device, c.head_dim, 1.0 / float(c.head_dim) ** 0.5
+        dev, before = self.token_embd.device, {s: self.cache.length(s) for s in seqs}
         starts = [0]
         for n in new:
             starts.append(starts[-1] + n)
         # what the host knows of this call, in one copy
         host = torch.tensor([t for ts in tokens for t in ts] + starts + [s - 1 for s in starts[1:]] + [S] + list(seqs), dtype=torch.int32)
         meta = host.to(dev)
+        self.cache.extend(dict(zip(seqs, new)))
+        try:
+            return self._run(seqs, new, meta)
+        except BaseException:
+            self.cache._shorten(before)
+            raise
+
+    def _run(self, seqs: List[int], new: List[int], meta: torch.Tensor) -> torch.Tensor:
+        c, e, rows, S = self.cfg, self.eng, sum(new), len(seqs)
+        hd, scale = c.head_dim, 1.0 / float(c.head_dim) ** 0.5
         ids, q_start, ends, count = meta[:rows], meta[rows:rows + S + 1], meta[rows + S + 1:rows + 2 * S + 1], meta[rows + 2 * S + 1:rows + 2 * S + 2]
         order = meta[rows + 2 * S + 2:].long()
         table, kv_len = self.cache.block_table[order], self.cache.kv_len[order]
@@ -254,15 +303,9 @@ class PagedDecoder:
         ones go on (the next chunk of a long prompt).  ``logits[i]`` / ``next_tokens[i]`` then belong to prompt i."""
         seqs = list(seqs) if seqs is not None else None
         if seqs is None:
-            seqs, made = [], []
-            try:
-                for _ in prompts:
-                    made.append(self.cache.add())
+            with self.cache._or_as_before():
+                made = [self.cache.add() for _ in prompts]
                 self._forward(made, [list(p) for p in prompts])
-            except (PagedCacheFull, ValueError):
-                for s in made:
-                    self.cache.release(s)
-                raise
             return made
         self._forward(seqs, [list(p) for p in prompts])
         return seqs
