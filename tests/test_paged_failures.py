@@ -130,3 +130,12 @@ def test_uploads_that_fail(decoder, monkeypatch):
     c.add()
     c.extend({b: 1})
     assert c.kv_len[b] == 21
+
+
+@pytest.mark.parametrize("n_embd,n_head,n_kv", [(18, 4, 2), (100, 3, 1)])
+def test_heads_that_do_not_fill_the_embedding_are_refused(n_embd, n_head, n_kv):
+    """The o projection would read columns that the attention does not write, as ``Decoder`` says, too."""
+    from turbo_lossless_b200 import DecoderConfig, PagedDecoder
+    cfg = DecoderConfig(n_embd=n_embd, n_head=n_head, n_head_kv=n_kv, n_ff=8, n_vocab=10, n_layer=1, max_seq=64)
+    with pytest.raises(ValueError, match="n_embd"):
+        PagedDecoder(cfg, [], None, torch.zeros(10, n_embd, dtype=torch.int16), {}, max_tokens=8, max_seqs=2, eng=Engine())

@@ -216,6 +216,8 @@ class PagedDecoder:
                  norms: Dict[str, torch.Tensor], max_tokens: int, max_seqs: int = 8, num_pages: Optional[int] = None, page_size: int = 64,
                  eng: Optional[Split12Engine] = None):
         self.cfg, self.layers, self.lm_head, self.token_embd, self.norms = cfg, layers, lm_head, token_embd, norms
+        if cfg.n_head * cfg.head_dim != cfg.n_embd:
+            raise ValueError(f"the attention output feeds the o projection: {cfg.n_head} heads of {cfg.head_dim} are not n_embd {cfg.n_embd}")
         self.eng = eng or Split12Engine()
         self.max_tokens = max(max_tokens, max_seqs)
         dev, n, hd, T = token_embd.device, cfg.n_embd, cfg.head_dim, self.max_tokens
