@@ -509,7 +509,8 @@ int s12_rope_store_kv_paged_async(const float* q, int q_stride, const float* k, 
  * multiple of n_head_kv): out[row][head] = sum_j softmax_j(scale * q . k_j) v_j
  * over the positions j up to the row's own; bf16 [num_tokens][out_stride].
  * Rows without a position (kv_len below the token's) give 0.  Positions whose
- * page the table does not have count as masked and set bit 0x100000.
+ * page the table does not have (an entry outside [0, num_pages), a position past
+ * table_pages and below max_len) count as masked and set bit 0x100000.
  * workspace: s12_attention_paged_workspace_bytes of device memory, 16-byte
  * aligned, zero before its first use; a call leaves it fit for the next.  Calls
  * that may overlap on the GPU need workspaces of their own. */

@@ -257,7 +257,7 @@ paged_attention_general_kernel(const __grid_constant__ PagedAttn P)
         for (int e = 0; e < 4; e++) { qv[c][e] = live[c] ? q[c * 128 + lane * 4 + e] * P.scale : 0.f; acc[c][e] = 0.f; }
     }
     float m = -INFINITY, l = 0.f;
-    bool bad = false;
+    bool bad = paged_past_table(C, own);
     for (int t = warp; t < n; t += kGenWarps) {
         const int page = paged_page(C, seq, t);
         if (page < 0) { bad = true; continue; }

@@ -38,6 +38,8 @@ __device__ __forceinline__ int paged_len(const PagedArgs& P, int s)
     const long long room = min((long long)P.table_pages << P.page_shift, (long long)P.max_len);
     return n < 0 ? 0 : n < room ? n : (int)room;
 }
+// whether a row that sees n positions, by its place, needs pages past the table's end
+__device__ __forceinline__ bool paged_past_table(const PagedArgs& P, int n) { return min(n, P.max_len) > (long long)P.table_pages << P.page_shift; }
 // rows [lo, hi) of the packed tokens that belong to sequence s
 __device__ __forceinline__ void paged_rows(const PagedArgs& P, int s, int& lo, int& hi)
 {

@@ -247,7 +247,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams P)
             const int room = paged_len(C, seq), before = C.kv_len[seq] - (hi - lo) + 1;   // row r sees min(before + token, room) positions
             const int least = min(before + token_of(row_base), room), most_seen = min(before + token_of(row_base + rows - 1), room);
             const int t_hi = kTeam == 1 || P.whole ? most_seen : (int)min((long long)((unsigned long long)units * (part + 1) / parts) * kUnit, (long long)most_seen);
-            bool missing = false;
+            bool missing = paged_past_table(C, before + token_of(row_base + rows - 1));
             // the page of position t, whose table entry was read; -1: none, or t not below t_hi
             auto page_of = [&](int entry, int t) {
                 if (t >= t_hi) return -1;

@@ -566,6 +566,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams P)
             if (pr_any(w.seq < 0)) break;                           // all four together, also where a wait gave up: they share a barrier
             const int halves = halves_of(w), n = (halves + 1) / 2, seen = w.seen, kvh = w.kvh;
             const int* table = C.table + (size_t)w.seq * C.table_stride;
+            if (paged_past_table(C, w.before + token_of(w.row0 + w.rows - 1))) missing = true;
             // the pools' row of position p, and whether there is one; -1 where the table has no page or no row sees p
             auto row_at = [&](int p) {
                 if (p >= seen) return -1ll;
