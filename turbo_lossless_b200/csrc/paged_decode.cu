@@ -599,7 +599,7 @@ static int decode_launch_hd(DecodeParams P, int tiles, void* stream, const char*
 {
     const PagedAttn& A = P.a;
     const long long items = (long long)A.c.num_seqs * A.c.n_head_kv * P.row_groups;
-    P.min_units = env_knob("S12_PAGED_MIN_UNITS", 2);
+    P.min_units = std::max(1, env_knob("S12_PAGED_MIN_UNITS", 2));
     if (tiles == 2) return decode_launch<kHD, 2, kDecWarps>(P, stream, who);
     // us with one / four warps, sequences of half of these lengths to all: 8 kv heads of 128, 64 sequences of 128 positions
     // 8.0 / 9.4, 320 15.8 / 15.6, 500 27.6 / 21.8; 256 of 500 57 / 60, 700 81 / 73; 800 of 900 237 / 255; 2 kv heads of 64, 100
