@@ -2,8 +2,8 @@
 // (tcgen05.mma, scores, weights and sums in tensor memory), head_dim 64 / 96 / 128.
 //
 // Bound: the two products, 4 * head_dim FLOP per (row, position), and as much time of the exponentials: 16 a clock of an SM
-// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1152 us
-// (1024 TFLOP/s; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 217 us.
+// against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1145 us
+// (1030 TFLOP/s in bursts, 896 in long runs; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 217 us.
 //
 // An item is 256 rows (128 where there are few) of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
 // products and softmax take turns, and the positions in tiles of 128.  The grid has a CTA for each; one that runs takes over, one
