@@ -511,7 +511,7 @@ int s12_rope_store_kv_paged_async(const float* q, int q_stride, const float* k, 
  * Sums are 32-bit.  With heads of 64, 96 and 128 the factors have fewer bits: q 15 of
  * its row's largest element and a weight times its value's scale 15 of the largest
  * of 32 neighbours; with many rows to a sequence q, k, weights and values 11 each.
- * q and values below 1e-30 in size may count as zero there.
+ * q and scales of values below 1e-30 may count as zero there.
  * Rows without a position (kv_len below the token's) give 0.  Positions whose
  * page the table does not have (an entry outside [0, num_pages), a position past
  * table_pages and below max_len) count as masked and set bit 0x100000.
