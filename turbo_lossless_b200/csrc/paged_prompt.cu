@@ -3,7 +3,7 @@
 //
 // Bound: the two products, 4 * head_dim FLOP per (row, position), and as much time of the exponentials: 16 a clock of an SM
 // against 128 x 128 x head_dim x 2 FLOP in 2 * head_dim clocks of its tensor cores.  32/8 heads of 128: 12 000 tokens 1145 us
-// (1030 TFLOP/s in bursts, 896 in long runs; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 217 us.
+// (1030 TFLOP/s in bursts, 896 in long runs; the softmax warps issue half of the time, their waits are the rest), 11 packed prompts of 41-1900 tokens 218 us.
 //
 // An item is 256 rows (128 where there are few) of one (sequence, kv head): row = (new token, query head of the group), two tiles of 128 whose
 // products and softmax take turns, and the positions in tiles of 128.  The grid has a CTA for each; one that runs takes over, one
@@ -167,7 +167,7 @@ __device__ __forceinline__ PrUnits pr_units(uint32_t before, float old, uint32_t
     if (u.wide) { if (!(before & 1u)) u.shift = before ? -65536.f * old : -1.f; return u; }
     u.key = __uint_as_float((uint32_t)(127 - pr_unit(orders_k)) << 23);
     u.value = __uint_as_float((uint32_t)(127 - pr_unit(orders_v)) << 23);
-    u.shift = u.value / old;
+    u.shift = u.value * pr_over_1(old);
     return u;
 }
 // asks for the work of a CTA that has not begun; the answer's 16 bytes arrive at `at`, counted on `bar`
